@@ -247,6 +247,84 @@ int qflash_fwd_fused_noalloc(const void* q, const void* k, const void* v, int dt
  */
 int qflash_fused_noalloc_status(const void* q, void* stream, int64_t* status);
 
+/*
+ * A key/value cache in 4 bits.  All buffers are the caller's, contiguous, on one
+ * device:
+ *   k_codes, v_codes  [Z, H, capacity, D / 2] bytes: element 2i of a vector in the
+ *                     low half of byte i, element 2i + 1 in the high half; 16-byte aligned
+ *   k_param, v_param  [Z, H, capacity, 2] bf16: scale and zero point (a whole number
+ *                     0..15) of each vector, which stands for scale * (code - zero)
+ *   weight            [Z, H, capacity] fp32: attention weight added up per position
+ *   lens              [Z] int32: stored tokens of each sequence
+ *   ctl               [2] int32, zero at first: a ticket of qflash_kv4_append, and a
+ *                     status word (bit 0: tokens outside [0, capacity) were dropped)
+ * D is 64 or 128, capacity at most 2^24.  Values of lens outside [0, capacity] are
+ * read as the nearer end.  The calls are asynchronous on `stream`; calls that write
+ * a cache must be ordered with all others on it, by one stream or by events.
+ * No counterpart in the reference, whose attention has neither a cache nor a
+ * single-token form.
+ */
+typedef struct qflash_kv4_cache {
+  void* k_codes;
+  void* v_codes;
+  void* k_param;
+  void* v_param;
+  float* weight;
+  int32_t* lens;
+  int32_t* ctl;
+  int32_t Z, H, capacity, D;
+} qflash_kv4_cache;
+
+/*
+ * Quantises keys and values [Z, H, N, D] (dtype 0 fp32, 1 fp16, 2 bf16; strides in
+ * elements, innermost 1) into the cache.  Row i of sequence z goes to position
+ * at[z] + i (NULL: lens[z] + i) for i < new_lens[z] (NULL: N; clamped to [0, N]);
+ * its weight becomes 0 and lens[z] becomes at[z] + new_lens[z].  Tokens outside
+ * [0, capacity) are dropped, lens stops at capacity, and bit 0 of ctl[1] is set.
+ *   lo = min(x, 0), hi = max(x, 0), scale = bf16(fp32((hi - lo) / 15)),
+ *   zero = clamp(rint(-lo / scale), 0, 15), code = clamp(rint(x / scale) + zero, 0, 15)
+ * with fp32 quotients.  A vector with an infinity or a NaN gets scale NaN.
+ */
+int qflash_kv4_append(const qflash_kv4_cache* cache, const void* k, const void* v, int dtype,
+                      const int64_t k_strides[4], const int64_t v_strides[4], int N, const int32_t* new_lens,
+                      const int32_t* at, void* stream);
+
+/*
+ * The values of positions start[z] + i (NULL: i), i < N, as contiguous [Z, H, N, D]
+ * tensors of `dtype`; zeros where nothing is stored.
+ */
+int qflash_kv4_read(const qflash_kv4_cache* cache, void* k, void* v, int dtype, int N, const int32_t* start,
+                    void* stream);
+
+/*
+ * out = softmax(scale * q . k) v over the stored tokens, for queries [Z, Hq, N, D]
+ * (dtype 1 fp16 or 2 bf16; out of the same type; strides in elements, innermost 1).
+ * Query head h reads key/value head h / (Hq / H); Hq / H is at most 64.  The rows
+ * i < new_lens[z] (NULL: N) are the sequence's last tokens: with `causal`, row i sees
+ * the positions up to lens[z] - new_lens[z] + i, else all lens[z].  Rows that see
+ * nothing, and rows i >= new_lens[z], are written as zeros.
+ * With weights_in ([Z, H, capacity] fp32; it may be cache->weight), cache->weight of
+ * every stored position j becomes weights_in[j] + the sum over rows and query heads
+ * of the probability that position j received.
+ * `workspace` holds qflash_kv4_attend_workspace(...) bytes, 16-byte aligned, for this
+ * call alone until it has run.
+ */
+int qflash_kv4_attend(const qflash_kv4_cache* cache, const void* q, int dtype, const int64_t q_strides[4], void* out,
+                      const int64_t out_strides[4], int Hq, int N, const int32_t* new_lens, double scale, int causal,
+                      const float* weights_in, void* workspace, size_t workspace_bytes, void* stream);
+size_t qflash_kv4_attend_workspace(const qflash_kv4_cache* cache, int dtype, int Hq, int N, int weights);
+
+/*
+ * Packs into `to` (same Z, H and D, no shared memory, capacity >= budget) what stays
+ * of `from`: sequences of at most `budget` tokens whole, of longer ones the last
+ * `recent` tokens and, per head, the heaviest of the others (by weight; of equal ones
+ * the first, NaN counts as heaviest), in order, with their weights.  to->lens becomes
+ * min(lens, budget); kept [Z, H, budget] gets the positions in `from`, -1 behind the
+ * last.  Positions of `to` behind the last token stay as they were.
+ */
+int qflash_kv4_evict(const qflash_kv4_cache* from, const qflash_kv4_cache* to, int budget, int recent, int32_t* kept,
+                     void* stream);
+
 /* Reads and clears the device-side error word the kernels set when a bounded
  * wait gives up (0 = none).  Synchronises the stream. */
 int qflash_device_error(void* stream, uint32_t* out);

@@ -23,6 +23,15 @@ ERRORS = {-1: "QFLASH_ERR_ARG", -2: "QFLASH_ERR_ALIGN", -3: "QFLASH_ERR_TMA", -4
 
 # name -> (restype, argtypes); every symbol the header declares
 _I64x4 = ctypes.POINTER(ctypes.c_int64)
+
+
+class KV4CacheStruct(ctypes.Structure):
+    """qflash_kv4_cache."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k_codes", "v_codes", "k_param", "v_param", "weight", "lens", "ctl")] + [
+        (n, ctypes.c_int32) for n in ("Z", "H", "capacity", "D")]
+
+
+_KV4 = ctypes.POINTER(KV4CacheStruct)
 SIGNATURES = {
     "qflash_i8_fwd": (ctypes.c_int, [
         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
@@ -77,6 +86,18 @@ SIGNATURES = {
         ctypes.c_uint32, ctypes.c_void_p]),
     "qflash_fused_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     "qflash_fused_status": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.POINTER(ctypes.c_int64)]),
+    "qflash_kv4_append": (ctypes.c_int, [
+        _KV4, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, _I64x4, _I64x4, ctypes.c_int, ctypes.c_void_p,
+        ctypes.c_void_p, ctypes.c_void_p]),
+    "qflash_kv4_read": (ctypes.c_int, [
+        _KV4, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p]),
+    "qflash_kv4_attend": (ctypes.c_int, [
+        _KV4, ctypes.c_void_p, ctypes.c_int, _I64x4, ctypes.c_void_p, _I64x4, ctypes.c_int, ctypes.c_int,
+        ctypes.c_void_p, ctypes.c_double, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
+        ctypes.c_void_p]),
+    "qflash_kv4_attend_workspace": (ctypes.c_size_t, [_KV4, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "qflash_kv4_evict": (ctypes.c_int, [
+        _KV4, _KV4, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p]),
     "qflash_device_error": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint32)]),
     "qflash_launch_count": (ctypes.c_uint64, []),
     "qflash_last_grid": (ctypes.c_int, []),
@@ -236,6 +257,50 @@ def fwd_fused_window(q, k, v, table, index, window_mask, num_windows, q8, k8, v8
                                      _strides(out), Z, H, N, D, scale_log2e, l_shift, acc_shift, flags,
                                      workspace.data_ptr(), workspace.numel(), stream)
     _check(rc, "qflash_fwd_fused_window")
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+_KV4_DTYPE = {}  # torch dtype -> DTYPES' number, filled on first use (this module does not import torch)
+
+
+def _kv4_dtype(t) -> int:
+    n = _KV4_DTYPE.get(t.dtype)
+    if n is None:
+        n = _KV4_DTYPE[t.dtype] = DTYPES[str(t.dtype)]
+    return n
+
+
+def kv4_append(cache, k, v, new_lens, at, stream) -> None:
+    """Launch qflash_kv4_append; no synchronisation."""
+    _check(load().qflash_kv4_append(cache, k.data_ptr(), v.data_ptr(), _kv4_dtype(k), _strides(k), _strides(v),
+                                    k.shape[2], _ptr(new_lens), _ptr(at), stream), "qflash_kv4_append")
+
+
+def kv4_read(cache, k, v, count, start, stream) -> None:
+    """Launch qflash_kv4_read; no synchronisation."""
+    _check(load().qflash_kv4_read(cache, k.data_ptr(), v.data_ptr(), _kv4_dtype(k), count, _ptr(start), stream),
+           "qflash_kv4_read")
+
+
+def kv4_attend(cache, q, out, new_lens, scale, causal, weights_in, stream) -> None:
+    """Launch qflash_kv4_attend with a workspace of its own; no synchronisation."""
+    import torch
+    lib = load()
+    _, Hq, N, _ = q.shape
+    dtype = _kv4_dtype(q)
+    ws = torch.empty(lib.qflash_kv4_attend_workspace(cache, dtype, Hq, N, weights_in is not None), dtype=torch.uint8,
+                     device=q.device)
+    _check(lib.qflash_kv4_attend(cache, q.data_ptr(), dtype, _strides(q), out.data_ptr(), _strides(out), Hq, N,
+                                 _ptr(new_lens), scale, causal, _ptr(weights_in), ws.data_ptr(), ws.numel(), stream),
+           "qflash_kv4_attend")
+
+
+def kv4_evict(cache, to, budget, recent, kept, stream) -> None:
+    """Launch qflash_kv4_evict; no synchronisation."""
+    _check(load().qflash_kv4_evict(cache, to, budget, recent, kept.data_ptr(), stream), "qflash_kv4_evict")
 
 
 def fused_workspace_bytes(mask_zb: int, mask_hb: int, N: int) -> int:

@@ -1,0 +1,120 @@
+// Shared by the kernels of the 4-bit key/value cache: its layout, the stored
+// parameters and the element types at the boundary.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+
+#include "../../include/qflash_b200.h"
+#include "qfb_internal.h"
+
+namespace qfb {
+namespace kv4 {
+
+// A cache's buffers, all contiguous:
+//   codes  [Z, H, C, D / 2] bytes, element 2i of a vector in the low half of byte i
+//   param  [Z, H, C, 2] bf16: scale, zero point (a whole number 0..15)
+//   weight [Z, H, C] fp32, lens [Z] int32, ctl [2] int32 (ticket, status)
+struct Cache {
+  uint8_t* codes[2];    // keys, values
+  uint32_t* param[2];   // one 32-bit word per vector: scale in the low half, zero point in the high half
+  float* weight;
+  int32_t* lens;
+  int32_t* ctl;
+  int Z, H, C, D;
+};
+
+inline Cache view(const qflash_kv4_cache* c) {
+  return {{(uint8_t*)c->k_codes, (uint8_t*)c->v_codes}, {(uint32_t*)c->k_param, (uint32_t*)c->v_param},
+          c->weight, c->lens, c->ctl, c->Z, c->H, c->capacity, c->D};
+}
+
+__device__ __forceinline__ float param_scale(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float param_zero(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// Stored tokens of sequence z, whatever the buffer holds: never outside [0, C].
+__device__ __forceinline__ int length_of(const Cache& c, int z) { return min(max(c.lens[z], 0), c.C); }
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <class T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// 8 elements of one thread, as one or two 16-byte transfers where `vec` says
+// that every row starts on a 16-byte boundary, else one by one.
+template <class T>
+__device__ __forceinline__ void load8(const T* p, bool vec, float (&x)[8]) {
+  alignas(16) T r[8];
+  if (vec) {
+    uint4* w = reinterpret_cast<uint4*>(r);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = p[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = to_float(r[i]);
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, bool vec, const float (&x)[8]) {
+  alignas(16) T r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = from_float<T>(x[i]);
+  if (vec) {
+    const uint4* w = reinterpret_cast<const uint4*>(r);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = r[i];
+  }
+}
+
+int check_cache(const qflash_kv4_cache* c, const char* what);
+int check_launch(const char* what, unsigned grid);
+
+// Attention of `ntok` tokens from token tok0 on; see qflash_kv4_attend.
+struct AttendArgs {
+  Cache c;
+  const void* q;
+  void* out;
+  int64_t qs[3], os[3];  // strides of (sequence, head, token) in elements
+  int rep, N;            // query heads per key/value head, rows of the query tensor
+  const int32_t* new_lens;
+  int causal;
+  float scale_log2e;
+  const float* weights_in;  // null: no weights are accumulated
+  int tok0, ntok;
+};
+
+// The rows of one sequence that a launch over tokens [tok0, tok0 + ntok) takes,
+// and how many stored tokens they see at most.
+struct Span {
+  int len, fresh;  // stored tokens; rows of the query tensor that the sequence brings
+  __device__ __forceinline__ int limit(const AttendArgs& a, int i) const {  // positions that token i sees
+    return i >= fresh ? 0 : a.causal ? max(0, len - fresh + i + 1) : len;
+  }
+  __device__ __forceinline__ int most(const AttendArgs& a) const {
+    return a.tok0 >= fresh ? 0 : limit(a, min(fresh, a.tok0 + a.ntok) - 1);
+  }
+};
+__device__ __forceinline__ Span span_of(const AttendArgs& a, int z) {
+  return {length_of(a.c, z), a.new_lens ? min(max(a.new_lens[z], 0), a.N) : a.N};
+}
+
+size_t rows_workspace(const qflash_kv4_cache* c, int Hq, int N, bool weights);
+int attend_rows(const AttendArgs& a, bool fp16, void* ws, int dev, cudaStream_t s);
+
+}  // namespace kv4
+}  // namespace qfb

@@ -39,6 +39,7 @@ struct WindowBiasSpec {
 };
 
 int set_err(int code, const char* fmt, ...);
+void note_launch(int grid);  // counts a kernel launch (qflash_launch_count, qflash_last_grid)
 
 // Restores the calling thread's current device when it goes out of scope: the
 // entry points make the device that owns the data current for their launches

@@ -1127,6 +1127,11 @@ static thread_local std::string t_err;
 static std::atomic<uint64_t> g_launches{0};
 static std::atomic<int> g_last_grid{0};
 
+void note_launch(int grid) {
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  g_last_grid.store(grid, std::memory_order_relaxed);
+}
+
 int set_err(int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;
@@ -1273,8 +1278,7 @@ static int launch(int dev, const CUtensorMap& mq, const CUtensorMap& mk, const C
   kern<<<grid, C::THREADS, C::SMEM, stream>>>(mq, mk, mv, mb, kb);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_err(QFLASH_ERR_LAUNCH, "launch: %s", cudaGetErrorString(e));
-  g_launches.fetch_add(1, std::memory_order_relaxed);
-  g_last_grid.store(grid, std::memory_order_relaxed);
+  note_launch(grid);
   return QFLASH_OK;
 }
 
