@@ -257,7 +257,8 @@ int qflash_fused_noalloc_status(const void* q, void* stream, int64_t* status);
  *   weight            [Z, H, capacity] fp32: attention weight added up per position
  *   lens              [Z] int32: stored tokens of each sequence
  *   ctl               [2] int32, zero at first: a ticket of qflash_kv4_append, and a
- *                     status word (bit 0: tokens outside [0, capacity) were dropped)
+ *                     status word (bit 0: tokens outside [0, capacity) were dropped;
+ *                     bit 1: a bounded wait inside a kernel gave up)
  * D is 64 or 128, capacity at most 2^24.  Values of lens outside [0, capacity] are
  * read as the nearer end.  The calls are asynchronous on `stream`; calls that write
  * a cache must be ordered with all others on it, by one stream or by events.

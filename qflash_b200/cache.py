@@ -165,9 +165,14 @@ class KV4Cache:
 
     def check(self) -> None:
         """Raise OverflowError if an append since the last check dropped tokens
-        outside [0, capacity).  Synchronises."""
-        if self._ctl[1].item() & 1:
+        outside [0, capacity), QFlashError if a wait inside a kernel gave up
+        (its output is then not valid).  Synchronises."""
+        status = int(self._ctl[1].item())
+        if status:
             self._ctl[1] = 0
+        if status & 2:
+            raise _lib.QFlashError("a bounded wait inside an attention kernel gave up")
+        if status & 1:
             raise OverflowError(f"tokens outside the cache's {self.shape[2]} positions were dropped")
 
     def _counts(self, name, t):

@@ -389,9 +389,16 @@ static int check_attend(const qflash_kv4_cache* cache, int dtype, int Hq, int N)
   return QFLASH_OK;
 }
 
+// Rows of a head from which the kernel for many rows is used.
+static bool many_rows(const qflash_kv4_cache* c, int Hq, int N) { return (long long)Hq / c->H * N > 64; }
+
+static size_t attend_workspace(const qflash_kv4_cache* c, int Hq, int N, bool weights) {
+  return many_rows(c, Hq, N) ? prompt_workspace(c, Hq, N, weights) : rows_workspace(c, Hq, N, weights);
+}
+
 extern "C" size_t qflash_kv4_attend_workspace(const qflash_kv4_cache* cache, int dtype, int Hq, int N, int weights) {
   if (check_attend(cache, dtype, Hq, N) || cache->Z == 0 || N == 0) return 0;
-  return rows_workspace(cache, Hq, N, weights != 0);
+  return attend_workspace(cache, Hq, N, weights != 0);
 }
 
 extern "C" int qflash_kv4_attend(const qflash_kv4_cache* cache, const void* q, int dtype, const int64_t q_strides[4],
@@ -403,7 +410,7 @@ extern "C" int qflash_kv4_attend(const qflash_kv4_cache* cache, const void* q, i
   if (cache->Z == 0 || N == 0) return QFLASH_OK;
   if (!q || !out || !q_strides || !out_strides) return set_err(QFLASH_ERR_ARG, "kv4 attend: null pointer");
   if (q_strides[3] != 1 || out_strides[3] != 1) return set_err(QFLASH_ERR_ARG, "kv4 attend: innermost (head-dim) stride must be 1");
-  const size_t need = rows_workspace(cache, Hq, N, weights_in != nullptr);
+  const size_t need = attend_workspace(cache, Hq, N, weights_in != nullptr);
   if (!workspace || workspace_bytes < need)
     return set_err(QFLASH_ERR_ARG, "kv4 attend: workspace of %zu bytes, %zu are needed", workspace ? workspace_bytes : 0, need);
   if ((uintptr_t)workspace & 15) return set_err(QFLASH_ERR_ALIGN, "kv4 attend: workspace must be 16-byte aligned");
@@ -418,5 +425,6 @@ extern "C" int qflash_kv4_attend(const qflash_kv4_cache* cache, const void* q, i
   a.scale_log2e = (float)(scale * 1.4426950408889634);
   a.weights_in = weights_in;
   a.tok0 = 0, a.ntok = N;
-  return attend_rows(a, dtype == kF16, workspace, dev, (cudaStream_t)stream);
+  return many_rows(cache, Hq, N) ? attend_prompt(a, dtype == kF16, workspace, dev, (cudaStream_t)stream)
+                                 : attend_rows(a, dtype == kF16, workspace, dev, (cudaStream_t)stream);
 }

@@ -115,6 +115,8 @@ __device__ __forceinline__ Span span_of(const AttendArgs& a, int z) {
 
 size_t rows_workspace(const qflash_kv4_cache* c, int Hq, int N, bool weights);
 int attend_rows(const AttendArgs& a, bool fp16, void* ws, int dev, cudaStream_t s);
+size_t prompt_workspace(const qflash_kv4_cache* c, int Hq, int N, bool weights);
+int attend_prompt(const AttendArgs& a, bool fp16, void* ws, int dev, cudaStream_t s);
 
 }  // namespace kv4
 }  // namespace qfb

@@ -1,0 +1,863 @@
+// Attention of many query rows over the 4-bit cache (prompts and their pieces):
+// qflash_kv4_attend's path for launches that arithmetic bounds.
+//
+// Rows of a key/value head are numbered token by token, its rep query heads
+// next to each other: row = token * rep + head, so that a tile of rows has one
+// narrow range of causal limits and a key tile serves all heads of the group.
+// A CTA holds 2 tiles of 128 rows and walks tiles of 128 keys:
+//   4 warps decode: a thread owns a key, turns its codes into bf16 (or fp16)
+//     numbers code - zero, exact, and writes them swizzled into shared memory;
+//     scales go to a ring of their own, and stay outside of the products
+//   1 thread issues tcgen05.mma: S = Q K^T into TMEM, O += P V with P from TMEM
+//   2 x 4 warps do the softmax of a row tile each, a thread a row, and write P
+//     over S.  The two tiles alternate: one's products run under the other's
+//     softmax.
+// P vs goes to the tensor cores as bf16 for bf16 queries, as the sum of two bf16
+// terms for fp16 queries (half steps 2^-8 and 2^-16).  O is rescaled only when a
+// row's maximum grew by more than 2^8: P is then at most 256, which costs no
+// bits in floating point.
+// The order of d within each 8 is 0 4 1 5 2 6 3 7 everywhere (codes d and d + 4
+// of a word come out of one mask): Q is stored so, and the epilogue undoes it.
+//
+// Work split as in the kernel for few rows: tiles of all (sequence, row tile,
+// head) units are numbered, each CTA takes an equal run, pieces of units are
+// joined by a second kernel.
+//
+// The attention weights need the rows' final maximum and sum, so a third kernel
+// forms S^T = K Q^T again, a thread a key, and adds up exp(S - m) / l along its
+// row of columns: no sum crosses threads, and no atomics.
+#include <algorithm>
+
+#include "kv4_common.cuh"
+#include "sm100_ptx.cuh"
+
+namespace qfb {
+namespace kv4 {
+
+constexpr int kM = 128;           // rows of a tile, TMEM lanes
+constexpr int kKeys = 128;        // keys of a tile
+constexpr int kRows = 2 * kM;     // rows of a CTA
+constexpr int kRing = 4;          // tiles of scales
+
+struct PromptArgs {
+  AttendArgs a;
+  int rows, row_tiles;  // N * rep, and that over 256
+  int grid;
+  bool vec_q, vec_o;
+  float* parts;   // [grid][2][256 (D + 2)]
+  float2* stats;  // [Z H][rows]: maximum (log2 units) and 1 / sum; null without weights
+};
+
+// kind::f16 instruction descriptor, fp32 accumulator: [4,6) D format 1 = f32,
+// [7,10) and [10,13) A and B format (0 f16, 1 bf16), [16] B major (1 = MN),
+// [17,23) N >> 3, [24,29) M >> 4.
+__host__ __device__ constexpr uint32_t idesc_f16(int N, bool bf16, bool b_mn_major) {
+  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn_major ? 1u : 0u) << 16) |
+         ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kM >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+               : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld32f(uint32_t addr, float* r) {
+  int v[32];
+  tmem_ld32(addr, v);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) r[i] = __int_as_float(v[i]);
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+               "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+               "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+               : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t y;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+  return y;
+}
+// pairs of fp32, one instruction for two
+__device__ __forceinline__ void mul2(float& a, float& b, float x, float y) {
+  asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmul.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(x), "f"(y));
+}
+__device__ __forceinline__ void add2(float& a, float& b, float x, float y) {
+  asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tadd.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(x), "f"(y));
+}
+// a, b = a * x + s, b * y + t
+__device__ __forceinline__ void fma2(float& a, float& b, float x, float y, float s, float t) {
+  asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmov.b64 r, {%4, %5};\n\t"
+      "fma.rn.f32x2 p, p, q, r;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(x), "f"(y), "f"(s), "f"(t));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+// Waits with a limit; after it (or another warp's) every role leaves its loops.
+struct Waiter {
+  volatile uint32_t* abort;
+  int32_t* ctl;
+  // A warp's lanes wait together and get the same answer.
+  __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity) const {
+    bool there = mbar_try_wait(bar, parity);
+    if (__all_sync(~0u, there)) return true;
+    const long long t0 = clock64();
+    while (!there) {
+      there = mbar_try_wait_hint(bar, parity, 100000);
+      if (there || *abort) break;
+      if (clock64() - t0 > kWaitCycles) {
+        *abort = 1;
+        atomicOr(&ctl[1], 2);
+        break;
+      }
+    }
+    return __all_sync(~0u, there);
+  }
+};
+
+// 8 codes as 4 words of two numbers code - zero, in the order 0 4, 1 5, 2 6, 3 7.
+template <bool FP16>
+__device__ __forceinline__ uint4 decode8(uint32_t w, uint32_t zero) {
+  uint32_t y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t m = (w >> (4 * i) & 0x000f000fu) | (FP16 ? 0x64006400u : 0x43004300u);
+    if (FP16)
+      asm("sub.f16x2 %0, %1, %2;" : "=r"(y[i]) : "r"(m), "r"(zero));
+    else
+      asm("sub.bf16x2 %0, %1, %2;" : "=r"(y[i]) : "r"(m), "r"(zero));
+  }
+  return make_uint4(y[0], y[1], y[2], y[3]);
+}
+template <bool FP16>
+__device__ __forceinline__ uint32_t zero_pair(uint32_t param) {
+  if (FP16) {
+    const __half2 x = __float2half2_rn(1024.f + param_zero(param));
+    return *reinterpret_cast<const uint32_t*>(&x);
+  }
+  return pack_bf16(128.f + param_zero(param), 128.f + param_zero(param));
+}
+
+// One vector's codes, decoded, as row `row` of a 128-row tile in shared memory:
+// blocks of 64 elements (128 bytes, swizzled by 16-byte chunks over 8 rows).
+template <int D, bool FP16>
+__device__ __forceinline__ void put_codes(uint32_t base, int row, const uint4 (&codes)[D / 32], uint32_t zero) {
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int chunk = 4 * i + j;
+      sts128(base + (chunk / 8) * (128 * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), decode8<FP16>(w[j], zero));
+    }
+  }
+}
+// One query row, likewise.
+template <int D>
+__device__ __forceinline__ void put_query(uint32_t base, int row, const uint16_t* q, bool vec) {
+#pragma unroll 4
+  for (int chunk = 0; chunk < D / 8; ++chunk) {
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (q) {
+      if (vec) {
+        x = __ldg(reinterpret_cast<const uint4*>(q) + chunk);
+      } else {
+        const uint16_t* p = q + 8 * chunk;
+        x = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
+      }
+    }
+    sts128(base + (chunk / 8) * (128 * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4),
+           make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410),
+                      __byte_perm(x.y, x.w, 0x7632)));
+  }
+}
+// K-major operand [128 rows][D]: step of 16 elements; MN-major operand (V): step of 16 keys.
+__device__ __forceinline__ uint64_t k_desc(uint32_t base, int step) {
+  return smem_desc(base + (step >> 2) * (128 * 128) + (step & 3) * 32, 16, 1024, kSw128);
+}
+__device__ __forceinline__ uint64_t mn_desc(uint32_t base, int step) {
+  return smem_desc(base + step * 16 * 128, 128 * 128, 1024, kSw128);
+}
+
+// ------------------------------------------------------------------ work split
+// Key tiles of row tile rt of sequence z.
+__device__ __forceinline__ int unit_tiles(const PromptArgs& p, int z, int rt) {
+  const AttendArgs& a = p.a;
+  const Span sp = span_of(a, z);
+  const int first = rt * kRows / a.rep, last = min(min(a.N, sp.fresh), (rt * kRows + kRows - 1) / a.rep + 1);
+  return first >= last ? 0 : (sp.limit(a, last - 1) + kKeys - 1) / kKeys;
+}
+
+// Where a CTA is in its run.  All lanes of a warp hold the same.
+struct Walk {
+  int z, rt, h, tiles;   // the unit
+  long long first;       // its first tile
+  long long at, stop;    // the run
+  int t0, t1;            // the piece: key tiles of the unit
+  bool whole;
+
+  __device__ __forceinline__ void cut() {
+    t0 = (int)(at - first);
+    t1 = (int)min((long long)tiles, t0 + (stop - at));
+    whole = t0 == 0 && t1 == tiles;
+  }
+  // The unit that holds tile `where` (of `total`).  One warp together.
+  __device__ __forceinline__ bool seek(const PromptArgs& p, long long where) {
+    const int lane = threadIdx.x & 31, n = p.a.c.Z * p.row_tiles, H = p.a.c.H;
+    long long base = 0;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const int i = i0 + lane;
+      const int t = i < n ? unit_tiles(p, i / p.row_tiles, i % p.row_tiles) : 0;
+      const long long mine = (long long)t * H;
+      long long sum = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(~0u, sum, o);
+        if (lane >= o) sum += up;
+      }
+      const unsigned hit = __ballot_sync(~0u, where >= base + sum - mine && where < base + sum);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        tiles = __shfl_sync(~0u, t, l);
+        first = base + __shfl_sync(~0u, sum - mine, l);
+        z = (i0 + l) / p.row_tiles, rt = (i0 + l) % p.row_tiles;
+        h = (int)((where - first) / tiles);
+        first += (long long)h * tiles;
+        return true;
+      }
+      base += __shfl_sync(~0u, sum, 31);
+    }
+    return false;
+  }
+  __device__ static long long total_tiles(const PromptArgs& p) {
+    const int lane = threadIdx.x & 31, n = p.a.c.Z * p.row_tiles;
+    long long sum = 0;
+    for (int i = lane; i < n; i += 32) sum += unit_tiles(p, i / p.row_tiles, i % p.row_tiles);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    return sum * p.a.c.H;
+  }
+  // On to the run's next piece; false behind its end.
+  __device__ __forceinline__ bool next(const PromptArgs& p) {
+    at += t1 - t0;
+    if (at >= stop) return false;
+    first += tiles;
+    if (++h == p.a.c.H) {
+      h = 0;
+      do {
+        if (++rt == p.row_tiles) {
+          rt = 0;
+          if (++z >= p.a.c.Z) return false;  // only if lens changed meanwhile
+        }
+        tiles = unit_tiles(p, z, rt);
+      } while (tiles == 0);
+    }
+    cut();
+    return true;
+  }
+};
+__device__ __forceinline__ long long run_begin(long long total, int grid, int cta) { return total * cta / grid; }
+
+// ------------------------------------------------------------------ attention
+template <int D>
+struct Layout {
+  static constexpr uint32_t TILE = 128 * D * 2;
+  static constexpr uint32_t Q = 0, K = 2 * TILE, V = 4 * TILE, KS = 6 * TILE, VS = KS + kRing * 512, BARS = VS + kRing * 512;
+  static constexpr uint32_t BYTES = BARS + 256 + 1024;  // with room to align the base
+};
+
+template <int D, bool FP16>
+__global__ void __launch_bounds__(512, 1) prompt_kernel(PromptArgs p) {
+  using L = Layout<D>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u;
+  uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const AttendArgs& a = p.a;
+  const Cache& c = a.c;
+  const uint32_t bars = base + L::BARS;
+  auto k_full = [&](int i) { return bars + 8 * i; };
+  auto k_empty = [&](int i) { return bars + 16 + 8 * i; };
+  auto v_full = [&](int i) { return bars + 32 + 8 * i; };
+  auto v_empty = [&](int i) { return bars + 48 + 8 * i; };
+  auto q_full = [&](int t) { return bars + 64 + 8 * t; };
+  auto s_full = [&](int t) { return bars + 80 + 8 * t; };
+  auto p_full = [&](int t) { return bars + 96 + 8 * t; };
+  auto o_full = [&](int t) { return bars + 112 + 8 * t; };
+  const uint32_t done = bars + 128, slot = bars + 136;
+  volatile uint32_t* abort = reinterpret_cast<volatile uint32_t*>(smem + L::BARS + 140);
+  float* const ks_ring = reinterpret_cast<float*>(smem + L::KS);
+  float* const vs_ring = reinterpret_cast<float*>(smem + L::VS);
+
+  if (warp == 12) {
+    if (lane == 0) {
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(k_full(i), 128), mbar_init(v_full(i), 128);
+        mbar_init(k_empty(i), 1), mbar_init(v_empty(i), 1);
+        mbar_init(q_full(i), 128), mbar_init(p_full(i), 128);
+        mbar_init(s_full(i), 2), mbar_init(o_full(i), 1);
+      }
+      mbar_init(done, 1);
+      *abort = 0;
+      fence_mbar_init();
+    }
+    __syncwarp();
+    tmem_alloc(slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  uint32_t tmem = 0;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
+  const Waiter wait{abort, c.ctl};
+
+  Walk w;
+  const long long total = Walk::total_tiles(p);
+  const int grid = (int)min((long long)p.grid, total);
+  bool any = (int)blockIdx.x < grid;
+  if (any) {
+    w.at = run_begin(total, grid, blockIdx.x);
+    w.stop = run_begin(total, grid, blockIdx.x + 1);
+    any = w.seek(p, w.at);  // false only if lens changed meanwhile
+    if (any) w.cut();
+  }
+
+  if (warp < 8) {
+    // ---------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    const int t = warp >> 2, lrow = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
+    uint32_t n = 0, pieces = 0;  // key tiles and pieces so far
+    while (any) {
+      const Span sp = span_of(a, w.z);
+      const int row = w.rt * kRows + t * kM + lrow, tok = row / a.rep, head = w.h * a.rep + row % a.rep;
+      const bool live = row < p.rows && tok < sp.fresh;
+      const int limit = live ? sp.limit(a, tok) : 0;
+      put_query<D>(base + L::Q + t * L::TILE, lrow,
+                   live ? (const uint16_t*)a.q + (w.z * a.qs[0] + head * a.qs[1] + tok * a.qs[2]) : nullptr, p.vec_q);
+      fence_proxy_async_smem();
+      mbar_arrive(q_full(t));
+      float m = -INFINITY, l = 0.f;
+      for (int j = w.t0; j < w.t1; ++j, ++n) {
+        if (!wait(s_full(t), n & 1)) goto out;
+        tc_fence_after();
+        const float4* ks = reinterpret_cast<const float4*>(ks_ring + (n & (kRing - 1)) * kKeys);
+        const float4* vs = reinterpret_cast<const float4*>(vs_ring + (n & (kRing - 1)) * kKeys);
+        const int lim = limit - j * kKeys;
+        float s[128];
+        float mx = -INFINITY;
+        const bool full = __all_sync(~0u, lim >= kKeys);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tmem_ld32f(s_at + 32 * q, s + 32 * q);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float4 f = ks[i];
+          mul2(s[4 * i], s[4 * i + 1], f.x, f.y);
+          mul2(s[4 * i + 2], s[4 * i + 3], f.z, f.w);
+        }
+        if (!full) {
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (i >= lim) s[i] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 128; i += 2) mx = max3(mx, s[i], s[i + 1]);
+        const bool up = mx > m + 8.f;
+        if (__any_sync(~0u, up)) {
+          const float f = up ? ex2(m - mx) : 1.f;
+          if (up) m = mx;
+          l *= f;
+          if (j > w.t0) {  // the last product into O is done: s_full was committed after it
+#pragma unroll 1
+            for (int q = 0; q < D / 32; ++q) {
+              int o[32];
+              tmem_ld32(o_at + 32 * q, o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_int(__int_as_float(o[i]) * f);
+              tmem_st32(o_at + 32 * q, o);
+            }
+          }
+        }
+        const float neg = m == -INFINITY ? 0.f : -m;
+        float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 f = vs[8 * q + i];
+            float* x = s + 32 * q + 4 * i;
+            add2(x[0], x[1], neg, neg);
+            add2(x[2], x[3], neg, neg);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = ex2(x[e]);
+            add2(l0, l1, x[0], x[1]);
+            add2(l0, l1, x[2], x[3]);
+            mul2(x[0], x[1], f.x, f.y);
+            mul2(x[2], x[3], f.z, f.w);
+            if (!full) {  // a masked position's scale may be anything
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (32 * q + 4 * i + e >= lim) x[e] = 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t y = pack_bf16(x[2 * e], x[2 * e + 1]);
+              hi[2 * i + e] = y;
+              if (FP16) {
+                add2(x[2 * e], x[2 * e + 1], -__uint_as_float(y << 16), -__uint_as_float(y & 0xffff0000u));
+                lo[2 * i + e] = pack_bf16(x[2 * e], x[2 * e + 1]);
+              }
+            }
+          }
+          tmem_st16(s_at + 16 * q, hi);
+          if (FP16) tmem_st16(s_at + 64 + 16 * q, lo);
+        }
+        l += l0 + l1;
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(p_full(t));
+      }
+      if (!wait(o_full(t), pieces & 1)) goto out;
+      tc_fence_after();
+      {
+        const float inv = 1.f / l;
+        const bool write = row < p.rows;
+        float* part = p.parts + ((size_t)blockIdx.x * 2 + (pieces ? 1 : 0)) * (kRows * (D + 2));
+        const size_t to = w.z * a.os[0] + head * a.os[1] + (size_t)tok * a.os[2];
+        if (write) {
+          if (!w.whole)
+            part[t * kM + lrow] = m, part[kRows + t * kM + lrow] = l;
+          else if (p.stats)
+            p.stats[((size_t)w.z * c.H + w.h) * p.rows + row] = make_float2(m, inv);
+        }
+#pragma unroll 1
+        for (int q = 0; q < D / 32; ++q) {
+          float o[32];
+          tmem_ld32f(o_at + 32 * q, o);
+          if (!write) continue;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float y[8] = {o[8 * g], o[8 * g + 2], o[8 * g + 4], o[8 * g + 6], o[8 * g + 1], o[8 * g + 3], o[8 * g + 5], o[8 * g + 7]};
+            if (w.whole) {
+              float x[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[e] = limit > 0 ? y[e] * inv : 0.f;
+              if (FP16)
+                store8((__half*)a.out + to + 32 * q + 8 * g, p.vec_o, x);
+              else
+                store8((__nv_bfloat16*)a.out + to + 32 * q + 8 * g, p.vec_o, x);
+            } else {
+              store8(part + 2 * kRows + (t * kM + lrow) * D + 32 * q + 8 * g, true, y);
+            }
+          }
+        }
+        tc_fence_before();
+      }
+      ++pieces;
+      any = w.next(p);
+    }
+  } else if (warp < 12) {
+    // ---------------------------------------------------------------- decoding
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    const int key = tid - 256;
+    uint32_t n = 0;
+    while (any) {
+      const size_t head = ((size_t)w.z * c.H + w.h) * c.C;
+      const int len = length_of(c, w.z);
+      for (int j = w.t0; j < w.t1; ++j, ++n) {
+        const int pos = j * kKeys + key, at = max(0, min(pos, len - 1));
+        const uint32_t kp = pos < len ? __ldg(c.param[0] + head + at) : 0u, vp = pos < len ? __ldg(c.param[1] + head + at) : 0u;
+        uint4 kc[D / 32], vc[D / 32];
+        const uint4* src = reinterpret_cast<const uint4*>(c.codes[0] + (head + at) * (D / 2));
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) kc[i] = __ldg(src + i);
+        src = reinterpret_cast<const uint4*>(c.codes[1] + (head + at) * (D / 2));
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) vc[i] = __ldg(src + i);
+        const int st = n & 1, ring = (n & (kRing - 1)) * kKeys;
+        if (!wait(k_empty(st), (n >> 1 & 1) ^ 1)) goto out;
+        // this slot's last tile is 4 back: the products of the tile 2 back, which k_empty waited for, came after its softmax
+        ks_ring[ring + key] = param_scale(kp) * a.scale_log2e;
+        vs_ring[ring + key] = param_scale(vp);
+        put_codes<D, FP16>(base + L::K + st * L::TILE, key, kc, zero_pair<FP16>(kp));
+        fence_proxy_async_smem();
+        mbar_arrive(k_full(st));
+        if (!wait(v_empty(st), (n >> 1 & 1) ^ 1)) goto out;
+        put_codes<D, false>(base + L::V + st * L::TILE, key, vc, zero_pair<false>(vp));
+        fence_proxy_async_smem();
+        mbar_arrive(v_full(st));
+      }
+      any = w.next(p);
+    }
+  } else {
+    // ---------------------------------------------------------------- products
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 12) {
+      constexpr uint32_t IS = idesc_f16(kKeys, !FP16, false), IO = idesc_f16(D, true, true);
+      uint32_t n = 0, pieces = 0;
+      auto scores = [&](int t, uint32_t g) {
+        if (lane == 0) {
+#pragma unroll
+          for (int s = 0; s < D / 16; ++s)
+            mma_ss(tmem + t * 128, k_desc(base + L::Q + t * L::TILE, s), k_desc(base + L::K + (g & 1) * L::TILE, s), IS, s > 0);
+          tc_commit(s_full(t));
+          mbar_arrive(s_full(t));  // passes on the scales that k_full's wait made visible here
+        }
+        __syncwarp();
+      };
+      while (any) {
+        const int tiles = w.t1 - w.t0;
+        if (!wait(k_full(n & 1), n >> 1 & 1)) goto out;
+        for (int t = 0; t < 2; ++t) {
+          if (!wait(q_full(t), pieces & 1)) goto out;
+          tc_fence_after();
+          scores(t, n);
+        }
+        if (lane == 0) tc_commit(k_empty(n & 1));
+        for (int j = 0; j < tiles; ++j, ++n) {
+          for (int t = 0; t < 2; ++t) {
+            if (!wait(v_full(n & 1), n >> 1 & 1) || !wait(p_full(t), n & 1)) goto out;
+            tc_fence_after();
+            if (lane == 0) {
+#pragma unroll
+              for (int s = 0; s < kKeys / 16; ++s)
+                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * s, mn_desc(base + L::V + (n & 1) * L::TILE, s), IO, j > 0 || s > 0);
+              if (FP16) {
+#pragma unroll
+                for (int s = 0; s < kKeys / 16; ++s)
+                  mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 64 + 8 * s, mn_desc(base + L::V + (n & 1) * L::TILE, s), IO, 1);
+              }
+              if (t == 1) tc_commit(v_empty(n & 1));
+              if (j + 1 == tiles) tc_commit(o_full(t));
+            }
+            __syncwarp();
+            if (j + 1 < tiles) {
+              if (!wait(k_full((n + 1) & 1), (n + 1) >> 1 & 1)) goto out;
+              tc_fence_after();
+              scores(t, n + 1);
+              if (t == 1 && lane == 0) tc_commit(k_empty((n + 1) & 1));
+            }
+          }
+        }
+        ++pieces;
+        any = w.next(p);
+      }
+    }
+  }
+out:
+  __syncwarp();
+  if (warp == 12) {  // nothing of this CTA's may be under way when its TMEM goes
+    if (lane == 0) tc_commit(done);
+    __syncwarp();
+    mbar_wait(done, 0);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+// Joins units that several CTAs held: blockIdx.x < 8 grid: 32 rows of the unit that
+// run blockIdx.x / 8's beginning is the first to cut; the others write the
+// zeros of units with nothing to see.
+template <int D, bool FP16>
+__global__ void __launch_bounds__(256) prompt_finish_kernel(PromptArgs p) {
+  const AttendArgs& a = p.a;
+  const Cache& c = a.c;
+  constexpr int kPart = kRows * (D + 2);
+  auto put = [&](int z, int h, int row, int col, const float (&x)[8]) {
+    const int tok = row / a.rep;
+    const size_t to = z * a.os[0] + (h * a.rep + row % a.rep) * a.os[1] + (size_t)tok * a.os[2] + col;
+    if (FP16)
+      store8((__half*)a.out + to, p.vec_o, x);
+    else
+      store8((__nv_bfloat16*)a.out + to, p.vec_o, x);
+  };
+  if ((int)blockIdx.x >= 8 * p.grid) {
+    const int i = blockIdx.x - 8 * p.grid, z = i / p.row_tiles, rt = i % p.row_tiles;
+    if (unit_tiles(p, z, rt) > 0) return;
+    const float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int e = threadIdx.x; e < kRows * (D / 8); e += 256) {
+      const int row = rt * kRows + e / (D / 8);
+      if (row < p.rows)
+        for (int h = 0; h < c.H; ++h) put(z, h, row, e % (D / 8) * 8, x);
+    }
+    return;
+  }
+  const int k = blockIdx.x / 8;
+  const long long total = Walk::total_tiles(p);
+  const int grid = (int)min((long long)p.grid, total);
+  if (k == 0 || k >= grid) return;
+  Walk w;
+  const long long cut = run_begin(total, grid, k);
+  if (!w.seek(p, cut) || w.first == cut || run_begin(total, grid, k - 1) > w.first) return;
+  const long long end = w.first + w.tiles;
+  const Span sp = span_of(a, w.z);
+  const int first = run_begin(total, grid, k - 1) < w.first ? 2 * (k - 1) + 1 : 2 * (k - 1);
+  for (int e = threadIdx.x; e < 32 * (D / 8); e += 256) {
+    const int r = (blockIdx.x & 7) * 32 + e / (D / 8), col = e % (D / 8) * 8, row = w.rt * kRows + r;
+    if (row >= p.rows) break;
+    const float* part = p.parts + (size_t)first * kPart;
+    float m = part[r], l = part[kRows + r], o[8];
+    load8(part + 2 * kRows + r * D + col, true, o);
+    for (int q = k; q < grid && run_begin(total, grid, q) < end; ++q) {
+      part = p.parts + (size_t)2 * q * kPart;
+      const float pm = part[r], pl = part[kRows + r], mx = fmaxf(m, pm);
+      const float f0 = m == -INFINITY ? 1.f : ex2(m - mx), f1 = pm == -INFINITY ? 1.f : ex2(pm - mx);
+      float x[8];
+      load8(part + 2 * kRows + r * D + col, true, x);
+      l = l * f0 + pl * f1;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = o[i] * f0 + x[i] * f1;
+      m = mx;
+    }
+    const int tok = row / a.rep;
+    const bool seen = tok < sp.fresh && sp.limit(a, tok) > 0;
+    const float inv = 1.f / l;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = seen ? o[i] * inv : 0.f;
+    put(w.z, w.h, row, col, o);
+    if (p.stats && col == 0) p.stats[((size_t)w.z * c.H + w.h) * p.rows + row] = make_float2(m, inv);
+  }
+}
+
+// ------------------------------------------------------------------ weights
+template <int D>
+struct WLayout {
+  static constexpr uint32_t TILE = 128 * D * 2;
+  static constexpr uint32_t K = 0, Q = TILE, COL = 3 * TILE, BARS = COL + 2 * 3 * 512;
+  static constexpr uint32_t BYTES = BARS + 128 + 1024;
+};
+
+// One CTA per 128 positions of a head: warps 0-3 add up (a thread a position),
+// warps 4-7 bring query tiles, warp 8 issues the products.
+template <int D, bool FP16>
+__global__ void __launch_bounds__(288, 2) prompt_weights_kernel(PromptArgs p) {
+  using L = WLayout<D>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u;
+  uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const AttendArgs& a = p.a;
+  const Cache& c = a.c;
+  const int key_tiles = (c.C + kKeys - 1) / kKeys;
+  const int zh = blockIdx.x / key_tiles, key0 = blockIdx.x % key_tiles * kKeys, z = zh / c.H, h = zh % c.H;
+  const Span sp = span_of(a, z);
+  if (key0 >= sp.len) return;
+  // rows that see position key0: from token `first` on
+  const int first = a.causal ? max(0, key0 - (sp.len - sp.fresh)) : 0;
+  const int rt0 = first < sp.fresh ? first * a.rep / kM : 0, rt1 = first < sp.fresh ? (sp.fresh * a.rep + kM - 1) / kM : 0;
+  const size_t head = (size_t)zh * c.C;
+  if (rt0 >= rt1) {
+    const int key = key0 + tid;
+    if (tid < kKeys && key < sp.len) c.weight[head + key] = a.weights_in[head + key];
+    return;
+  }
+  const uint32_t bars = base + L::BARS;
+  auto q_full = [&](int i) { return bars + 8 * i; };
+  auto q_empty = [&](int i) { return bars + 16 + 8 * i; };
+  auto s_full = [&](int i) { return bars + 32 + 8 * i; };
+  auto s_empty = [&](int i) { return bars + 48 + 8 * i; };
+  const uint32_t k_full = bars + 64, done = bars + 72, slot = bars + 80;
+  volatile uint32_t* abort = reinterpret_cast<volatile uint32_t*>(smem + L::BARS + 84);
+  float* const col = reinterpret_cast<float*>(smem + L::COL);  // [2][3][128]: maximum, 1 / sum, limit
+  if (warp == 8) {
+    if (lane == 0) {
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(q_full(i), 128), mbar_init(q_empty(i), 129);
+        mbar_init(s_full(i), 1), mbar_init(s_empty(i), 128);
+      }
+      mbar_init(k_full, 128), mbar_init(done, 1);
+      *abort = 0;
+      fence_mbar_init();
+    }
+    __syncwarp();
+    tmem_alloc(slot, 256);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  uint32_t tmem = 0;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
+  const Waiter wait{abort, c.ctl};
+
+  if (warp < 4) {
+    const int key = key0 + tid, at = min(key, sp.len - 1);
+    const uint32_t kp = key < sp.len ? __ldg(c.param[0] + head + at) : 0u;
+    const float ks = param_scale(kp) * a.scale_log2e;
+    uint4 kc[D / 32];
+    const uint4* src = reinterpret_cast<const uint4*>(c.codes[0] + (head + at) * (D / 2));
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) kc[i] = __ldg(src + i);
+    put_codes<D, FP16>(base + L::K, tid, kc, zero_pair<FP16>(kp));
+    fence_proxy_async_smem();
+    mbar_arrive(k_full);
+    const uint32_t s_at = tmem + ((uint32_t)(warp * 32) << 16);
+    float sum0 = 0.f, sum1 = 0.f;
+    for (int rt = rt0; rt < rt1; ++rt) {
+      const int g = rt - rt0, b = g & 1;
+      if (!wait(s_full(b), g >> 1 & 1) || !wait(q_full(b), g >> 1 & 1)) goto out;
+      tc_fence_after();
+      const float4* cm = reinterpret_cast<const float4*>(col + b * 384);
+      const float4* ci = cm + 32;
+      const int4* cl = reinterpret_cast<const int4*>(cm + 64);
+      // every row of the tile is there and sees all 128 positions
+      const bool full = (rt + 1) * kM <= sp.fresh * a.rep && sp.limit(a, rt * kM / a.rep) >= key0 + kKeys;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float s[32];
+        tmem_ld32f(s_at + b * 128 + 32 * q, s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 m = cm[8 * q + i], v = ci[8 * q + i];
+          float* x = s + 4 * i;
+          fma2(x[0], x[1], ks, ks, -m.x, -m.y);
+          fma2(x[2], x[3], ks, ks, -m.z, -m.w);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = ex2(x[e]);
+          if (!full) {
+            const int4 lim = cl[8 * q + i];
+            sum0 += key < lim.x ? x[0] * v.x : 0.f;
+            sum1 += key < lim.y ? x[1] * v.y : 0.f;
+            sum0 += key < lim.z ? x[2] * v.z : 0.f;
+            sum1 += key < lim.w ? x[3] * v.w : 0.f;
+          } else {
+            fma2(x[0], x[1], v.x, v.y, sum0, sum1);
+            fma2(x[2], x[3], v.z, v.w, x[0], x[1]);
+            sum0 = x[2], sum1 = x[3];
+          }
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(s_empty(b));
+      mbar_arrive(q_empty(b));
+    }
+    if (key < sp.len) c.weight[head + key] = a.weights_in[head + key] + (sum0 + sum1);
+  } else if (warp < 8) {
+    const int r = tid - 128;
+    for (int rt = rt0; rt < rt1; ++rt) {
+      const int g = rt - rt0, b = g & 1, row = rt * kM + r, tok = row / a.rep;
+      const int limit = row < p.rows && tok < sp.fresh ? sp.limit(a, tok) : 0;
+      const float2 st = limit > 0 ? __ldg(p.stats + (size_t)zh * p.rows + row) : make_float2(0.f, 0.f);
+      if (!wait(q_empty(b), (g >> 1 & 1) ^ 1)) goto out;
+      put_query<D>(base + L::Q + b * L::TILE, r,
+                   limit > 0 ? (const uint16_t*)a.q + (z * a.qs[0] + (h * a.rep + row % a.rep) * a.qs[1] + tok * a.qs[2]) : nullptr,
+                   p.vec_q);
+      col[b * 384 + r] = st.x == -INFINITY ? 0.f : st.x;
+      col[b * 384 + 128 + r] = st.y;
+      reinterpret_cast<int*>(col)[b * 384 + 256 + r] = limit;
+      fence_proxy_async_smem();
+      mbar_arrive(q_full(b));
+    }
+  } else {
+    constexpr uint32_t IS = idesc_f16(kM, !FP16, false);
+    if (!wait(k_full, 0)) goto out;
+    for (int rt = rt0; rt < rt1; ++rt) {
+      const int g = rt - rt0, b = g & 1;
+      if (!wait(q_full(b), g >> 1 & 1) || !wait(s_empty(b), (g >> 1 & 1) ^ 1)) goto out;
+      tc_fence_after();
+      if (lane == 0) {
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+          mma_ss(tmem + b * 128, k_desc(base + L::K, s), k_desc(base + L::Q + b * L::TILE, s), IS, s > 0);
+        tc_commit(s_full(b));
+        tc_commit(q_empty(b));
+      }
+      __syncwarp();
+    }
+  }
+out:
+  __syncwarp();
+  if (warp == 8) {
+    if (lane == 0) tc_commit(done);
+    __syncwarp();
+    mbar_wait(done, 0);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8) tmem_dealloc(tmem, 256);
+}
+
+// ------------------------------------------------------------------ host
+static PromptArgs plan_prompt(const AttendArgs& a, bool weights, int sms, size_t* bytes) {
+  PromptArgs p;
+  p.a = a;
+  p.rows = a.N * a.rep;
+  p.row_tiles = (p.rows + kRows - 1) / kRows;
+  p.grid = sms;
+  const size_t parts = (size_t)2 * sms * kRows * (a.c.D + 2) * 4;
+  const size_t stats = weights ? (size_t)a.c.Z * a.c.H * p.rows * 8 : 0;
+  p.parts = nullptr;
+  p.stats = (float2*)parts;  // offset, for now
+  *bytes = parts + stats;
+  return p;
+}
+
+constexpr int kSms = 148;
+
+size_t prompt_workspace(const qflash_kv4_cache* c, int Hq, int N, bool weights) {
+  AttendArgs a;
+  a.c = view(c), a.rep = Hq / c->H, a.N = N;
+  size_t n;
+  plan_prompt(a, weights, kSms, &n);
+  return n;
+}
+
+template <class K>
+static int allow_smem(K* kernel, uint32_t bytes) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess)
+    return set_err(QFLASH_ERR_LAUNCH, "kv4 prompt: shared memory: %s", cudaGetErrorString(cudaGetLastError()));
+  return QFLASH_OK;
+}
+
+template <int D, bool FP16>
+static int launch_prompt(const PromptArgs& p, cudaStream_t s) {
+  if (int rc = allow_smem(prompt_kernel<D, FP16>, Layout<D>::BYTES)) return rc;
+  prompt_kernel<D, FP16><<<p.grid, 512, Layout<D>::BYTES, s>>>(p);
+  if (int rc = check_launch("kv4 prompt", p.grid)) return rc;
+  const unsigned n = 8 * p.grid + p.a.c.Z * p.row_tiles;
+  prompt_finish_kernel<D, FP16><<<n, 256, 0, s>>>(p);
+  if (int rc = check_launch("kv4 prompt finish", n)) return rc;
+  if (!p.stats) return QFLASH_OK;
+  if (int rc = allow_smem(prompt_weights_kernel<D, FP16>, WLayout<D>::BYTES)) return rc;
+  const unsigned nw = (unsigned)(p.a.c.Z * p.a.c.H) * ((p.a.c.C + kKeys - 1) / kKeys);
+  prompt_weights_kernel<D, FP16><<<nw, 288, WLayout<D>::BYTES, s>>>(p);
+  return check_launch("kv4 prompt weights", nw);
+}
+
+int attend_prompt(const AttendArgs& a, bool fp16, void* ws, int dev, cudaStream_t s) {
+  size_t n;
+  PromptArgs p = plan_prompt(a, a.weights_in != nullptr, std::min(kSms, sm_count(dev)), &n);
+  p.parts = (float*)ws;
+  p.stats = a.weights_in ? (float2*)((uint8_t*)ws + (size_t)p.stats) : nullptr;
+  auto aligned = [](const void* q, const int64_t* st) { return (((uintptr_t)q | (st[0] * 2) | (st[1] * 2) | (st[2] * 2)) & 15) == 0; };
+  p.vec_q = aligned(a.q, a.qs), p.vec_o = aligned(a.out, a.os);
+  if (a.c.D == 64) return fp16 ? launch_prompt<64, true>(p, s) : launch_prompt<64, false>(p, s);
+  return fp16 ? launch_prompt<128, true>(p, s) : launch_prompt<128, false>(p, s);
+}
+
+}  // namespace kv4
+}  // namespace qfb
