@@ -11,18 +11,20 @@
 // split into two bf16 terms (2^-16), since one would cost the output's last
 // three bits.
 //
-// Both products are transposed, so that the cache is the MMA's A operand and is
-// decoded straight into A fragments in registers, with no shared memory:
+// Both products are transposed, so that the cache is the MMA's A operand, decoded
+// straight into A fragments:
 //   S^T = K Q^T: 16 keys x 8 rows per m16n8k16.  A thread (g, t) holds rows g
 //     and g + 8 of K, and since the order of the reduction over d is free, it
-//     loads one run of D / 8 bytes of its keys: the warp's loads are whole rows.
-//   O^T = V^T P^T: 16 dims x 8 rows, reduced over keys.  Thread (g, t) holds
-//     dims [g D/8, (g + 1) D/8) of keys 2t, 2t + 1 of each 8: two words of
-//     neighbouring keys are interleaved with prmt, after which a half2 is
-//     masked out of a word as in K's case.
+//     reads one run of D / 8 bytes of its keys.
+//   O^T = V^T P^T: 16 dims x 8 rows, reduced over keys.  ldmatrix.trans over
+//     16-bit units of 4 codes leaves a thread with the units of keys 2t and
+//     2t + 1 in the halves of a word: pairs of codes are masked out as in K's case.
 // S^T's accumulator layout becomes P^T's B fragment by one 8x8 transpose
 // (movmatrix) per 8 keys; rows of the softmax are columns here, so the maximum
 // is taken over registers and 3 shuffles.
+// Each warp has a ring of its own in shared memory, filled by cp.async two tiles
+// ahead (a head's codes are contiguous), with 16-byte chunks swizzled against
+// bank conflicts; no barrier but __syncwarp until the CTA's warps join.
 //
 // Work split: (sequence, kv head, row tile) units are cut into tiles of 128
 // keys, all tiles are numbered, and the CTAs of one resident wave each take an
@@ -30,6 +32,8 @@
 // CTA holds whole is written by it; pieces go to the workspace with their
 // maximum and sum, and a second kernel joins them in order.
 #include <algorithm>
+#include <atomic>
+#include <climits>
 
 #include "kv4_common.cuh"
 
@@ -38,6 +42,7 @@ namespace kv4 {
 
 constexpr int kTile = 128;        // keys per CTA tile: 4 warps of 32
 constexpr int kWarps = 4;
+constexpr int kGridMax = 148 * 5;  // CTAs of one resident wave at most
 constexpr int kRowsMax = 64;      // query rows (tokens x rep) per launch that accumulates weights
 
 struct RowsArgs {
@@ -136,49 +141,227 @@ __device__ __forceinline__ int sequence_of(const RowsArgs& p, long long at, long
 
 __device__ __forceinline__ long long run_start(long long total, int grid, int cta) { return total * cta / grid; }
 
-template <int D>
-struct Raw {
-  uint32_t k[4][D / 32];  // keys 8 i + g: D / 8 bytes each
-  uint32_t v[8][D / 64];  // keys 8 (i / 2) + 2 t + (i & 1): D / 16 bytes each
-  uint32_t kp, vp;        // parameters of key `lane`
-};
+__device__ __forceinline__ uint32_t shared_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool there) {  // zeros where nothing is there
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-template <int W>
-__device__ __forceinline__ void load_words(uint32_t (&r)[W], const uint8_t* p) {
-  if constexpr (W == 4) {
-    const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
-    r[0] = x.x, r[1] = x.y, r[2] = x.z, r[3] = x.w;
-  } else if constexpr (W == 2) {
-    const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
-    r[0] = x.x, r[1] = x.y;
-  } else {
-    r[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-  }
+// A warp's stage: 32 keys' codes, values' codes, and both parameter words.
+template <int D>
+struct Stage {
+  static constexpr int ROW = D / 2, CHUNKS = ROW / 16;
+  static constexpr uint32_t K = 0, V = 32 * ROW, KP = 64 * ROW, VP = KP + 128, BYTES = VP + 128;
+  static constexpr int COUNT = D == 128 ? 3 : 4;
+  // row r's 16-byte chunk c lies at chunk c ^ turn(r): 8 rows' chunks c cover all banks
+  __device__ static int turn(int r) { return D == 128 ? (r >> 1) & 3 : (r >> 2) & 1; }
+};
+constexpr int kJoinPad = 4;
+template <int D, int NT>
+constexpr uint32_t rows_smem() {
+  constexpr uint32_t ring = kWarps * Stage<D>::COUNT * Stage<D>::BYTES, join = kWarps * 8 * NT * (D + kJoinPad) * 4;
+  return ring > join ? ring : join;
 }
 
-// The 32 keys from key0 on; keys past `most` read the last one's codes (they are masked) and parameters 0.
+// Starts the copy of the 32 keys from key0 on; what lies behind `most` becomes zeros.
 template <int D>
-__device__ __forceinline__ void load_tile(Raw<D>& r, const uint8_t* kc, const uint8_t* vc, const uint32_t* kp,
-                                          const uint32_t* vp, int key0, int most) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+__device__ __forceinline__ void fetch(uint32_t stage, const uint8_t* kc, const uint8_t* vc, const uint32_t* kp,
+                                      const uint32_t* vp, int key0, int most) {
+  using S = Stage<D>;
+  const int lane = threadIdx.x & 31, r = lane / S::CHUNKS, c = lane % S::CHUNKS;
+  const uint32_t to = stage + r * S::ROW + ((c ^ S::turn(r)) << 4);  // the turn is the same 8 and 16 rows on
+  const size_t from = (size_t)key0 * S::ROW + lane * 16;
+  const int left = most - key0;
+  const bool whole = left >= 32;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    load_words<D / 32>(r.k[i], kc + (uint32_t)min(key0 + 8 * i + g, most - 1) * (D / 2u) + t * (D / 8));
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    load_words<D / 64>(r.v[i], vc + (uint32_t)min(key0 + 8 * (i >> 1) + 2 * t + (i & 1), most - 1) * (D / 2u) + g * (D / 16));
-  const int key = key0 + lane;
-  r.kp = key < most ? __ldg(kp + key) : 0u;
-  r.vp = key < most ? __ldg(vp + key) : 0u;
+  for (int i = 0; i < S::CHUNKS; ++i) {
+    const bool there = whole || r + i * (32 / S::CHUNKS) < left;
+    copy_async<16>(to + S::K + i * 512, there ? kc + from + i * 512 : kc, there);
+    copy_async<16>(to + S::V + i * 512, there ? vc + from + i * 512 : vc, there);
+  }
+  const bool there = lane < left;
+  copy_async<4>(stage + S::KP + 4 * lane, there ? kp + key0 + lane : kp, there);
+  copy_async<4>(stage + S::VP + 4 * lane, there ? vp + key0 + lane : vp, there);
 }
 
 template <int D, int NT, bool FP16>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) rows_kernel(RowsArgs p) {
+struct RowsState {
+  uint32_t q[NT][D / 16][2];  // queries as B fragments, in the order of d that K's runs are read in
+  int limit[NT][2];           // positions that rows 2t, 2t + 1 of each 8 see
+  float o[NT][D / 16][4], m[NT][2], l[NT][2];
+};
+
+// One stage of 32 keys.  FULL: every row sees all of them.
+template <int D, int NT, bool FP16, bool FULL>
+__device__ __forceinline__ void rows_step(RowsState<D, NT, FP16>& st, uint32_t stage, int key0, int most, float scale_log2e,
+                                          float* scores, int score_rows, int rows_left) {
+  using S = Stage<D>;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint32_t kpw, vpw;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(kpw) : "r"(stage + S::KP + 4 * lane));
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(vpw) : "r"(stage + S::VP + 4 * lane));
+  const float kscale = param_scale(kpw) * scale_log2e, vscale = param_scale(vpw);
+  // zero points behind the offset that code_pair's numbers carry
+  uint32_t kzero, vzero;
+  {
+    const float zk = param_zero(kpw), zv = param_zero(vpw);
+    if (FP16) {
+      const __half2 x = __float2half2_rn(1024.f + zk);
+      kzero = *reinterpret_cast<const uint32_t*>(&x);
+    } else {
+      kzero = pack_bf16(128.f + zk, 128.f + zk);
+    }
+    const float other = __shfl_down_sync(~0u, zv, 1);
+    vzero = pack_bf16(128.f + zv, 128.f + other);  // read from even lanes
+  }
+  float s[NT][2][4];
+#pragma unroll
+  for (int mt = 0; mt < 2; ++mt) {
+    const uint32_t z0 = __shfl_sync(~0u, kzero, 16 * mt + g), z1 = __shfl_sync(~0u, kzero, 16 * mt + 8 + g);
+    uint32_t k0[D / 32], k1[D / 32];
+    const uint32_t at = stage + S::K + (16 * mt + g) * S::ROW +
+                        (D == 128 ? (t ^ S::turn(g)) << 4 : (((t >> 1) ^ S::turn(g)) << 4) + (t & 1) * 8);
+    if constexpr (D == 128) {
+      asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(k0[0]), "=r"(k0[1]), "=r"(k0[2]), "=r"(k0[3]) : "r"(at));
+      asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(k1[0]), "=r"(k1[1]), "=r"(k1[2]), "=r"(k1[3]) : "r"(at + 8 * S::ROW));
+    } else {
+      asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(k0[0]), "=r"(k0[1]) : "r"(at));
+      asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(k1[0]), "=r"(k1[1]) : "r"(at + 8 * S::ROW));
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[n][mt][j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const uint32_t w0 = k0[i >> 1], w1 = k1[i >> 1];
+      const int sh = 8 * (i & 1);
+      const uint32_t af[4] = {code_pair<FP16>(w0 >> sh, z0), code_pair<FP16>(w1 >> sh, z1),
+                              code_pair<FP16>(w0 >> (sh + 4), z0), code_pair<FP16>(w1 >> (sh + 4), z1)};
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if (FP16)
+          mma_fp16(s[n][mt], af, st.q[n][i][0], st.q[n][i][1]);
+        else
+          mma_bf16(s[n][mt], af, st.q[n][i][0], st.q[n][i][1]);
+      }
+    }
+  }
+  // scale, mask, running maximum
+  float vs[4], mn[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) mn[n][0] = st.m[n][0], mn[n][1] = st.m[n][1];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float ks = __shfl_sync(~0u, kscale, 8 * i + g);
+    vs[i] = __shfl_sync(~0u, vscale, 8 * i + g);
+    const int key = key0 + 8 * i + g;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float* x = s[n][i >> 1] + 2 * (i & 1);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        x[j] *= ks;
+        if (!FULL && key >= st.limit[n][j]) x[j] = -INFINITY;
+        mn[n][j] = fmaxf(mn[n][j], x[j]);
+      }
+      if (scores && key < most && 8 * n + 2 * t < rows_left)
+        *reinterpret_cast<float2*>(scores + (size_t)key * score_rows + 8 * n + 2 * t) = make_float2(x[0], x[1]);
+    }
+  }
+  bool moved = false;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) mn[n][j] = fmaxf(mn[n][j], __shfl_xor_sync(~0u, mn[n][j], x));
+      moved |= mn[n][j] > st.m[n][j];
+    }
+  if (__any_sync(~0u, moved)) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float f[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        f[j] = mn[n][j] == -INFINITY ? 1.f : ex2(st.m[n][j] - mn[n][j]);
+        st.l[n][j] *= f[j];
+        st.m[n][j] = mn[n][j];
+      }
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        st.o[n][i][0] *= f[0], st.o[n][i][1] *= f[1];
+        st.o[n][i][2] *= f[0], st.o[n][i][3] *= f[1];
+      }
+    }
+  }
+  // P vs as B fragments [keys of 8][rows]
+  uint32_t ph[NT][4], pl[NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float top[2];  // a maximum of -inf (nothing seen yet, or scores of -inf alone) is no number to subtract
+#pragma unroll
+    for (int j = 0; j < 2; ++j) top[j] = st.m[n][j] == -INFINITY ? 0.f : st.m[n][j];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float y[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float e = ex2(s[n][i >> 1][2 * (i & 1) + j] - top[j]);
+        st.l[n][j] += e;
+        y[j] = e * vs[i];
+        if (!FULL && key0 + 8 * i + g >= st.limit[n][j]) y[j] = 0.f;  // a masked position's scale may be anything
+      }
+      const uint32_t hi = pack_bf16(y[0], y[1]);
+      ph[n][i] = transpose8(hi);
+      if (FP16) {
+        const uint32_t lo = pack_bf16(y[0] - __uint_as_float(hi << 16), y[1] - __uint_as_float(hi & 0xffff0000u));
+        pl[n][i] = transpose8(lo);
+      }
+    }
+  }
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    const uint32_t z0 = __shfl_sync(~0u, vzero, 16 * ks + 2 * t), z1 = __shfl_sync(~0u, vzero, 16 * ks + 8 + 2 * t);
+    // matrices of an x4: keys 0-7 and 8-15 of dims 32 seg .., the same of the next 32 dims
+    const int key = 16 * ks + 8 * (lane >> 3 & 1) + (lane & 7);
+#pragma unroll
+    for (int seg = 0; seg < D / 32; seg += 2) {
+      uint32_t x[4];
+      const uint32_t at = stage + S::V + key * S::ROW + (((seg + (lane >> 4)) ^ S::turn(lane & 7)) << 4);
+      asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // dims 32 (seg + i / 2) + 4 g + 2 (i & 1), and the next
+        const uint32_t a = x[i & 2], b = x[(i & 2) + 1];
+        const int sh = 8 * (i & 1);
+        const uint32_t af[4] = {code_pair<false>(a >> sh, z0), code_pair<false>(a >> (sh + 4), z0),
+                                code_pair<false>(b >> sh, z1), code_pair<false>(b >> (sh + 4), z1)};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma_bf16(st.o[n][2 * seg + i], af, ph[n][2 * ks], ph[n][2 * ks + 1]);
+          if (FP16) mma_bf16(st.o[n][2 * seg + i], af, pl[n][2 * ks], pl[n][2 * ks + 1]);
+        }
+      }
+    }
+  }
+}
+
+template <int D, int NT, bool FP16>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(RowsArgs p) {
+  using S = Stage<D>;
   constexpr int R = 8 * NT;
-  constexpr int kPad = D + 4;
-  __shared__ float so[kWarps][R][kPad];
+  extern __shared__ __align__(128) uint8_t smem[];
+  float(*so)[R][D + kJoinPad] = reinterpret_cast<float(*)[R][D + kJoinPad]>(smem);  // over the rings, when they are done
   __shared__ float sm[kWarps][R], sl[kWarps][R];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const uint32_t ring = shared_addr(smem) + warp * (S::COUNT * S::BYTES);
   const AttendArgs& a = p.a;
   const Cache& c = a.c;
   long long before, total;
@@ -214,9 +397,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) rows_kernel(Rows
     const uint32_t* kp = c.param[0] + head * c.C;
     const uint32_t* vp = c.param[1] + head * c.C;
 
-    // queries as B fragments, in the order of d that K's runs are loaded in
-    uint32_t qf[NT][D / 16][2];
-    int limit[NT][2];
+    auto start = [&](int tile) {
+      const int key0 = tile * kTile + warp * 32;
+      if (tile < t1 && key0 < most) fetch<D>(ring + (tile - t0) % S::COUNT * S::BYTES, kc, vc, kp, vp, key0, most);
+      copies_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < S::COUNT - 1; ++i) start(t0 + i);
+
+    RowsState<D, NT, FP16> st;
+    int least = INT_MAX;  // positions that every row sees
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int row = row0 + 8 * n + g, tok = a.tok0 + row / a.rep;
@@ -227,173 +417,40 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) rows_kernel(Rows
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int d = t * (D / 4) + 8 * (s >> 1) + 2 * (s & 1) + j;
-          qf[n][s][j] = live ? (uint32_t)__ldg(q + d) | ((uint32_t)__ldg(q + d + 4) << 16) : 0u;
+          st.q[n][s][j] = live ? (uint32_t)__ldg(q + d) | ((uint32_t)__ldg(q + d + 4) << 16) : 0u;
         }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int r = row0 + 8 * n + 2 * t + j;
-        limit[n][j] = r < p.rows ? sp.limit(a, a.tok0 + r / a.rep) : 0;
+        const int r = row0 + 8 * n + 2 * t + j, tk = a.tok0 + r / a.rep;
+        // rows that are not there see everything: nothing of them is used, and they must not keep the others from FULL
+        st.limit[n][j] = r < p.rows && tk < sp.fresh ? sp.limit(a, tk) : INT_MAX;
+        least = min(least, st.limit[n][j]);
       }
-    }
-    float o[NT][D / 16][4], m[NT][2], l[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[n][i][j] = 0.f;
-      m[n][0] = m[n][1] = -INFINITY;
-      l[n][0] = l[n][1] = 0.f;
+        for (int j = 0; j < 4; ++j) st.o[n][i][j] = 0.f;
+      st.m[n][0] = st.m[n][1] = -INFINITY;
+      st.l[n][0] = st.l[n][1] = 0.f;
     }
+    least = min(most, __reduce_min_sync(~0u, least));
+    float* scores = p.scores ? p.scores + head * c.C * p.score_rows + row0 : nullptr;
 
-    Raw<D> raw;
-    load_tile<D>(raw, kc, vc, kp, vp, t0 * kTile + warp * 32, most);
+    int at_stage = 0;
     for (int tile = t0; tile < t1; ++tile) {
+      copies_wait<S::COUNT - 2>();
+      __syncwarp();  // this tile's copies are there for all lanes, and all have left the stage that is filled next
+      start(tile + S::COUNT - 1);
       const int key0 = tile * kTile + warp * 32;
-      const Raw<D> cur = raw;
-      if (tile + 1 < t1) load_tile<D>(raw, kc, vc, kp, vp, key0 + kTile, most);
-      if (key0 >= most) continue;
-      const float kscale = param_scale(cur.kp) * a.scale_log2e, vscale = param_scale(cur.vp);
-      // zero points behind the offset that code_pair's numbers carry
-      uint32_t kzero, vzero;
-      {
-        const float zk = param_zero(cur.kp), zv = param_zero(cur.vp);
-        if (FP16) {
-          const __half2 x = __float2half2_rn(1024.f + zk);
-          kzero = *reinterpret_cast<const uint32_t*>(&x);
-        } else {
-          kzero = pack_bf16(128.f + zk, 128.f + zk);
-        }
-        const float other = __shfl_xor_sync(~0u, zv, 1);
-        vzero = lane & 1 ? pack_bf16(128.f + other, 128.f + zv) : pack_bf16(128.f + zv, 128.f + other);
-      }
-      float s[NT][2][4];
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const uint32_t z0 = __shfl_sync(~0u, kzero, 16 * mt + g), z1 = __shfl_sync(~0u, kzero, 16 * mt + 8 + g);
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[n][mt][j] = 0.f;
-#pragma unroll
-        for (int st = 0; st < D / 16; ++st) {
-          const uint32_t w0 = cur.k[2 * mt][st >> 1], w1 = cur.k[2 * mt + 1][st >> 1];
-          const int sh = 8 * (st & 1);
-          const uint32_t af[4] = {code_pair<FP16>(w0 >> sh, z0), code_pair<FP16>(w1 >> sh, z1),
-                                  code_pair<FP16>(w0 >> (sh + 4), z0), code_pair<FP16>(w1 >> (sh + 4), z1)};
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            if (FP16)
-              mma_fp16(s[n][mt], af, qf[n][st][0], qf[n][st][1]);
-            else
-              mma_bf16(s[n][mt], af, qf[n][st][0], qf[n][st][1]);
-          }
-        }
-      }
-      // scale, mask, running maximum
-      float vs[4];
-      bool moved = false;
-      float mn[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) mn[n][0] = m[n][0], mn[n][1] = m[n][1];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float ks = __shfl_sync(~0u, kscale, 8 * i + g);
-        vs[i] = __shfl_sync(~0u, vscale, 8 * i + g);
-        const int key = key0 + 8 * i + g;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float x[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            x[j] = s[n][i >> 1][2 * (i & 1) + j] * ks;
-            if (key >= limit[n][j]) x[j] = -INFINITY;
-            s[n][i >> 1][2 * (i & 1) + j] = x[j];
-            mn[n][j] = fmaxf(mn[n][j], x[j]);
-          }
-          if (p.scores && key < most && row0 + 8 * n + 2 * t < p.rows)
-            *reinterpret_cast<float2*>(p.scores + (head * c.C + key) * p.score_rows + row0 + 8 * n + 2 * t) = make_float2(x[0], x[1]);
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) mn[n][j] = fmaxf(mn[n][j], __shfl_xor_sync(~0u, mn[n][j], x));
-          moved |= mn[n][j] > m[n][j];
-        }
-      if (__any_sync(~0u, moved)) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float f[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            f[j] = mn[n][j] == -INFINITY ? 1.f : ex2(m[n][j] - mn[n][j]);
-            l[n][j] *= f[j];
-            m[n][j] = mn[n][j];
-          }
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            o[n][i][0] *= f[0], o[n][i][1] *= f[1];
-            o[n][i][2] *= f[0], o[n][i][3] *= f[1];
-          }
-        }
-      }
-      float top[NT][2];  // a maximum of -inf (nothing seen yet, or scores of -inf alone) is no number to subtract
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) top[n][j] = m[n][j] == -INFINITY ? 0.f : m[n][j];
-      // P vs as B fragments [keys of 8][rows]
-      uint32_t ph[NT][4], pl[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float y[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float x = s[n][i >> 1][2 * (i & 1) + j];
-            const bool seen = key0 + 8 * i + g < limit[n][j];
-            const float e = seen ? ex2(x - top[n][j]) : 0.f;
-            l[n][j] += e;
-            y[j] = seen ? e * vs[i] : 0.f;  // a masked position's scale may be anything
-          }
-          const uint32_t hi = pack_bf16(y[0], y[1]);
-          ph[n][i] = transpose8(hi);
-          if (FP16) {
-            const uint32_t lo = pack_bf16(y[0] - __uint_as_float(hi << 16), y[1] - __uint_as_float(hi & 0xffff0000u));
-            pl[n][i] = transpose8(lo);
-          }
-        }
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        const uint32_t z0 = __shfl_sync(~0u, vzero, 16 * ks + 2 * t), z1 = __shfl_sync(~0u, vzero, 16 * ks + 8 + 2 * t);
-#pragma unroll
-        for (int w = 0; w < D / 64; ++w) {
-          // words of neighbouring keys, interleaved by halves
-          uint32_t x[2][2];
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const uint32_t e = cur.v[4 * ks + 2 * b][w], f = cur.v[4 * ks + 2 * b + 1][w];
-            x[b][0] = __byte_perm(e, f, 0x5410);
-            x[b][1] = __byte_perm(e, f, 0x7632);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {  // dims 8 w + 2 i, 8 w + 2 i + 1 of this thread's run
-            const int half = i >> 1, sh = 8 * (i & 1);
-            const uint32_t af[4] = {code_pair<false>(x[0][half] >> sh, z0), code_pair<false>(x[0][half] >> (sh + 4), z0),
-                                    code_pair<false>(x[1][half] >> sh, z1), code_pair<false>(x[1][half] >> (sh + 4), z1)};
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              mma_bf16(o[n][4 * w + i], af, ph[n][2 * ks], ph[n][2 * ks + 1]);
-              if (FP16) mma_bf16(o[n][4 * w + i], af, pl[n][2 * ks], pl[n][2 * ks + 1]);
-            }
-          }
-        }
-      }
+      const uint32_t stage = ring + at_stage * S::BYTES;
+      at_stage = at_stage + 1 == S::COUNT ? 0 : at_stage + 1;
+      if (key0 + 32 <= least)
+        rows_step<D, NT, FP16, true>(st, stage, key0, most, a.scale_log2e, scores, p.score_rows, p.rows - row0);
+      else if (key0 < most)
+        rows_step<D, NT, FP16, false>(st, stage, key0, most, a.scale_log2e, scores, p.score_rows, p.rows - row0);
     }
+    copies_wait<0>();
+    __syncthreads();
 
     // join the 4 warps
 #pragma unroll
@@ -401,15 +458,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) rows_kernel(Rows
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) l[n][j] += __shfl_xor_sync(~0u, l[n][j], x);
+        for (int x = 4; x < 32; x <<= 1) st.l[n][j] += __shfl_xor_sync(~0u, st.l[n][j], x);
         const int r = 8 * n + 2 * t + j;
-        if (g == 0) sm[warp][r] = m[n][j], sl[warp][r] = l[n][j];
+        if (g == 0) sm[warp][r] = st.m[n][j], sl[warp][r] = st.l[n][j];
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          // accumulator rows g and g + 8 of m-tile i are dims 2 i and 2 i + 1 of run g
-          so[warp][r][g * (D / 8) + 2 * i] = o[n][i][j];
-          so[warp][r][g * (D / 8) + 2 * i + 1] = o[n][i][2 + j];
-        }
+        for (int i = 0; i < D / 16; ++i)  // accumulator rows g and g + 8
+          *reinterpret_cast<float2*>(&so[warp][r][32 * (i >> 1) + 4 * g + 2 * (i & 1)]) = make_float2(st.o[n][i][j], st.o[n][i][2 + j]);
       }
     __syncthreads();
     const bool whole = t0 == 0 && t1 == tiles;
@@ -423,19 +477,19 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) rows_kernel(Rows
       float ll = 0.f, oo = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = sm[w][r] == -INFINITY ? 0.f : ex2(sm[w][r] - mm);
         // a warp that saw no key of this row holds l = 0 and O = 0; one that saw only NaN holds NaN
-        ll += sm[w][r] == -INFINITY ? sl[w][r] : sl[w][r] * f;
-        oo += sm[w][r] == -INFINITY ? so[w][r][d] : so[w][r][d] * f;
+        const float f = sm[w][r] == -INFINITY ? 1.f : ex2(sm[w][r] - mm);
+        ll += sl[w][r] * f;
+        oo += so[w][r][d] * f;
       }
       if (whole) {
         const int tok = a.tok0 + row / a.rep;
         const float y = sp.limit(a, tok) > 0 ? oo / ll : 0.f;
-        const size_t at_out = z * a.os[0] + (h * a.rep + row % a.rep) * a.os[1] + tok * a.os[2] + d;
+        const size_t to = z * a.os[0] + (h * a.rep + row % a.rep) * a.os[1] + tok * a.os[2] + d;
         if (FP16)
-          ((__half*)a.out)[at_out] = __float2half_rn(y);
+          ((__half*)a.out)[to] = __float2half_rn(y);
         else
-          ((__nv_bfloat16*)a.out)[at_out] = __float2bfloat16_rn(y);
+          ((__nv_bfloat16*)a.out)[to] = __float2bfloat16_rn(y);
         if (d == 0 && p.scores) p.stats[(head * p.row_tiles + unit % p.row_tiles) * R + r] = make_float2(mm, ll);
       } else {
         part[2 * R + r * D + d] = oo;
@@ -448,98 +502,126 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) rows_kernel(Rows
   }
 }
 
-// Joins the pieces of units that several CTAs held, writes zeros for units with
-// nothing to see, and adds the attention weights: blockIdx.x is a unit,
-// blockIdx.y 0 its output, y > 0 a run of kChunk positions' weights.
+// Joins the pieces of units that several CTAs held and writes zeros for units
+// with nothing to see (a block per row of a unit), and adds the attention
+// weights (the blocks behind them: kChunk positions of a head each).
 constexpr int kChunk = 1024;
+constexpr int kJoin = 256;  // threads
 
 template <int D, int NT, bool FP16>
-__global__ void __launch_bounds__(256) rows_finish_kernel(RowsArgs p) {
+__global__ void __launch_bounds__(kJoin) rows_finish_kernel(RowsArgs p) {
   constexpr int R = 8 * NT;
   constexpr int kPart = R * (D + 2);
+  __shared__ float sf[kGridMax];
+  __shared__ float red[kJoin / 32], sums[kJoin];
+  __shared__ float sm[kRowsMax], sinv[kRowsMax];
   const AttendArgs& a = p.a;
   const Cache& c = a.c;
-  const int rt = blockIdx.x % p.row_tiles, zh = blockIdx.x / p.row_tiles, z = zh / c.H, h = zh % c.H;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int joins = c.Z * c.H * p.rows;
+  const bool weigh = (int)blockIdx.x >= joins;
+  const int chunks = (c.C + kChunk - 1) / kChunk;
+  const int zh = weigh ? (blockIdx.x - joins) / chunks : blockIdx.x / p.rows, z = zh / c.H, h = zh % c.H;
   const Span sp = span_of(a, z);
   const int most = sp.most(a), tiles = (most + kTile - 1) / kTile;
-  const int tid = threadIdx.x;
-  if (blockIdx.y > 0 && rt > 0) return;
   long long before = 0, total = 0;
   if (tiles) tiles_before(p, z, &before, &total);
   const int ctas = (int)min((long long)p.grid, total);
+  // The CTAs that hold pieces of a unit whose first tile is `first`, and where CTA k's piece is
+  auto holder = [&](long long tile) { return (int)min(ctas - 1LL, ((tile + 1) * ctas - 1) / total); };
+  auto part_of = [&](long long first, int c0, int k) {
+    return p.parts + (size_t)(k == c0 && run_start(total, ctas, k) < first ? 2 * k + 1 : 2 * k) * kPart;
+  };
 
-  // slot of the piece that CTA k holds of the unit whose first tile is `at`
-  auto slot = [&](long long at, int k) { return 2 * k + (run_start(total, ctas, k) < at ? 1 : 0); };
-  auto holder = [&](long long at) { return (int)min(ctas - 1LL, ((at + 1) * ctas - 1) / total); };
-
-  if (blockIdx.y == 0) {
-    const int row0 = rt * R, rows = min(R, p.rows - row0);
-    int c0 = 0, c1 = 0;
-    const long long at = before + ((long long)h * p.row_tiles + rt) * tiles;
-    if (tiles) {
-      c0 = holder(at), c1 = holder(at + tiles - 1);
-      if (c0 == c1) return;  // written by its holder
-    }
-    for (int e = tid; e < rows * D; e += 256) {
-      const int r = e / D, d = e % D, row = row0 + r, tok = a.tok0 + row / a.rep;
-      float y = 0.f;
-      if (tiles && sp.limit(a, tok) > 0) {
-        float mm = -INFINITY, ll = 0.f, oo = 0.f;
-        for (int k = c0; k <= c1; ++k) {
-          const float* part = p.parts + (size_t)(k == c0 ? slot(at, k) : 2 * k) * kPart;
-          const float pm = part[r], plv = part[R + r], po = part[2 * R + r * D + d];
-          const float mx = fmaxf(mm, pm);
-          const float f0 = mm == -INFINITY ? 1.f : ex2(mm - mx), f1 = pm == -INFINITY ? 1.f : ex2(pm - mx);
-          ll = ll * f0 + plv * f1;
-          oo = oo * f0 + po * f1;
-          mm = mx;
-        }
-        y = oo / ll;
+  if (!weigh) {
+    const int row = blockIdx.x % p.rows, u = row / R, r = row % R, tok = a.tok0 + row / a.rep;
+    const size_t to = z * a.os[0] + (h * a.rep + row % a.rep) * a.os[1] + tok * a.os[2];
+    const bool seen = sp.limit(a, tok) > 0;
+    const long long first = before + ((long long)h * p.row_tiles + u) * tiles;
+    const int c0 = tiles ? holder(first) : 0, n = tiles ? holder(first + tiles - 1) - c0 + 1 : 0;
+    if (n == 1) return;  // written by its holder
+    constexpr int G = kJoin / D;  // groups of threads that share a row's pieces
+    const int d = tid % D, group = tid / D;
+    float y = 0.f;
+    if (seen) {
+      float mx = -INFINITY;
+      for (int k = tid; k < n; k += kJoin) mx = fmaxf(mx, part_of(first, c0, c0 + k)[r]);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
+      if (lane == 0) red[warp] = mx;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kJoin / 32; ++w) mx = fmaxf(mx, red[w]);
+      __syncthreads();
+      float l = 0.f;
+      for (int k = tid; k < n; k += kJoin) {
+        const float* part = part_of(first, c0, c0 + k);
+        const float f = part[r] == -INFINITY ? 1.f : ex2(part[r] - mx);
+        sf[k] = f;
+        l += f * part[R + r];
       }
-      const size_t to = z * a.os[0] + (h * a.rep + row % a.rep) * a.os[1] + tok * a.os[2] + d;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
+      if (lane == 0) red[warp] = l;
+      __syncthreads();
+      l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kJoin / 32; ++w) l += red[w];
+      // all but the first piece lie in their CTAs' slot 0
+      if (group == 0) y = sf[0] * part_of(first, c0, c0)[2 * R + r * D + d];
+      const float* part = p.parts + (size_t)2 * c0 * kPart + 2 * R + r * D + d;
+#pragma unroll 8
+      for (int k = 1 + group; k < n; k += G) y += sf[k] * part[(size_t)2 * k * kPart];
+      sums[tid] = y;
+      __syncthreads();
+#pragma unroll
+      for (int q = 1; q < G; ++q) y += sums[q * D + d];
+      y /= l;
+    }
+    if (group == 0) {
       if (FP16)
-        ((__half*)a.out)[to] = __float2half_rn(y);
+        ((__half*)a.out)[to + d] = __float2half_rn(y);
       else
-        ((__nv_bfloat16*)a.out)[to] = __float2bfloat16_rn(y);
+        ((__nv_bfloat16*)a.out)[to + d] = __float2bfloat16_rn(y);
     }
     return;
   }
 
   // weights: w_j += sum over rows of 2^(S_rj - m_r) / l_r
-  const int j0 = (blockIdx.y - 1) * kChunk, j1 = min(sp.len, j0 + kChunk);
+  const int j0 = (blockIdx.x - joins) % chunks * kChunk, j1 = min(sp.len, j0 + kChunk);
   if (j0 >= j1) return;
-  __shared__ float sm[kRowsMax], sinv[kRowsMax];
-  for (int row = tid; row < p.rows; row += 256) {
-    float mm = -INFINITY, ll = 0.f;
-    if (tiles && sp.limit(a, a.tok0 + row / a.rep) > 0) {
+  for (int row = warp; row < p.rows; row += kJoin / 32) {
+    float mx = -INFINITY, l = 0.f;
+    const bool seen = tiles && sp.limit(a, a.tok0 + row / a.rep) > 0;
+    if (seen) {
       const int u = row / R, r = row % R;
-      const long long at = before + ((long long)h * p.row_tiles + u) * tiles;
-      const int c0 = holder(at), c1 = holder(at + tiles - 1);
-      if (c0 == c1) {
+      const long long first = before + ((long long)h * p.row_tiles + u) * tiles;
+      const int c0 = holder(first), n = holder(first + tiles - 1) - c0 + 1;
+      if (n == 1) {
         const float2 s = p.stats[((size_t)zh * p.row_tiles + u) * R + r];
-        mm = s.x, ll = s.y;
+        mx = s.x, l = s.y;
       } else {
-        for (int k = c0; k <= c1; ++k) {
-          const float* part = p.parts + (size_t)(k == c0 ? slot(at, k) : 2 * k) * kPart;
-          const float pm = part[r], plv = part[R + r], mx = fmaxf(mm, pm);
-          ll = ll * (mm == -INFINITY ? 1.f : ex2(mm - mx)) + plv * (pm == -INFINITY ? 1.f : ex2(pm - mx));
-          mm = mx;
+        for (int k = lane; k < n; k += 32) mx = fmaxf(mx, part_of(first, c0, c0 + k)[r]);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
+        for (int k = lane; k < n; k += 32) {
+          const float* part = part_of(first, c0, c0 + k);
+          l += part[R + r] * (part[r] == -INFINITY ? 1.f : ex2(part[r] - mx));
         }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
       }
-      sm[row] = mm, sinv[row] = 1.f / ll;
-    } else {
-      sm[row] = 0.f, sinv[row] = 0.f;
     }
+    if (lane == 0) sm[row] = mx == -INFINITY ? 0.f : mx, sinv[row] = seen ? 1.f / l : 0.f;
   }
   __syncthreads();
-  for (int j = j0 + tid; j < j1; j += 256) {
+  for (int j = j0 + tid; j < j1; j += kJoin) {
     float add = 0.f;
     if (j < most) {
       const float* s = p.scores + ((size_t)zh * c.C + j) * p.score_rows;
-      for (int row = 0; row < p.rows; ++row) {
-        const int lim = sp.limit(a, a.tok0 + row / a.rep);
-        if (j < lim) add += ex2(s[row] - sm[row]) * sinv[row];
-      }
+#pragma unroll 4
+      for (int row = 0; row < p.rows; ++row)
+        if (j < sp.limit(a, a.tok0 + row / a.rep)) add += ex2(s[row] - sm[row]) * sinv[row];
     }
     const size_t w = (size_t)zh * c.C + j;
     c.weight[w] = a.weights_in[w] + add;
@@ -553,7 +635,7 @@ struct RowsPlan {
   int nt, row_tiles, rows, score_rows;
   long long parts, stats, scores;  // floats
 };
-constexpr int kGridMax = 148 * 3 * 2;
+constexpr int kDevices = 64;  // as many as select_device knows
 
 static RowsPlan plan_rows(const Cache& c, int rep, int ntok, bool weights) {
   RowsPlan p;
@@ -576,20 +658,24 @@ size_t rows_workspace(const qflash_kv4_cache* c, int Hq, int N, bool weights) {
 template <int D, int NT, bool FP16>
 static int launch_rows(RowsArgs r, int dev, cudaStream_t s) {
   const Cache& c = r.a.c;
-  static int per_sm = 0;
-  if (!per_sm) {
+  constexpr uint32_t smem = rows_smem<D, NT>();
+  static std::atomic<int> per_sm_on[kDevices];  // 0: not asked yet
+  std::atomic<int>& per_sm = per_sm_on[dev];
+  if (!per_sm.load()) {
     int n = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, rows_kernel<D, NT, FP16>, kWarps * 32, 0) != cudaSuccess || n < 1)
+    if (cudaFuncSetAttribute(rows_kernel<D, NT, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+        cudaFuncSetAttribute(rows_kernel<D, NT, FP16>, cudaFuncAttributePreferredSharedMemoryCarveout, 100) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, rows_kernel<D, NT, FP16>, kWarps * 32, smem) != cudaSuccess || n < 1)
       return set_err(QFLASH_ERR_LAUNCH, "kv4 rows: occupancy: %s", cudaGetErrorString(cudaGetLastError()));
-    per_sm = n;
+    per_sm.store(n);
   }
   const long long tiles = (long long)c.Z * c.H * r.row_tiles * ((c.C + kTile - 1) / kTile);
-  r.grid = (int)std::min<long long>(std::min<long long>((long long)sm_count(dev) * per_sm, kGridMax), tiles);
-  rows_kernel<D, NT, FP16><<<r.grid, kWarps * 32, 0, s>>>(r);
+  r.grid = (int)std::min<long long>(std::min<long long>((long long)sm_count(dev) * per_sm.load(), kGridMax), tiles);
+  rows_kernel<D, NT, FP16><<<r.grid, kWarps * 32, smem, s>>>(r);
   if (int rc = check_launch("kv4 rows", r.grid)) return rc;
-  const dim3 grid(c.Z * c.H * r.row_tiles, r.scores ? 1 + (c.C + kChunk - 1) / kChunk : 1);
-  rows_finish_kernel<D, NT, FP16><<<grid, 256, 0, s>>>(r);
-  return check_launch("kv4 rows finish", grid.x);
+  const unsigned grid = (unsigned)(c.Z * c.H) * (r.rows + (r.scores ? (c.C + kChunk - 1) / kChunk : 0));
+  rows_finish_kernel<D, NT, FP16><<<grid, kJoin, 0, s>>>(r);
+  return check_launch("kv4 rows finish", grid);
 }
 
 int attend_rows(const AttendArgs& a0, bool fp16, void* ws, int dev, cudaStream_t s) {
