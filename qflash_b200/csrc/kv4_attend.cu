@@ -50,6 +50,7 @@ struct RowsArgs {
   int rows;       // ntok * rep
   int row_tiles;  // ceil(rows / (8 NT))
   int grid;       // CTAs of the first kernel
+  bool vec_q;     // query rows start on 16-byte boundaries
   int score_rows; // rows rounded up to even: the score buffer's row length
   float* parts;   // [grid][2][8 NT (D + 2)]: m, l, O of a piece
   float2* stats;  // [Z H row_tiles][8 NT]: m, l of units that one CTA held
@@ -169,25 +170,41 @@ constexpr uint32_t rows_smem() {
   return ring > join ? ring : join;
 }
 
-// Starts the copy of the 32 keys from key0 on; what lies behind `most` becomes zeros.
+// Where a lane's share of a warp's stages comes from; advanced tile by tile.
 template <int D>
-__device__ __forceinline__ void fetch(uint32_t stage, const uint8_t* kc, const uint8_t* vc, const uint32_t* kp,
-                                      const uint32_t* vp, int key0, int most) {
+struct Source {
+  const uint8_t *kc, *vc;      // 16 bytes per lane and chunk step
+  const uint32_t *kp, *vp;     // one word per lane
+};
+
+// Starts the copy of the next 32 keys, `left` of which are there; zeros for the others.
+template <int D>
+__device__ __forceinline__ void fetch(uint32_t stage, Source<D>& src, int left) {
   using S = Stage<D>;
   const int lane = threadIdx.x & 31, r = lane / S::CHUNKS, c = lane % S::CHUNKS;
   const uint32_t to = stage + r * S::ROW + ((c ^ S::turn(r)) << 4);  // the turn is the same 8 and 16 rows on
-  const size_t from = (size_t)key0 * S::ROW + lane * 16;
-  const int left = most - key0;
-  const bool whole = left >= 32;
+  if (left >= 32) {
 #pragma unroll
-  for (int i = 0; i < S::CHUNKS; ++i) {
-    const bool there = whole || r + i * (32 / S::CHUNKS) < left;
-    copy_async<16>(to + S::K + i * 512, there ? kc + from + i * 512 : kc, there);
-    copy_async<16>(to + S::V + i * 512, there ? vc + from + i * 512 : vc, there);
+    for (int i = 0; i < S::CHUNKS; ++i) {
+      copy_async<16>(to + S::K + i * 512, src.kc + i * 512, true);
+      copy_async<16>(to + S::V + i * 512, src.vc + i * 512, true);
+    }
+    copy_async<4>(stage + S::KP + 4 * lane, src.kp, true);
+    copy_async<4>(stage + S::VP + 4 * lane, src.vp, true);
+  } else if (left > 0) {
+#pragma unroll
+    for (int i = 0; i < S::CHUNKS; ++i) {
+      const bool there = r + i * (32 / S::CHUNKS) < left;
+      const int step = there ? i * 512 : -(lane * 16);  // the tile's first bytes, of which nothing is read
+      copy_async<16>(to + S::K + i * 512, src.kc + step, there);
+      copy_async<16>(to + S::V + i * 512, src.vc + step, there);
+    }
+    const bool there = lane < left;
+    copy_async<4>(stage + S::KP + 4 * lane, src.kp - (there ? 0 : lane), there);
+    copy_async<4>(stage + S::VP + 4 * lane, src.vp - (there ? 0 : lane), there);
   }
-  const bool there = lane < left;
-  copy_async<4>(stage + S::KP + 4 * lane, there ? kp + key0 + lane : kp, there);
-  copy_async<4>(stage + S::VP + 4 * lane, there ? vp + key0 + lane : vp, there);
+  src.kc += kTile * S::ROW, src.vc += kTile * S::ROW;
+  src.kp += kTile, src.vp += kTile;
 }
 
 template <int D, int NT, bool FP16>
@@ -253,7 +270,8 @@ __device__ __forceinline__ void rows_step(RowsState<D, NT, FP16>& st, uint32_t s
       }
     }
   }
-  // scale, mask, running maximum
+  // scale, mask, running maximum.  O is rescaled only when a row's maximum grew by more than 2^8: P is at
+  // most 256 then, which costs no bits in floating point
   float vs[4], mn[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) mn[n][0] = st.m[n][0], mn[n][1] = st.m[n][1];
@@ -282,7 +300,7 @@ __device__ __forceinline__ void rows_step(RowsState<D, NT, FP16>& st, uint32_t s
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) mn[n][j] = fmaxf(mn[n][j], __shfl_xor_sync(~0u, mn[n][j], x));
-      moved |= mn[n][j] > st.m[n][j];
+      moved |= mn[n][j] > st.m[n][j] + 8.f;
     }
   if (__any_sync(~0u, moved)) {
 #pragma unroll
@@ -293,7 +311,7 @@ __device__ __forceinline__ void rows_step(RowsState<D, NT, FP16>& st, uint32_t s
         f[j] = mn[n][j] == -INFINITY ? 1.f : ex2(st.m[n][j] - mn[n][j]);
         st.l[n][j] *= f[j];
         st.m[n][j] = mn[n][j];
-      }
+      }  // all rows are brought up to date when one has to be
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
         st.o[n][i][0] *= f[0], st.o[n][i][1] *= f[1];
@@ -397,13 +415,19 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
     const uint32_t* kp = c.param[0] + head * c.C;
     const uint32_t* vp = c.param[1] + head * c.C;
 
-    auto start = [&](int tile) {
-      const int key0 = tile * kTile + warp * 32;
-      if (tile < t1 && key0 < most) fetch<D>(ring + (tile - t0) % S::COUNT * S::BYTES, kc, vc, kp, vp, key0, most);
+    const int first_key = t0 * kTile + warp * 32;
+    Source<D> src = {kc + (size_t)first_key * S::ROW + lane * 16, vc + (size_t)first_key * S::ROW + lane * 16,
+                     kp + first_key + lane, vp + first_key + lane};
+    const int end = min(most, t1 * kTile);
+    int fetched = first_key, to_stage = 0;
+    auto start = [&] {
+      fetch<D>(ring + to_stage * S::BYTES, src, end - fetched);
       copies_commit();
+      fetched += kTile;
+      to_stage = to_stage + 1 == S::COUNT ? 0 : to_stage + 1;
     };
 #pragma unroll
-    for (int i = 0; i < S::COUNT - 1; ++i) start(t0 + i);
+    for (int i = 0; i < S::COUNT - 1; ++i) start();
 
     RowsState<D, NT, FP16> st;
     int least = INT_MAX;  // positions that every row sees
@@ -411,14 +435,19 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
     for (int n = 0; n < NT; ++n) {
       const int row = row0 + 8 * n + g, tok = a.tok0 + row / a.rep;
       const bool live = row < p.rows && tok < sp.fresh;
-      const uint16_t* q = (const uint16_t*)a.q + (live ? z * a.qs[0] + (h * a.rep + row % a.rep) * a.qs[1] + tok * a.qs[2] : 0);
+      const uint16_t* q = (const uint16_t*)a.q + (live ? z * a.qs[0] + (h * a.rep + row % a.rep) * a.qs[1] + tok * a.qs[2] : 0) + t * (D / 4);
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int d = t * (D / 4) + 8 * (s >> 1) + 2 * (s & 1) + j;
-          st.q[n][s][j] = live ? (uint32_t)__ldg(q + d) | ((uint32_t)__ldg(q + d + 4) << 16) : 0u;
+      for (int s = 0; s < D / 16; s += 2) {  // 8 elements: pairs d, d + 4
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (live && p.vec_q) {
+          x = __ldg(reinterpret_cast<const uint4*>(q + 4 * s));
+        } else if (live) {
+          const uint16_t* e = q + 4 * s;
+          x = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
         }
+        st.q[n][s][0] = __byte_perm(x.x, x.z, 0x5410), st.q[n][s][1] = __byte_perm(x.x, x.z, 0x7632);
+        st.q[n][s + 1][0] = __byte_perm(x.y, x.w, 0x5410), st.q[n][s + 1][1] = __byte_perm(x.y, x.w, 0x7632);
+      }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int r = row0 + 8 * n + 2 * t + j, tk = a.tok0 + r / a.rep;
@@ -440,7 +469,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
     for (int tile = t0; tile < t1; ++tile) {
       copies_wait<S::COUNT - 2>();
       __syncwarp();  // this tile's copies are there for all lanes, and all have left the stage that is filled next
-      start(tile + S::COUNT - 1);
+      start();
       const int key0 = tile * kTile + warp * 32;
       const uint32_t stage = ring + at_stage * S::BYTES;
       at_stage = at_stage + 1 == S::COUNT ? 0 : at_stage + 1;
@@ -468,31 +497,37 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
     __syncthreads();
     const bool whole = t0 == 0 && t1 == tiles;
     float* part = p.parts + ((size_t)blockIdx.x * 2 + (piece ? 1 : 0)) * (R * (D + 2));
-    for (int e = tid; e < R * D; e += kWarps * 32) {
-      const int r = e / D, d = e % D, row = row0 + r;
+    for (int e = tid; e < R * (D / 4); e += kWarps * 32) {
+      const int r = e / (D / 4), d = e % (D / 4) * 4, row = row0 + r;
       if (row >= p.rows) break;
       float mm = sm[0][r];
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) mm = fmaxf(mm, sm[w][r]);
-      float ll = 0.f, oo = 0.f;
+      float ll = 0.f;
+      float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         // a warp that saw no key of this row holds l = 0 and O = 0; one that saw only NaN holds NaN
         const float f = sm[w][r] == -INFINITY ? 1.f : ex2(sm[w][r] - mm);
+        const float4 x = *reinterpret_cast<const float4*>(&so[w][r][d]);
         ll += sl[w][r] * f;
-        oo += so[w][r][d] * f;
+        oo.x += x.x * f, oo.y += x.y * f, oo.z += x.z * f, oo.w += x.w * f;
       }
       if (whole) {
         const int tok = a.tok0 + row / a.rep;
-        const float y = sp.limit(a, tok) > 0 ? oo / ll : 0.f;
+        const bool seen = sp.limit(a, tok) > 0;
+        const float inv = 1.f / ll, y[4] = {seen ? oo.x * inv : 0.f, seen ? oo.y * inv : 0.f, seen ? oo.z * inv : 0.f, seen ? oo.w * inv : 0.f};
         const size_t to = z * a.os[0] + (h * a.rep + row % a.rep) * a.os[1] + tok * a.os[2] + d;
-        if (FP16)
-          ((__half*)a.out)[to] = __float2half_rn(y);
-        else
-          ((__nv_bfloat16*)a.out)[to] = __float2bfloat16_rn(y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (FP16)
+            ((__half*)a.out)[to + i] = __float2half_rn(y[i]);
+          else
+            ((__nv_bfloat16*)a.out)[to + i] = __float2bfloat16_rn(y[i]);
+        }
         if (d == 0 && p.scores) p.stats[(head * p.row_tiles + unit % p.row_tiles) * R + r] = make_float2(mm, ll);
       } else {
-        part[2 * R + r * D + d] = oo;
+        *reinterpret_cast<float4*>(part + 2 * R + r * D + d) = oo;
         if (d == 0) part[r] = mm, part[R + r] = ll;
       }
     }
@@ -692,6 +727,7 @@ int attend_rows(const AttendArgs& a0, bool fp16, void* ws, int dev, cudaStream_t
     r.rows = p.rows;
     r.row_tiles = p.row_tiles;
     r.score_rows = p.score_rows;
+    r.vec_q = (((uintptr_t)a0.q | (a0.qs[0] * 2) | (a0.qs[1] * 2) | (a0.qs[2] * 2)) & 15) == 0;
     r.parts = (float*)ws;
     r.stats = (float2*)(r.parts + most.parts);
     r.scores = weights ? r.parts + most.parts + most.stats : nullptr;
