@@ -50,6 +50,7 @@ struct RowsArgs {
   int rows;       // ntok * rep
   int row_tiles;  // ceil(rows / (8 NT))
   int grid;       // CTAs of the first kernel
+  uint32_t magic_k, magic_v;
   bool vec_q;     // query rows start on 16-byte boundaries
   int score_rows; // rows rounded up to even: the score buffer's row length
   float* parts;   // [grid][2][8 NT (D + 2)]: m, l, O of a piece
@@ -83,11 +84,15 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return y;
 }
 // Codes (low 4 bits of both halves) as numbers minus `zero`, exact: the code is
-// set into the mantissa of 128 (bf16) or 1024 (fp16), `zero` is 128 (1024) + zero point.
+// set into the mantissa of 128 (bf16) or 1024 (fp16), `zero` is 128 (1024) +
+// zero point.  `magic`, 128 or 1024 twice, comes from the kernel's arguments: as
+// a known constant it and the mask became an instruction each (lop3 takes one
+// immediate), and the integer pipe is what bounds this kernel.
+constexpr uint32_t kMagicBf16 = 0x43004300u, kMagicFp16 = 0x64006400u;
 template <bool FP16>
-__device__ __forceinline__ uint32_t code_pair(uint32_t x, uint32_t zero) {
-  const uint32_t m = (x & 0x000f000fu) | (FP16 ? 0x64006400u : 0x43004300u);
-  uint32_t y;
+__device__ __forceinline__ uint32_t code_pair(uint32_t x, uint32_t magic, uint32_t zero) {
+  uint32_t m, y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(m) : "r"(x), "r"(0x000f000fu), "r"(magic));  // (x & mask) | magic
   if (FP16)
     asm("sub.f16x2 %0, %1, %2;" : "=r"(y) : "r"(m), "r"(zero));
   else
@@ -217,7 +222,7 @@ struct RowsState {
 // One stage of 32 keys.  FULL: every row sees all of them.
 template <int D, int NT, bool FP16, bool FULL>
 __device__ __forceinline__ void rows_step(RowsState<D, NT, FP16>& st, uint32_t stage, int key0, int most, float scale_log2e,
-                                          float* scores, int score_rows, int rows_left) {
+                                          uint32_t mk, uint32_t mv, float* scores, int score_rows, int rows_left) {
   using S = Stage<D>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint32_t kpw, vpw;
@@ -259,8 +264,8 @@ __device__ __forceinline__ void rows_step(RowsState<D, NT, FP16>& st, uint32_t s
     for (int i = 0; i < D / 16; ++i) {
       const uint32_t w0 = k0[i >> 1], w1 = k1[i >> 1];
       const int sh = 8 * (i & 1);
-      const uint32_t af[4] = {code_pair<FP16>(w0 >> sh, z0), code_pair<FP16>(w1 >> sh, z1),
-                              code_pair<FP16>(w0 >> (sh + 4), z0), code_pair<FP16>(w1 >> (sh + 4), z1)};
+      const uint32_t af[4] = {code_pair<FP16>(w0 >> sh, mk, z0), code_pair<FP16>(w1 >> sh, mk, z1),
+                              code_pair<FP16>(w0 >> (sh + 4), mk, z0), code_pair<FP16>(w1 >> (sh + 4), mk, z1)};
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         if (FP16)
@@ -359,8 +364,8 @@ __device__ __forceinline__ void rows_step(RowsState<D, NT, FP16>& st, uint32_t s
       for (int i = 0; i < 4; ++i) {  // dims 32 (seg + i / 2) + 4 g + 2 (i & 1), and the next
         const uint32_t a = x[i & 2], b = x[(i & 2) + 1];
         const int sh = 8 * (i & 1);
-        const uint32_t af[4] = {code_pair<false>(a >> sh, z0), code_pair<false>(a >> (sh + 4), z0),
-                                code_pair<false>(b >> sh, z1), code_pair<false>(b >> (sh + 4), z1)};
+        const uint32_t af[4] = {code_pair<false>(a >> sh, mv, z0), code_pair<false>(a >> (sh + 4), mv, z0),
+                                code_pair<false>(b >> sh, mv, z1), code_pair<false>(b >> (sh + 4), mv, z1)};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           mma_bf16(st.o[n][2 * seg + i], af, ph[n][2 * ks], ph[n][2 * ks + 1]);
@@ -474,9 +479,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
       const uint32_t stage = ring + at_stage * S::BYTES;
       at_stage = at_stage + 1 == S::COUNT ? 0 : at_stage + 1;
       if (key0 + 32 <= least)
-        rows_step<D, NT, FP16, true>(st, stage, key0, most, a.scale_log2e, scores, p.score_rows, p.rows - row0);
+        rows_step<D, NT, FP16, true>(st, stage, key0, most, a.scale_log2e, p.magic_k, p.magic_v, scores, p.score_rows, p.rows - row0);
       else if (key0 < most)
-        rows_step<D, NT, FP16, false>(st, stage, key0, most, a.scale_log2e, scores, p.score_rows, p.rows - row0);
+        rows_step<D, NT, FP16, false>(st, stage, key0, most, a.scale_log2e, p.magic_k, p.magic_v, scores, p.score_rows, p.rows - row0);
     }
     copies_wait<0>();
     __syncthreads();
@@ -727,6 +732,8 @@ int attend_rows(const AttendArgs& a0, bool fp16, void* ws, int dev, cudaStream_t
     r.rows = p.rows;
     r.row_tiles = p.row_tiles;
     r.score_rows = p.score_rows;
+    r.magic_k = fp16 ? kMagicFp16 : kMagicBf16;
+    r.magic_v = kMagicBf16;
     r.vec_q = (((uintptr_t)a0.q | (a0.qs[0] * 2) | (a0.qs[1] * 2) | (a0.qs[2] * 2)) & 15) == 0;
     r.parts = (float*)ws;
     r.stats = (float2*)(r.parts + most.parts);
