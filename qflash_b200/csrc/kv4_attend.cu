@@ -30,7 +30,9 @@
 // keys, all tiles are numbered, and the CTAs of one resident wave each take an
 // equal run of them (lengths are known on the device only).  A unit that one
 // CTA holds whole is written by it; pieces go to the workspace with their
-// maximum and sum, and a second kernel joins them in order.
+// maximum and sum, and a second kernel joins them in order.  A unit counts for
+// kBegin tiles more than it has, for its queries and its output: without that a CTA
+// that got many units of a tile each was the last by far.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -44,6 +46,8 @@ constexpr int kTile = 128;        // keys per CTA tile: 4 warps of 32
 constexpr int kWarps = 4;
 constexpr int kGridMax = 148 * 5;  // CTAs of one resident wave at most
 constexpr int kRowsMax = 64;      // query rows (tokens x rep) per launch that accumulates weights
+
+constexpr int kBegin = 2;
 
 struct RowsArgs {
   AttendArgs a;
@@ -61,6 +65,11 @@ struct RowsArgs {
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -100,13 +109,17 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t x, uint32_t magic, uint32
   return y;
 }
 
-// Tiles of all units before sequence z, and of all sequences.  One warp.
-__device__ __forceinline__ void tiles_before(const RowsArgs& p, int z, long long* before, long long* total) {
+// A unit of a sequence that shows `most` positions: its tiles, and what it counts for.
+__device__ __forceinline__ int tiles_of(int most) { return (most + kTile - 1) / kTile; }
+__device__ __forceinline__ int cost_of(int most) { return most > 0 ? tiles_of(most) + kBegin : 0; }
+
+// The cost of all units before sequence z, and of all sequences.  One warp.
+__device__ __forceinline__ void cost_before(const RowsArgs& p, int z, long long* before, long long* total) {
   const int lane = threadIdx.x & 31;
   const long long units = (long long)p.a.c.H * p.row_tiles;
   long long blo = 0, ball = 0;
   for (int i = lane; i < p.a.c.Z; i += 32) {
-    const int t = (span_of(p.a, i).most(p.a) + kTile - 1) / kTile;
+    const int t = cost_of(span_of(p.a, i).most(p.a));
     ball += t;
     if (i < z) blo += t;
   }
@@ -119,14 +132,14 @@ __device__ __forceinline__ void tiles_before(const RowsArgs& p, int z, long long
   *total = ball * units;
 }
 
-// The sequence that holds tile `at`, and the number of its first tile.  One warp.
+// The sequence that holds place `at`, and where it begins.  One warp.
 __device__ __forceinline__ int sequence_of(const RowsArgs& p, long long at, long long* first) {
   const int lane = threadIdx.x & 31;
   const long long units = (long long)p.a.c.H * p.row_tiles;
   long long base = 0;
   for (int z0 = 0; z0 < p.a.c.Z; z0 += 32) {
     const int i = z0 + lane;
-    const long long mine = i < p.a.c.Z ? (long long)((span_of(p.a, i).most(p.a) + kTile - 1) / kTile) * units : 0;
+    const long long mine = i < p.a.c.Z ? (long long)cost_of(span_of(p.a, i).most(p.a)) * units : 0;
     long long sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -275,11 +288,11 @@ __device__ __forceinline__ void rows_step(RowsState<D, NT, FP16>& st, uint32_t s
       }
     }
   }
-  // scale, mask, running maximum.  O is rescaled only when a row's maximum grew by more than 2^8: P is at
-  // most 256 then, which costs no bits in floating point
+  // Scale and mask.  O is rescaled only when a score exceeds its row's maximum so far by more than 8 (in log2):
+  // P is at most 256 else, which costs no bits in floating point, and only then is the maximum formed over threads.
   float vs[4], mn[NT][2];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) mn[n][0] = st.m[n][0], mn[n][1] = st.m[n][1];
+  for (int n = 0; n < NT; ++n) mn[n][0] = mn[n][1] = -INFINITY;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float ks = __shfl_sync(~0u, kscale, 8 * i + g);
@@ -292,7 +305,6 @@ __device__ __forceinline__ void rows_step(RowsState<D, NT, FP16>& st, uint32_t s
       for (int j = 0; j < 2; ++j) {
         x[j] *= ks;
         if (!FULL && key >= st.limit[n][j]) x[j] = -INFINITY;
-        mn[n][j] = fmaxf(mn[n][j], x[j]);
       }
       if (scores && key < most && 8 * n + 2 * t < rows_left)
         *reinterpret_cast<float2*>(scores + (size_t)key * score_rows + 8 * n + 2 * t) = make_float2(x[0], x[1]);
@@ -303,8 +315,7 @@ __device__ __forceinline__ void rows_step(RowsState<D, NT, FP16>& st, uint32_t s
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-#pragma unroll
-      for (int x = 4; x < 32; x <<= 1) mn[n][j] = fmaxf(mn[n][j], __shfl_xor_sync(~0u, mn[n][j], x));
+      mn[n][j] = max3(fmaxf(s[n][0][j], s[n][0][2 + j]), s[n][1][j], s[n][1][2 + j]);
       moved |= mn[n][j] > st.m[n][j] + 8.f;
     }
   if (__any_sync(~0u, moved)) {
@@ -312,11 +323,14 @@ __device__ __forceinline__ void rows_step(RowsState<D, NT, FP16>& st, uint32_t s
     for (int n = 0; n < NT; ++n) {
       float f[2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < 2; ++j) {  // all rows are brought up to date when one has to be
+        mn[n][j] = fmaxf(mn[n][j], st.m[n][j]);
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) mn[n][j] = fmaxf(mn[n][j], __shfl_xor_sync(~0u, mn[n][j], x));
         f[j] = mn[n][j] == -INFINITY ? 1.f : ex2(st.m[n][j] - mn[n][j]);
         st.l[n][j] *= f[j];
         st.m[n][j] = mn[n][j];
-      }  // all rows are brought up to date when one has to be
+      }
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
         st.o[n][i][0] *= f[0], st.o[n][i][1] *= f[1];
@@ -388,7 +402,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
   const AttendArgs& a = p.a;
   const Cache& c = a.c;
   long long before, total;
-  tiles_before(p, 0, &before, &total);
+  cost_before(p, 0, &before, &total);
   const int grid = (int)min((long long)p.grid, total);  // no CTA's run is empty
   if ((int)blockIdx.x >= grid) return;
   long long at = run_start(total, grid, blockIdx.x);
@@ -398,21 +412,22 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
   if (z >= c.Z) return;  // only if lens changed meanwhile
   Span sp = span_of(a, z);
   int most = sp.most(a);
-  int tiles = (most + kTile - 1) / kTile;
   int piece = 0;  // the first piece of a CTA goes to slot 0, a later cut one (its last) to slot 1
   const int units = c.H * p.row_tiles;
   while (at < stop) {
     long long in_z = at - zfirst;
-    while (tiles == 0 || in_z >= (long long)units * tiles) {  // on to the next sequence that has tiles
-      zfirst += (long long)units * tiles;
+    while (most <= 0 || in_z >= (long long)units * cost_of(most)) {  // on to the next sequence that shows anything
+      zfirst += (long long)units * cost_of(most);
       in_z = at - zfirst;
       if (++z >= c.Z) return;
       sp = span_of(a, z);
       most = sp.most(a);
-      tiles = (most + kTile - 1) / kTile;
     }
-    const int unit = (int)(in_z / tiles), t0 = (int)(in_z % tiles);
-    const int t1 = (int)min((long long)tiles, t0 + (stop - at));
+    const int tiles = tiles_of(most), cost = cost_of(most);
+    const int unit = (int)(in_z / cost), u0 = (int)(in_z % cost);  // kBegin places, then the tiles
+    const int u1 = (int)min((long long)cost, u0 + (stop - at)), t0 = max(0, u0 - kBegin), t1 = u1 - kBegin;
+    at += u1 - u0;
+    if (t1 <= t0) continue;
     const int h = unit / p.row_tiles, row0 = (unit % p.row_tiles) * R;
     const size_t head = (size_t)z * c.H + h;
     const uint8_t* kc = c.codes[0] + head * c.C * (D / 2);
@@ -537,7 +552,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
       }
     }
     __syncthreads();
-    at += t1 - t0;
     ++piece;
   }
 }
@@ -563,12 +577,12 @@ __global__ void __launch_bounds__(kJoin) rows_finish_kernel(RowsArgs p) {
   const int chunks = (c.C + kChunk - 1) / kChunk;
   const int zh = weigh ? (blockIdx.x - joins) / chunks : blockIdx.x / p.rows, z = zh / c.H, h = zh % c.H;
   const Span sp = span_of(a, z);
-  const int most = sp.most(a), tiles = (most + kTile - 1) / kTile;
+  const int most = sp.most(a), tiles = tiles_of(most), cost = cost_of(most);
   long long before = 0, total = 0;
-  if (tiles) tiles_before(p, z, &before, &total);
+  if (tiles) cost_before(p, z, &before, &total);
   const int ctas = (int)min((long long)p.grid, total);
-  // The CTAs that hold pieces of a unit whose first tile is `first`, and where CTA k's piece is
-  auto holder = [&](long long tile) { return (int)min(ctas - 1LL, ((tile + 1) * ctas - 1) / total); };
+  // The CTA that holds a place; and where CTA k's piece of a unit that begins at `first` is, c0 its first holder
+  auto holder = [&](long long place) { return (int)min(ctas - 1LL, ((place + 1) * ctas - 1) / total); };
   auto part_of = [&](long long first, int c0, int k) {
     return p.parts + (size_t)(k == c0 && run_start(total, ctas, k) < first ? 2 * k + 1 : 2 * k) * kPart;
   };
@@ -577,8 +591,8 @@ __global__ void __launch_bounds__(kJoin) rows_finish_kernel(RowsArgs p) {
     const int row = blockIdx.x % p.rows, u = row / R, r = row % R, tok = a.tok0 + row / a.rep;
     const size_t to = z * a.os[0] + (h * a.rep + row % a.rep) * a.os[1] + tok * a.os[2];
     const bool seen = sp.limit(a, tok) > 0;
-    const long long first = before + ((long long)h * p.row_tiles + u) * tiles;
-    const int c0 = tiles ? holder(first) : 0, n = tiles ? holder(first + tiles - 1) - c0 + 1 : 0;
+    const long long first = before + ((long long)h * p.row_tiles + u) * cost;
+    const int c0 = tiles ? holder(first + kBegin) : 0, n = tiles ? holder(first + cost - 1) - c0 + 1 : 0;
     if (n == 1) return;  // written by its holder
     constexpr int G = kJoin / D;  // groups of threads that share a row's pieces
     const int d = tid % D, group = tid / D;
@@ -635,8 +649,8 @@ __global__ void __launch_bounds__(kJoin) rows_finish_kernel(RowsArgs p) {
     const bool seen = tiles && sp.limit(a, a.tok0 + row / a.rep) > 0;
     if (seen) {
       const int u = row / R, r = row % R;
-      const long long first = before + ((long long)h * p.row_tiles + u) * tiles;
-      const int c0 = holder(first), n = holder(first + tiles - 1) - c0 + 1;
+      const long long first = before + ((long long)h * p.row_tiles + u) * cost;
+      const int c0 = holder(first + kBegin), n = holder(first + cost - 1) - c0 + 1;
       if (n == 1) {
         const float2 s = p.stats[((size_t)zh * p.row_tiles + u) * R + r];
         mx = s.x, l = s.y;
