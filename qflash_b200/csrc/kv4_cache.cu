@@ -9,6 +9,7 @@
 // rint to even.  A vector of zeros has scale 0; one with an infinity or a NaN
 // has scale NaN (all it stands for is NaN) and codes 0.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv4_common.cuh"
 
@@ -23,6 +24,29 @@ int check_launch(const char* what, unsigned grid) {
 }
 
 // ---------------------------------------------------------------- append
+constexpr int kThreads = 256;
+
+// How threads are shared out: a unit is the keys or the values of a (sequence,
+// head), unit = (z H + h) 2 + kv, and is worked on by 2^log_group threads of a
+// block, so that neither a single token nor a prompt leaves threads idle and no
+// thread divides but once.
+struct Share {
+  int log_group, units;
+  // One resident wave of blocks, which go on to further parts of their units: a block's beginning and end
+  // (lengths, the ticket) cost several microseconds of latency.  work: threads' worth of a unit.
+  dim3 grid(long long work, int per_thread, int blocks) const {
+    const long long group = 1LL << log_group;
+    const unsigned x = (unsigned)((units + (kThreads >> log_group) - 1) / (kThreads >> log_group));
+    const long long parts = (work + group * per_thread - 1) / (group * per_thread);
+    return dim3(x, (unsigned)std::min<long long>(std::min<long long>(parts, 65535), std::max(1u, blocks / x)));
+  }
+};
+static Share share(long long work, long long units, int least) {
+  int lg = 0;
+  while ((1 << lg) < kThreads && (1LL << lg) < std::max<long long>(work, least)) ++lg;
+  return {lg, (int)units};
+}
+
 struct AppendArgs {
   Cache c;
   const void* x[2];
@@ -31,55 +55,151 @@ struct AppendArgs {
   const int32_t* new_lens;
   const int32_t* at;
   bool vec[2];
+  Share share;
 };
 
-constexpr int kThreads = 256;
+// bf16(fp32((hi - lo) / 15)).  The fp32 product is off by at most 3 units in the
+// last place, so only one that lies near a border between bf16 numbers has to be
+// formed in fp64.
+__device__ __forceinline__ float scale_of(float lo, float hi) {
+  const float q = (hi - lo) * (1.f / 15.f);
+  const int below = (int)(__float_as_uint(q) & 0xffffu) - 0x8000;
+  if (q > 1e-30f && q < 1e30f && (below > 8 || below < -8)) return __bfloat162float(__float2bfloat16_rn(q));
+  return __bfloat162float(__float2bfloat16_rn((float)(((double)hi - (double)lo) / 15.0)));
+}
 
-// D / 8 lanes per vector, 8 elements each.
-template <class T, int D>
+// rint(fp32(x / s)) for x and s of 16 bits, and their quotient below 32: t = x inv is
+// off by a few 2^-23 of itself, and the residual x - t s, exact in one fma, takes that
+// to 2^-44.  A quotient n + 1/2 is then hit exactly, and any other quotient of
+// numbers of 11 and 8 bits lies further than that from n + 1/2 (by 2^-17 of itself
+// at least), so rounding it is rounding the exact quotient, and so is rounding the fp32 one.
+__device__ __forceinline__ float quotient16(float x, float s, float inv) {
+  const float t = x * inv;
+  return __fmaf_rn(__fmaf_rn(-t, s, x), inv, t);
+}
+constexpr float kRound = 12582912.f;  // 1.5 2^23: adding it rounds to even like rint, the whole number in the low bits
+
+// The codes of 8 elements, clamp(rint(fp32(x / s)) + zero, 0, 15), one to 4 bits.
+template <bool WIDE>
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s, float inv, bool plain, float zero) {
+  uint32_t word = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float q;
+    if (plain && !WIDE) {
+      q = quotient16(x[i], s, inv);
+    } else {
+      q = x[i] * inv;
+      // fp32 elements: only a product near to a border needs the division itself
+      if (!plain || !(fabsf(q - rintf(q)) < 0.5f - 1e-5f)) q = __fdiv_rn(x[i], s);
+    }
+    // clamp first, between whole numbers; then sums mod 2^32 of what lies above the rounding constant
+    const float c = fminf(fmaxf(q, -zero), 15.f - zero);
+    word += __float_as_uint(__fadd_rn(c, kRound)) << (4 * i);
+  }
+  constexpr uint32_t kOnes = 0x11111111u;
+  return word + ((uint32_t)(int)zero - 0x4b400000u) * kOnes;  // 0x4b400000: kRound's bits
+}
+
+// Least and greatest of 8 elements and 0.  16-bit elements in pairs; NaN stays.
+template <class T>
+__device__ __forceinline__ void range8(const T (&r)[8], float& lo, float& hi) {
+  if constexpr (sizeof(T) == 4) {
+    lo = hi = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      asm("min.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(r[i]));
+      asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(r[i]));
+    }
+  } else {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(r);
+    uint32_t l = 0, h = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __half>::value) {
+        asm("min.NaN.f16x2 %0, %0, %1;" : "+r"(l) : "r"(w[i]));
+        asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(h) : "r"(w[i]));
+      } else {
+        asm("min.NaN.bf16x2 %0, %0, %1;" : "+r"(l) : "r"(w[i]));
+        asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(h) : "r"(w[i]));
+      }
+    }
+    const T* lp = reinterpret_cast<const T*>(&l);
+    const T* hp = reinterpret_cast<const T*>(&h);
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(lo) : "f"(to_float(lp[0])), "f"(to_float(lp[1])));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(hi) : "f"(to_float(hp[0])), "f"(to_float(hp[1])));
+  }
+}
+
+// D / 8 lanes per vector, 8 elements each; a thread holds U vectors' elements at
+// once.  Bound by the bytes of the floats it reads.
+template <class T, int D, int U>
 __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
   constexpr int L = D / 8;
   const Cache& c = a.c;
-  const int lane = threadIdx.x % L;
-  const unsigned row = blockIdx.x * (kThreads / L) + threadIdx.x / L;
-  const unsigned n = row % a.N, rest = row / a.N, h = rest % c.H, kv = rest / c.H & 1, z = rest / c.H / 2;
-  if (z < (unsigned)c.Z) {  // whole groups of L lanes leave together
-    const int base = a.at ? a.at[z] : c.lens[z];
-    const int fresh = a.new_lens ? min(max(a.new_lens[z], 0), a.N) : a.N;
-    const long long pos = (long long)base + n;
-    if ((int)n < fresh && pos >= 0 && pos < c.C) {
-      float x[8];
-      load8((const T*)a.x[kv] + z * a.st[kv][0] + h * a.st[kv][1] + n * a.st[kv][2] + lane * 8, a.vec[kv], x);
-      float lo = 0.f, hi = 0.f;
-      bool bad = false;
+  const int lg = a.share.log_group, in_group = threadIdx.x & ((1 << lg) - 1), lane = threadIdx.x % L;
+  const int unit = blockIdx.x * (kThreads >> lg) + (threadIdx.x >> lg);
+  const bool there = unit < a.share.units;
+  const int kv = unit & 1, zh = min(unit, a.share.units - 1) >> 1, z = zh / c.H, h = zh - z * c.H;
+  const int base = a.at ? a.at[z] : c.lens[z];
+  const int fresh = there ? (a.new_lens ? min(max(a.new_lens[z], 0), a.N) : a.N) : 0;
+  const T* x0 = (const T*)(kv ? a.x[1] : a.x[0]) + z * (kv ? a.st[1][0] : a.st[0][0]) + h * (kv ? a.st[1][1] : a.st[0][1]) + lane * 8;
+  const int64_t x_step = kv ? a.st[1][2] : a.st[0][2];
+  const bool vec = kv ? a.vec[1] : a.vec[0];
+  uint32_t* codes = reinterpret_cast<uint32_t*>(kv ? c.codes[1] : c.codes[0]);
+  uint32_t* param = kv ? c.param[1] : c.param[0];
+  const size_t head = (size_t)zh * c.C;
+  const int per = (1 << lg) / L;  // vectors of a group's step
+  const unsigned group = (L == 32 ? ~0u : (1u << L) - 1) << (threadIdx.x % 32 / L * L);
+  for (int n0 = (blockIdx.y * U) * per + in_group / L; n0 < fresh; n0 += gridDim.y * U * per) {
+    alignas(16) T r[U][8];
+    bool in[U];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, x[i]);
-        bad |= !(fabsf(x[i]) < INFINITY);
+    for (int u = 0; u < U; ++u) {
+      const int n = n0 + u * per;
+      const long long pos = (long long)base + n;
+      in[u] = n < fresh && pos >= 0 && pos < c.C;
+      if (in[u]) {
+        const T* from = x0 + n * x_step;
+        if (vec) {
+#pragma unroll
+          for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+            reinterpret_cast<uint4*>(r[u])[i] = __ldg(reinterpret_cast<const uint4*>(from) + i);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) r[u][i] = from[i];
+        }
       }
-      const unsigned group = (L == 32 ? ~0u : (1u << L) - 1) << (threadIdx.x % 32 / L * L);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!in[u]) continue;  // the vector's lanes together
+      float lo, hi;
+      range8(r[u], lo, hi);
 #pragma unroll
       for (int o = L / 2; o; o >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(group, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(group, hi, o));
+        asm("min.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(__shfl_xor_sync(group, lo, o)));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(__shfl_xor_sync(group, hi, o)));
       }
-      bad = __any_sync(group, bad);
-      __nv_bfloat16 scale = __float2bfloat16_rn((float)(((double)hi - (double)lo) / 15.0));
-      if (bad) scale = __ushort_as_bfloat16(0x7fc0);
-      const float s = __bfloat162float(scale);
+      const bool good = lo > -INFINITY && hi < INFINITY;  // no infinity, no NaN
+      const float s = good ? scale_of(lo, hi) : __uint_as_float(0x7fc00000u);
       float zero = 0.f;
       uint32_t word = 0;
       if (s > 0.f) {
-        zero = fminf(rintf(__fdiv_rn(-lo, s)), 15.f);
+        const bool plain = s > 1e-30f && s < 1e30f;
+        float inv, x[8];
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          word |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x[i], s)) + zero, 0.f), 15.f) << (4 * i);
+        for (int i = 0; i < 8; ++i) x[i] = to_float(r[u][i]);
+        constexpr bool kWide = sizeof(T) == 4;
+        zero = rintf(plain && !kWide ? quotient16(-lo, s, inv) : __fdiv_rn(-lo, s));
+        zero = fminf(fmaxf(zero, 0.f), 15.f);
+        word = codes_of<kWide>(x, s, inv, plain, zero);
       }
-      const size_t to = ((size_t)z * c.H + h) * c.C + pos;
-      reinterpret_cast<uint32_t*>(c.codes[kv])[to * (D / 8) + lane] = word;
+      const size_t to = head + (base + n0 + u * per);
+      codes[to * L + lane] = word;
       if (lane == 0) {
-        c.param[kv][to] = (uint32_t)__bfloat16_as_ushort(scale) | (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(zero)) << 16;
+        param[to] = __float_as_uint(s) >> 16 | __float_as_uint(zero) & 0xffff0000u;
         if (kv == 0) c.weight[to] = 0.f;
       }
     }
@@ -89,14 +209,14 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
   __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();
-    last = atomicAdd(&c.ctl[0], 1) == (int)gridDim.x - 1;
+    last = atomicAdd(&c.ctl[0], 1) == (int)(gridDim.x * gridDim.y) - 1;
   }
   __syncthreads();
   if (!last) return;
   for (int i = threadIdx.x; i < c.Z; i += kThreads) {
-    const int base = a.at ? a.at[i] : c.lens[i];
-    const long long end = (long long)base + (a.new_lens ? min(max(a.new_lens[i], 0), a.N) : a.N);
-    if (base < 0 || end > c.C) atomicOr(&c.ctl[1], 1);
+    const int first = a.at ? a.at[i] : c.lens[i];
+    const long long end = (long long)first + (a.new_lens ? min(max(a.new_lens[i], 0), a.N) : a.N);
+    if (first < 0 || end > c.C) atomicOr(&c.ctl[1], 1);
     c.lens[i] = (int)min(max(end, 0LL), (long long)c.C);
   }
   if (threadIdx.x == 0) c.ctl[0] = 0;
@@ -108,26 +228,76 @@ struct ReadArgs {
   void* out[2];
   int N;
   const int32_t* start;
+  Share share;
 };
 
-template <class T, int D>
+__device__ __forceinline__ uint32_t pair_sub(uint32_t a, uint32_t b) {
+  uint32_t y;
+  asm("sub.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+__device__ __forceinline__ uint32_t pair_mul(uint32_t a, uint32_t b) {
+  uint32_t y;
+  asm("mul.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+
+// The 8 values of a word of codes.  code - zero is exact in bf16 (set into the
+// mantissa of 128), and so is scale * (code - zero) in fp32: one rounding, to T.
+template <class T>
+__device__ __forceinline__ void put_values(T* out, uint32_t w, uint32_t param) {
+  const uint32_t z1 = __float_as_uint(128.f + param_zero(param)) >> 16, zero = z1 | z1 << 16;
+  uint32_t y[4];  // elements i and i + 4
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = pair_sub(w >> (4 * i) & 0x000f000fu | 0x43004300u, zero);
+  if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
+    const uint32_t s = __byte_perm(param, param, 0x1010);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = pair_mul(y[i], s);
+    *reinterpret_cast<uint4*>(out) = make_uint4(__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410),
+                                                __byte_perm(y[0], y[1], 0x7632), __byte_perm(y[2], y[3], 0x7632));
+  } else {
+    const float s = param_scale(param);
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = s * __uint_as_float(y[i] << 16);
+      x[i + 4] = s * __uint_as_float(y[i] & 0xffff0000u);
+    }
+    store8(out, true, x);
+  }
+}
+
+// A unit's words are in one run, and so are its values: a thread takes U words
+// of 8 codes (coalesced 4 bytes in, 16 out), loads before stores.
+template <class T, int D, int U>
 __global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs a) {
   constexpr int L = D / 8;
   const Cache& c = a.c;
-  const int lane = threadIdx.x % L;
-  const unsigned row = blockIdx.x * (kThreads / L) + threadIdx.x / L;
-  const unsigned n = row % a.N, rest = row / a.N, h = rest % c.H, kv = rest / c.H & 1, z = rest / c.H / 2;
-  if (z >= (unsigned)c.Z) return;
-  const long long pos = (a.start ? (long long)a.start[z] : 0) + n;
-  float y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (pos >= 0 && pos < length_of(c, z)) {
-    const size_t at = ((size_t)z * c.H + h) * c.C + pos;
-    const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(c.codes[kv]) + at * (D / 8) + lane), p = __ldg(c.param[kv] + at);
-    const float s = param_scale(p), zero = param_zero(p);
+  const int lg = a.share.log_group, in_group = threadIdx.x & ((1 << lg) - 1);
+  const int unit = blockIdx.x * (kThreads >> lg) + (threadIdx.x >> lg);
+  if (unit >= a.share.units) return;
+  const int kv = unit & 1, zh = unit >> 1, z = zh / c.H;
+  const int first = a.start ? a.start[z] : 0, len = length_of(c, z);
+  const uint32_t* codes = reinterpret_cast<const uint32_t*>(kv ? c.codes[1] : c.codes[0]) + (size_t)zh * c.C * L;
+  const uint32_t* param = (kv ? c.param[1] : c.param[0]) + (size_t)zh * c.C;
+  T* out = (T*)(kv ? a.out[1] : a.out[0]) + (size_t)zh * a.N * D;
+  const long long words = (long long)a.N * L, step = (long long)gridDim.y * U << lg;
+  for (long long w0 = ((long long)blockIdx.y * U << lg) + in_group; w0 < words; w0 += step) {
+    uint32_t w[U], p[U];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = s * ((float)(w >> (4 * i) & 15) - zero);  // 13 bits: exact in fp32
+    for (int u = 0; u < U; ++u) {
+      const long long i = w0 + ((long long)u << lg), pos = first + i / L;
+      const bool in = i < words && pos >= 0 && pos < len;
+      w[u] = in ? __ldg(codes + pos * L + i % L) : 0u;
+      p[u] = in ? __ldg(param + pos) : 0u;  // scale 0
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long i = w0 + ((long long)u << lg);
+      if (i < words) put_values(out + i * 8, w[u], p[u]);
+    }
   }
-  store8((T*)a.out[kv] + (((size_t)z * c.H + h) * a.N + n) * D + lane * 8, true, y);
 }
 
 // ---------------------------------------------------------------- evict
@@ -144,96 +314,205 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Which positions stay, one CTA per (sequence, head): a radix selection finds
-// the least weight that stays (4 passes of 8 bits), then one pass in order
-// lists the heavier positions, the first of the equal ones and the last tokens.
+// Which positions stay, a cluster of CTAs per (sequence, head), each with a run
+// of the positions: a radix selection over digits of 11, 11 and 10 bits finds the
+// least weight that stays, then the heavier positions, the first of the equal ones
+// and the last tokens are listed in order.  The CTAs add up their counts through
+// shared memory of the cluster.  A run of up to 16384 positions is read once and
+// kept in registers; latency bounds this kernel, not bytes.
 constexpr int kSelect = 1024;
+constexpr int kKeep = 16;  // positions per thread and tile
+constexpr int kDigits = 2048;
+constexpr int kCluster = 8;
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// CTA `rank`'s copy of a word of shared memory
+__device__ __forceinline__ uint32_t peer_word(const uint32_t* p, uint32_t rank) {
+  uint32_t at, v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at));
+  return v;
+}
 
 __global__ void __launch_bounds__(kSelect) evict_select_kernel(EvictArgs a) {
-  __shared__ unsigned hist[256];
-  __shared__ unsigned warp_sum[2][32];
-  __shared__ unsigned s_prefix, s_left;
-  const int zh = blockIdx.x, z = zh / a.from.H, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int W = kSelect / 32, PER = kDigits / kSelect, TILE = kSelect * kKeep;
+  __shared__ uint32_t hist[2][kDigits];  // of even and odd passes: peers may still read the last pass's
+  __shared__ uint32_t sums[W], counts[2], s_digit, s_left;
+  __shared__ uint32_t warp_more[W], warp_same[W];
+  const int cs = (int)cluster_size(), rank = (int)cluster_rank();
+  const int zh = blockIdx.x / cs, z = zh / a.from.H, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n = length_of(a.from, z);
   int32_t* kept = a.kept + (size_t)zh * a.budget;
   const float* weight = a.from.weight + (size_t)zh * a.from.C;
-  if (zh % a.from.H == 0 && tid == 0) a.to.lens[z] = min(n, a.budget);
-  if (n <= a.budget) {
-    for (int i = tid; i < a.budget; i += kSelect) kept[i] = i < n ? i : -1;
+  if (zh % a.from.H == 0 && rank == 0 && tid == 0) a.to.lens[z] = min(n, a.budget);
+  const int stride = cs * kSelect, mine = rank * kSelect + tid;
+  if (n <= a.budget) {  // all CTAs of the cluster return together
+    for (int i = mine; i < a.budget; i += stride) kept[i] = i < n ? i : -1;
     return;
   }
   const int old = n - a.recent, need = a.budget - a.recent;
-  for (int i = tid; i < a.recent; i += kSelect) kept[need + i] = old + i;
+  for (int i = mine; i < a.recent; i += stride) kept[need + i] = old + i;
   if (need == 0) return;
+  const int run = (old + cs - 1) / cs, i0 = min(old, rank * run), i1 = min(old, i0 + run);
+  const bool once = run <= TILE;
+  // a warp holds kKeep * 32 neighbouring positions: position at(t, j) of tile t in u[j]
+  uint32_t u[kKeep];
+  auto at = [&](int t, int j) { return i0 + t * TILE + (warp * kKeep + j) * 32 + lane; };
+  auto load = [&](int t) {
+    float w[kKeep];
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j) w[j] = at(t, j) < i1 ? __ldg(weight + at(t, j)) : 0.f;
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j) u[j] = order_of(w[j]);
+  };
+  const int tiles = (i1 - i0 + TILE - 1) / TILE;
   uint32_t prefix = 0, left = need;  // among weights that begin with prefix, the left-th largest is looked for
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    uint32_t* h = hist[pass & 1];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) h[i * kSelect + tid] = 0;
+    if (tid < 2) counts[tid] = 0;
     __syncthreads();
-    for (int i = tid; i < old; i += kSelect) {
-      const uint32_t u = order_of(weight[i]);
-      if (shift == 24 || u >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&hist[u >> shift & 255], 1u);
+    for (int t = 0; t < tiles; ++t) {
+      if (pass == 0 || !once) load(t);
+#pragma unroll
+      for (int j = 0; j < kKeep; ++j)
+        if (at(t, j) < i1 && (pass == 0 || u[j] >> (shift + bits) == prefix >> (shift + bits)))
+          atomicAdd(&h[u[j] >> shift & ((1 << bits) - 1)], 1u);
+    }
+    if (cs > 1) cluster_sync(); else __syncthreads();
+    // thread t holds digits from the top: kDigits - 1 - PER t downwards
+    uint32_t d[PER], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) d[i] = 0;
+    if (cs == 1) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) d[i] = h[kDigits - 1 - PER * tid - i];
+    } else {
+      uint32_t x[kCluster][PER];  // all on their way before the first is added
+#pragma unroll
+      for (int r = 0; r < kCluster; ++r)
+#pragma unroll
+        for (int i = 0; i < PER; ++i) x[r][i] = r < cs ? peer_word(h + kDigits - 1 - PER * tid - i, r) : 0;
+#pragma unroll
+      for (int r = 0; r < kCluster; ++r)
+#pragma unroll
+        for (int i = 0; i < PER; ++i) d[i] += x[r][i];
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sum += d[i];
+    uint32_t upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(~0u, upto, o);
+      if (lane >= o) upto += up;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    upto += __reduce_add_sync(~0u, lane < warp ? sums[lane] : 0u);
+    uint32_t above = upto - sum;
+    if (above < left && left <= upto) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (above < left && left <= above + d[i]) s_digit = kDigits - 1 - PER * tid - i, s_left = left - above;
+        above += d[i];
+      }
     }
     __syncthreads();
-    if (warp == 0) {
-      // lane holds digits 255 - 8 lane .. 248 - 8 lane
-      unsigned mine = 0;
-      for (int i = 0; i < 8; ++i) mine += hist[255 - 8 * lane - i];
-      unsigned sum = mine;
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned up = __shfl_up_sync(~0u, sum, o);
-        if (lane >= o) sum += up;
-      }
-      unsigned above = sum - mine;
-      if (above < left && left <= sum) {
-        int d = 255 - 8 * lane;
-        while (above + hist[d] < left) above += hist[d--];
-        s_prefix = prefix | (uint32_t)d << shift;
-        s_left = left - above;
-      }
+    prefix |= s_digit << shift, left = s_left;
+  }
+  // heavier and equal positions of a warp's part of a tile
+  auto count = [&](int t, uint32_t& more, uint32_t& same) {
+    more = same = 0;
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j) {
+      const bool in = at(t, j) < i1;
+      more += __popc(__ballot_sync(~0u, in && u[j] > prefix));
+      same += __popc(__ballot_sync(~0u, in && u[j] == prefix));
     }
+  };
+  // how many of them the CTAs before this one have
+  uint32_t done = 0, equal = 0, more, same;
+  if (cs > 1) {
+    for (int t = 0; t < tiles; ++t) {
+      if (!once) load(t);
+      count(t, more, same);
+      if (lane == 0) atomicAdd(&counts[0], more), atomicAdd(&counts[1], same);
+    }
+    cluster_sync();
+    for (int r = 0; r < rank; ++r) done += peer_word(&counts[0], r), equal += peer_word(&counts[1], r);
+  }
+  for (int t = 0; t < tiles; ++t) {
+    if (!once) load(t);
+    count(t, more, same);
+    if (lane == 0) warp_more[warp] = more, warp_same[warp] = same;
     __syncthreads();
-    prefix = s_prefix, left = s_left;
+    const uint32_t m = warp_more[lane], e = warp_same[lane];  // kSelect / 32 is 32
+    uint32_t pm = done + __reduce_add_sync(~0u, lane < warp ? m : 0u), ps = equal + __reduce_add_sync(~0u, lane < warp ? e : 0u);
+    done += __reduce_add_sync(~0u, m), equal += __reduce_add_sync(~0u, e);
+    const unsigned below = (1u << lane) - 1;
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j) {
+      const bool in = at(t, j) < i1, heavy = in && u[j] > prefix, even = in && u[j] == prefix;
+      const unsigned bm = __ballot_sync(~0u, heavy), be = __ballot_sync(~0u, even);
+      const uint32_t em = pm + __popc(bm & below), es = ps + __popc(be & below);
+      // rank among the kept: heavier ones before, and equal ones before as far as they stay
+      if (heavy || (even && es < left)) kept[em + min(es, left)] = at(t, j);
+      pm += __popc(bm), ps += __popc(be);
+    }
     __syncthreads();
   }
-  // `left` of the weights equal to prefix stay: the first ones
-  unsigned done = 0, equal = 0;
-  for (int i0 = 0; i0 < old; i0 += kSelect) {
-    const int i = i0 + tid;
-    const uint32_t u = i < old ? order_of(weight[i]) : 0u;
-    const bool more = i < old && u > prefix, same = i < old && u == prefix;
-    const unsigned bm = __ballot_sync(~0u, more), bs = __ballot_sync(~0u, same), below = (1u << lane) - 1;
-    if (lane == 0) warp_sum[0][warp] = __popc(bm), warp_sum[1][warp] = __popc(bs);
-    __syncthreads();
-    unsigned pm = 0, ps = 0, tm = 0, ts = 0;
-    for (int w = 0; w < kSelect / 32; ++w) {
-      const unsigned x = warp_sum[0][w], y = warp_sum[1][w];
-      if (w < warp) pm += x, ps += y;
-      tm += x, ts += y;
-    }
-    const unsigned em = done + pm + __popc(bm & below), es = equal + ps + __popc(bs & below);
-    // rank among the kept: heavier ones before, and equal ones before as far as they stay
-    if (more || (same && es < left)) kept[em + min(es, left)] = i;
-    done += tm, equal += ts;
-    __syncthreads();
-  }
+  if (cs > 1) cluster_sync();  // no CTA's shared memory goes while a peer may read it
 }
 
-// Moves what stays: D / 32 lanes of 16 bytes for the key and as many for the value.
+// Moves what stays: D / 32 lanes of 16 bytes for the key and as many for the
+// value, kMove positions at once.
+constexpr int kMove = 4;
 template <int D>
 __global__ void __launch_bounds__(kThreads) evict_move_kernel(EvictArgs a) {
-  constexpr int L = D / 16;
+  constexpr int L = D / 16, G = kThreads / L;
   const Cache &f = a.from, &t = a.to;
-  const int zh = blockIdx.y, i = blockIdx.x * (kThreads / L) + threadIdx.x / L, lane = threadIdx.x % L;
-  if (i >= a.budget) return;
-  const int src = a.kept[(size_t)zh * a.budget + i];
-  if (src < 0) return;
+  const int zh = blockIdx.y, i0 = blockIdx.x * (G * kMove) + threadIdx.x / L, lane = threadIdx.x % L;
   const int kv = lane / (L / 2), part = lane % (L / 2);
-  const size_t from = (size_t)zh * f.C + src, to = (size_t)zh * t.C + i;
-  reinterpret_cast<uint4*>(t.codes[kv])[to * (D / 32) + part] = __ldg(reinterpret_cast<const uint4*>(f.codes[kv]) + from * (D / 32) + part);
-  if (part == 0) {
-    t.param[kv][to] = __ldg(f.param[kv] + from);
-    if (kv == 0) t.weight[to] = __ldg(f.weight + from);
-  }
+  const uint4* from = reinterpret_cast<const uint4*>(kv ? f.codes[1] : f.codes[0]) + (size_t)zh * f.C * (D / 32) + part;
+  uint4* to = reinterpret_cast<uint4*>(kv ? t.codes[1] : t.codes[0]) + (size_t)zh * t.C * (D / 32) + part;
+  const uint32_t* from_param = (kv ? f.param[1] : f.param[0]) + (size_t)zh * f.C;
+  uint32_t* to_param = (kv ? t.param[1] : t.param[0]) + (size_t)zh * t.C;
+  int src[kMove];
+  uint4 x[kMove];
+  uint32_t p[kMove];
+  float w[kMove];
+#pragma unroll
+  for (int k = 0; k < kMove; ++k) src[k] = i0 + k * G < a.budget ? __ldg(a.kept + (size_t)zh * a.budget + i0 + k * G) : -1;
+#pragma unroll
+  for (int k = 0; k < kMove; ++k)
+    if (src[k] >= 0) {
+      x[k] = __ldg(from + (size_t)src[k] * (D / 32));
+      if (part == 0) p[k] = __ldg(from_param + src[k]);
+      if (lane == 0) w[k] = __ldg(f.weight + (size_t)zh * f.C + src[k]);
+    }
+#pragma unroll
+  for (int k = 0; k < kMove; ++k)
+    if (src[k] >= 0) {
+      const int i = i0 + k * G;
+      to[(size_t)i * (D / 32)] = x[k];
+      if (part == 0) to_param[i] = p[k];
+      if (lane == 0) t.weight[(size_t)zh * t.C + i] = w[k];
+    }
 }
 
 // ------------------------------------------------------------------ host
@@ -266,25 +545,29 @@ static bool overlap(const void* a, size_t na, const void* b, size_t nb) {
 }
 
 template <class T>
-static int launch_append(const AppendArgs& a, cudaStream_t s) {
-  const unsigned per = kThreads / (a.c.D / 8);
-  const unsigned grid = (unsigned)((2LL * a.c.Z * a.c.H * a.N + per - 1) / per);
+static int launch_append(AppendArgs& a, int sms, cudaStream_t s) {
+  const int L = a.c.D / 8;
+  constexpr int U = 2;
+  a.share = share((long long)a.N * L, 2LL * a.c.Z * a.c.H, L);
+  const dim3 grid = a.share.grid((long long)a.N * L, U, sms * 5);
   if (a.c.D == 64)
-    append_kernel<T, 64><<<grid, kThreads, 0, s>>>(a);
+    append_kernel<T, 64, U><<<grid, kThreads, 0, s>>>(a);
   else
-    append_kernel<T, 128><<<grid, kThreads, 0, s>>>(a);
-  return check_launch("kv4 append", grid);
+    append_kernel<T, 128, U><<<grid, kThreads, 0, s>>>(a);
+  return check_launch("kv4 append", grid.x * grid.y);
 }
 
 template <class T>
-static int launch_read(const ReadArgs& a, cudaStream_t s) {
-  const unsigned per = kThreads / (a.c.D / 8);
-  const unsigned grid = (unsigned)((2LL * a.c.Z * a.c.H * a.N + per - 1) / per);
+static int launch_read(ReadArgs& a, int sms, cudaStream_t s) {
+  const int L = a.c.D / 8;
+  constexpr int U = 4;
+  a.share = share((long long)a.N * L, 2LL * a.c.Z * a.c.H, L);
+  const dim3 grid = a.share.grid((long long)a.N * L, U, sms * 8);
   if (a.c.D == 64)
-    read_kernel<T, 64><<<grid, kThreads, 0, s>>>(a);
+    read_kernel<T, 64, U><<<grid, kThreads, 0, s>>>(a);
   else
-    read_kernel<T, 128><<<grid, kThreads, 0, s>>>(a);
-  return check_launch("kv4 read", grid);
+    read_kernel<T, 128, U><<<grid, kThreads, 0, s>>>(a);
+  return check_launch("kv4 read", grid.x * grid.y);
 }
 
 }  // namespace kv4
@@ -313,7 +596,7 @@ extern "C" int qflash_kv4_append(const qflash_kv4_cache* cache, const void* k, c
   a.vec[0] = aligned16(k, k_strides, dtype), a.vec[1] = aligned16(v, v_strides, dtype);
   a.N = N, a.new_lens = new_lens, a.at = at;
   cudaStream_t s = (cudaStream_t)stream;
-  return dtype == kF32 ? launch_append<float>(a, s) : dtype == kF16 ? launch_append<__half>(a, s) : launch_append<__nv_bfloat16>(a, s);
+  return dtype == kF32 ? launch_append<float>(a, sm_count(dev), s) : dtype == kF16 ? launch_append<__half>(a, sm_count(dev), s) : launch_append<__nv_bfloat16>(a, sm_count(dev), s);
 }
 
 extern "C" int qflash_kv4_read(const qflash_kv4_cache* cache, void* k, void* v, int dtype, int N, const int32_t* start,
@@ -328,9 +611,9 @@ extern "C" int qflash_kv4_read(const qflash_kv4_cache* cache, void* k, void* v, 
   DeviceGuard keep_device;
   int dev = 0;
   if (int rc = select_device(cache->k_codes, &dev)) return rc;
-  const ReadArgs a = {view(cache), {k, v}, N, start};
+  ReadArgs a = {view(cache), {k, v}, N, start, {}};
   cudaStream_t s = (cudaStream_t)stream;
-  return dtype == kF32 ? launch_read<float>(a, s) : dtype == kF16 ? launch_read<__half>(a, s) : launch_read<__nv_bfloat16>(a, s);
+  return dtype == kF32 ? launch_read<float>(a, sm_count(dev), s) : dtype == kF16 ? launch_read<__half>(a, sm_count(dev), s) : launch_read<__nv_bfloat16>(a, sm_count(dev), s);
 }
 
 extern "C" int qflash_kv4_evict(const qflash_kv4_cache* from, const qflash_kv4_cache* to, int budget, int recent,
@@ -358,9 +641,18 @@ extern "C" int qflash_kv4_evict(const qflash_kv4_cache* from, const qflash_kv4_c
   if (int rc = select_device(from->k_codes, &dev)) return rc;
   const EvictArgs a = {view(from), view(to), budget, recent, kept};
   cudaStream_t s = (cudaStream_t)stream;
-  evict_select_kernel<<<(unsigned)heads, kSelect, 0, s>>>(a);
-  if (int rc = check_launch("kv4 evict select", (unsigned)heads)) return rc;
-  const int per = kThreads / (from->D / 16);
+  // CTAs per head: as many as have SMs of their own, as long as each has some thousand positions
+  int cs = 1;
+  while (cs < kCluster && heads * cs * 2 <= (size_t)sm_count(dev) && from->capacity > 4096 * cs) cs *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)heads * cs), cfg.blockDim = dim3(kSelect), cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = cs, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, evict_select_kernel, a);
+  if (int rc = check_launch("kv4 evict select", cfg.gridDim.x)) return rc;
+  const int per = kThreads / (from->D / 16) * kMove;
   const unsigned nx = (unsigned)((budget + per - 1) / per);
   for (size_t h0 = 0; h0 < heads; h0 += 65535) {
     EvictArgs b = a;
