@@ -79,26 +79,13 @@ __device__ __forceinline__ float quotient16(float x, float s, float inv) {
 }
 constexpr float kRound = 12582912.f;  // 1.5 2^23: adding it rounds to even like rint, the whole number in the low bits
 
-// The codes of 8 elements, clamp(rint(fp32(x / s)) + zero, 0, 15), one to 4 bits.
-template <bool WIDE>
-__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s, float inv, bool plain, float zero) {
+// The codes of 8 quotients, clamp(rint(q) + zero, 0, 15), one to 4 bits.
+__device__ __forceinline__ uint32_t codes_of(const float (&q)[8], float zero) {
   uint32_t word = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float q;
-    if (plain && !WIDE) {
-      q = quotient16(x[i], s, inv);
-    } else {
-      q = x[i] * inv;
-      // fp32 elements: only a product near to a border needs the division itself
-      if (!plain || !(fabsf(q - rintf(q)) < 0.5f - 1e-5f)) q = __fdiv_rn(x[i], s);
-    }
-    // clamp first, between whole numbers; then sums mod 2^32 of what lies above the rounding constant
-    const float c = fminf(fmaxf(q, -zero), 15.f - zero);
-    word += __float_as_uint(__fadd_rn(c, kRound)) << (4 * i);
-  }
-  constexpr uint32_t kOnes = 0x11111111u;
-  return word + ((uint32_t)(int)zero - 0x4b400000u) * kOnes;  // 0x4b400000: kRound's bits
+  for (int i = 0; i < 8; ++i)  // clamp first, between whole numbers; then sums mod 2^32 of what lies above the rounding constant
+    word += __float_as_uint(__fadd_rn(fminf(fmaxf(q[i], -zero), 15.f - zero), kRound)) << (4 * i);
+  return word + ((uint32_t)(int)zero - 0x4b400000u) * 0x11111111u;  // 0x4b400000: kRound's bits
 }
 
 // Least and greatest of 8 elements and 0.  16-bit elements in pairs; NaN stays.
@@ -186,15 +173,23 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
       float zero = 0.f;
       uint32_t word = 0;
       if (s > 0.f) {
-        const bool plain = s > 1e-30f && s < 1e30f;
-        float inv, x[8];
+        float inv, q[8];
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+        if (sizeof(T) == 2 && s > 1e-30f && s < 1e30f) {
+          zero = quotient16(-lo, s, inv);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_float(r[u][i]);
-        constexpr bool kWide = sizeof(T) == 4;
-        zero = rintf(plain && !kWide ? quotient16(-lo, s, inv) : __fdiv_rn(-lo, s));
-        zero = fminf(fmaxf(zero, 0.f), 15.f);
-        word = codes_of<kWide>(x, s, inv, plain, zero);
+          for (int i = 0; i < 8; ++i) q[i] = quotient16(to_float(r[u][i]), s, inv);
+        } else {  // fp32 elements: only a product near to a border needs the division itself
+          zero = __fdiv_rn(-lo, s);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float x = to_float(r[u][i]);
+            q[i] = x * inv;
+            if (!(s > 1e-30f && s < 1e30f && fabsf(q[i] - rintf(q[i])) < 0.5f - 1e-5f)) q[i] = __fdiv_rn(x, s);
+          }
+        }
+        zero = fminf(fmaxf(rintf(zero), 0.f), 15.f);
+        word = codes_of(q, zero);
       }
       const size_t to = head + (base + n0 + u * per);
       codes[to * L + lane] = word;
