@@ -44,6 +44,7 @@ struct PromptArgs {
   int rows, row_tiles;  // N * rep, and that over 256
   int grid;
   bool vec_q, vec_o;
+  uint32_t magic_k, magic_v;
   float* parts;   // [grid][2][256 (D + 2)]
   float2* stats;  // [Z H][rows]: maximum (log2 units) and 1 / sum; null without weights
 };
@@ -70,6 +71,24 @@ __device__ __forceinline__ void tmem_ld32f(uint32_t addr, float* r) {
   tmem_ld32(addr, v);
 #pragma unroll
   for (int i = 0; i < 32; ++i) r[i] = __int_as_float(v[i]);
+}
+// 32 lanes x 64 columns of 32 bits, complete when this returns.
+__device__ __forceinline__ void tmem_ld64f(uint32_t addr, float* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+        "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+        "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
+        "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31]),
+        "=f"(r[32]), "=f"(r[33]), "=f"(r[34]), "=f"(r[35]), "=f"(r[36]), "=f"(r[37]), "=f"(r[38]), "=f"(r[39]),
+        "=f"(r[40]), "=f"(r[41]), "=f"(r[42]), "=f"(r[43]), "=f"(r[44]), "=f"(r[45]), "=f"(r[46]), "=f"(r[47]),
+        "=f"(r[48]), "=f"(r[49]), "=f"(r[50]), "=f"(r[51]), "=f"(r[52]), "=f"(r[53]), "=f"(r[54]), "=f"(r[55]),
+        "=f"(r[56]), "=f"(r[57]), "=f"(r[58]), "=f"(r[59]), "=f"(r[60]), "=f"(r[61]), "=f"(r[62]), "=f"(r[63])
+      : "r"(addr)
+      : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
@@ -133,13 +152,17 @@ struct Waiter {
   }
 };
 
-// 8 codes as 4 words of two numbers code - zero, in the order 0 4, 1 5, 2 6, 3 7.
+// 8 codes as 4 words of two numbers code - zero, in the order 0 4, 1 5, 2 6, 3 7:
+// set into the mantissa of `magic`, 128 (bf16) or 1024 (fp16), which is a kernel
+// argument because lop3 takes one immediate and the mask is it.
+constexpr uint32_t kMagicBf16 = 0x43004300u, kMagicFp16 = 0x64006400u;
 template <bool FP16>
-__device__ __forceinline__ uint4 decode8(uint32_t w, uint32_t zero) {
+__device__ __forceinline__ uint4 decode8(uint32_t w, uint32_t magic, uint32_t zero) {
   uint32_t y[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t m = (w >> (4 * i) & 0x000f000fu) | (FP16 ? 0x64006400u : 0x43004300u);
+    uint32_t m;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(m) : "r"(w >> (4 * i)), "r"(0x000f000fu), "r"(magic));  // (w & mask) | magic
     if (FP16)
       asm("sub.f16x2 %0, %1, %2;" : "=r"(y[i]) : "r"(m), "r"(zero));
     else
@@ -159,14 +182,14 @@ __device__ __forceinline__ uint32_t zero_pair(uint32_t param) {
 // One vector's codes, decoded, as row `row` of a 128-row tile in shared memory:
 // blocks of 64 elements (128 bytes, swizzled by 16-byte chunks over 8 rows).
 template <int D, bool FP16>
-__device__ __forceinline__ void put_codes(uint32_t base, int row, const uint4 (&codes)[D / 32], uint32_t zero) {
+__device__ __forceinline__ void put_codes(uint32_t base, int row, const uint4 (&codes)[D / 32], uint32_t magic, uint32_t zero) {
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) {
     const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int chunk = 4 * i + j;
-      sts128(base + (chunk / 8) * (128 * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), decode8<FP16>(w[j], zero));
+      sts128(base + (chunk / 8) * (128 * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), decode8<FP16>(w[j], magic, zero));
     }
   }
 }
@@ -343,7 +366,7 @@ __global__ void __launch_bounds__(512, 1) prompt_kernel(PromptArgs p) {
 
   if (warp < 8) {
     // ---------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     const int t = warp >> 2, lrow = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
@@ -364,11 +387,12 @@ __global__ void __launch_bounds__(512, 1) prompt_kernel(PromptArgs p) {
         const float4* ks = reinterpret_cast<const float4*>(ks_ring + (n & (kRing - 1)) * kKeys);
         const float4* vs = reinterpret_cast<const float4*>(vs_ring + (n & (kRing - 1)) * kKeys);
         const int lim = limit - j * kKeys;
+        // Every step below is written over many independent elements: a warp's own latencies, not its
+        // instructions, are what this loop waits for.
         float s[128];
-        float mx = -INFINITY;
         const bool full = __all_sync(~0u, lim >= kKeys);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) tmem_ld32f(s_at + 32 * q, s + 32 * q);
+        tmem_ld64f(s_at, s);
+        tmem_ld64f(s_at + 64, s + 64);
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           const float4 f = ks[i];
@@ -380,12 +404,14 @@ __global__ void __launch_bounds__(512, 1) prompt_kernel(PromptArgs p) {
           for (int i = 0; i < 128; ++i)
             if (i >= lim) s[i] = -INFINITY;
         }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 128; i += 2) mx = max3(mx, s[i], s[i + 1]);
-        const bool up = mx > m + 8.f;
+        for (int i = 0; i < 128; i += 2) mx[i / 2 & 3] = max3(mx[i / 2 & 3], s[i], s[i + 1]);
+        mx[0] = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
+        const bool up = mx[0] > m + 8.f;
         if (__any_sync(~0u, up)) {
-          const float f = up ? ex2(m - mx) : 1.f;
-          if (up) m = mx;
+          const float f = up ? ex2(m - mx[0]) : 1.f;
+          if (up) m = mx[0];
           l *= f;
           if (j > w.t0) {  // the last product into O is done: s_full was committed after it
 #pragma unroll 1
@@ -399,41 +425,41 @@ __global__ void __launch_bounds__(512, 1) prompt_kernel(PromptArgs p) {
           }
         }
         const float neg = m == -INFINITY ? 0.f : -m;
-        float l0 = 0.f, l1 = 0.f;
+        float ls[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          uint32_t hi[16], lo[16];
+          float* x = s + 32 * q;
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) add2(x[i], x[i + 1], neg, neg);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = ex2(x[i]);
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) add2(ls[i & 6], ls[(i & 6) + 1], x[i], x[i + 1]);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float4 f = vs[8 * q + i];
-            float* x = s + 32 * q + 4 * i;
-            add2(x[0], x[1], neg, neg);
-            add2(x[2], x[3], neg, neg);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = ex2(x[e]);
-            add2(l0, l1, x[0], x[1]);
-            add2(l0, l1, x[2], x[3]);
-            mul2(x[0], x[1], f.x, f.y);
-            mul2(x[2], x[3], f.z, f.w);
-            if (!full) {  // a masked position's scale may be anything
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (32 * q + 4 * i + e >= lim) x[e] = 0.f;
-            }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t y = pack_bf16(x[2 * e], x[2 * e + 1]);
-              hi[2 * i + e] = y;
-              if (FP16) {
-                add2(x[2 * e], x[2 * e + 1], -__uint_as_float(y << 16), -__uint_as_float(y & 0xffff0000u));
-                lo[2 * i + e] = pack_bf16(x[2 * e], x[2 * e + 1]);
-              }
-            }
+            mul2(x[4 * i], x[4 * i + 1], f.x, f.y);
+            mul2(x[4 * i + 2], x[4 * i + 3], f.z, f.w);
           }
-          tmem_st16(s_at + 16 * q, hi);
-          if (FP16) tmem_st16(s_at + 64 + 16 * q, lo);
+          if (!full) {  // a masked position's scale may be anything
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (32 * q + i >= lim) x[i] = 0.f;
+          }
+          uint32_t y[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) y[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+          tmem_st16(s_at + 16 * q, y);
+          if (FP16) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              add2(x[2 * i], x[2 * i + 1], -__uint_as_float(y[i] << 16), -__uint_as_float(y[i] & 0xffff0000u));
+              y[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+            }
+            tmem_st16(s_at + 64 + 16 * q, y);
+          }
         }
-        l += l0 + l1;
+        l += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(p_full(t));
@@ -479,7 +505,7 @@ __global__ void __launch_bounds__(512, 1) prompt_kernel(PromptArgs p) {
     }
   } else if (warp < 12) {
     // ---------------------------------------------------------------- decoding
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     const int key = tid - 256;
     uint32_t n = 0;
     while (any) {
@@ -500,11 +526,11 @@ __global__ void __launch_bounds__(512, 1) prompt_kernel(PromptArgs p) {
         // this slot's last tile is 4 back: the products of the tile 2 back, which k_empty waited for, came after its softmax
         ks_ring[ring + key] = param_scale(kp) * a.scale_log2e;
         vs_ring[ring + key] = param_scale(vp);
-        put_codes<D, FP16>(base + L::K + st * L::TILE, key, kc, zero_pair<FP16>(kp));
+        put_codes<D, FP16>(base + L::K + st * L::TILE, key, kc, p.magic_k, zero_pair<FP16>(kp));
         fence_proxy_async_smem();
         mbar_arrive(k_full(st));
         if (!wait(v_empty(st), (n >> 1 & 1) ^ 1)) goto out;
-        put_codes<D, false>(base + L::V + st * L::TILE, key, vc, zero_pair<false>(vp));
+        put_codes<D, false>(base + L::V + st * L::TILE, key, vc, p.magic_v, zero_pair<false>(vp));
         fence_proxy_async_smem();
         mbar_arrive(v_full(st));
       }
@@ -512,7 +538,7 @@ __global__ void __launch_bounds__(512, 1) prompt_kernel(PromptArgs p) {
     }
   } else {
     // ---------------------------------------------------------------- products
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp == 12) {
       constexpr uint32_t IS = idesc_f16(kKeys, !FP16, false), IO = idesc_f16(D, true, true);
       uint32_t n = 0, pieces = 0;
@@ -711,7 +737,7 @@ __global__ void __launch_bounds__(288, 2) prompt_weights_kernel(PromptArgs p) {
     const uint4* src = reinterpret_cast<const uint4*>(c.codes[0] + (head + at) * (D / 2));
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) kc[i] = __ldg(src + i);
-    put_codes<D, FP16>(base + L::K, tid, kc, zero_pair<FP16>(kp));
+    put_codes<D, FP16>(base + L::K, tid, kc, p.magic_k, zero_pair<FP16>(kp));
     fence_proxy_async_smem();
     mbar_arrive(k_full);
     const uint32_t s_at = tmem + ((uint32_t)(warp * 32) << 16);
@@ -852,6 +878,7 @@ int attend_prompt(const AttendArgs& a, bool fp16, void* ws, int dev, cudaStream_
   size_t n;
   PromptArgs p = plan_prompt(a, a.weights_in != nullptr, std::min(kSms, sm_count(dev)), &n);
   p.parts = (float*)ws;
+  p.magic_k = fp16 ? kMagicFp16 : kMagicBf16, p.magic_v = kMagicBf16;
   p.stats = a.weights_in ? (float2*)((uint8_t*)ws + (size_t)p.stats) : nullptr;
   auto aligned = [](const void* q, const int64_t* st) { return (((uintptr_t)q | (st[0] * 2) | (st[1] * 2) | (st[2] * 2)) & 15) == 0; };
   p.vec_q = aligned(a.q, a.qs), p.vec_o = aligned(a.out, a.os);
