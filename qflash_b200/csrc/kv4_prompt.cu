@@ -8,14 +8,16 @@
 //   4 warps decode: a thread owns a key, turns its codes into bf16 (or fp16)
 //     numbers code - zero, exact, and writes them swizzled into shared memory;
 //     scales go to a ring of their own, and stay outside of the products
-//   1 thread issues tcgen05.mma: S = Q K^T into TMEM, O += P V with P from TMEM
 //   2 x 4 warps do the softmax of a row tile each, a thread a row, and write P
-//     over S.  The two tiles alternate: one's products run under the other's
-//     softmax.
+//     over S; a thread of each issues its tile's tcgen05.mma: S = Q K^T into TMEM,
+//     O += P V with P from TMEM.  The two tiles alternate: one's products run
+//     under the other's softmax.
 // P vs goes to the tensor cores as bf16 for bf16 queries, as the sum of two bf16
-// terms for fp16 queries (half steps 2^-8 and 2^-16).  O is rescaled only when a
-// row's maximum grew by more than 2^8: P is then at most 256, which costs no
-// bits in floating point.
+// terms for fp16 queries (half steps 2^-8 and 2^-16).  A tile's P is formed against
+// the maximum of the tiles before it, in one pass that takes 32 columns at a time
+// and overwrites them: P of any size costs no bits in floating point.  The new
+// maximum counts from the next tile on, if it is larger by 8 (in log2) or more; only a
+// score that is larger by 64 stops the pass, and what the tile has so far is scaled.
 // The order of d within each 8 is 0 4 1 5 2 6 3 7 everywhere (codes d and d + 4
 // of a word come out of one mask): Q is stored so, and the epilogue undoes it.
 //
@@ -38,6 +40,7 @@ constexpr int kM = 128;           // rows of a tile, TMEM lanes
 constexpr int kKeys = 128;        // keys of a tile
 constexpr int kRows = 2 * kM;     // rows of a CTA
 constexpr int kRing = 4;          // tiles of scales
+constexpr int kPrompt = 384;      // threads: 8 warps of softmax, which issue the products, and 4 that decode
 
 struct PromptArgs {
   AttendArgs a;
@@ -72,29 +75,37 @@ __device__ __forceinline__ void tmem_ld32f(uint32_t addr, float* r) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) r[i] = __int_as_float(v[i]);
 }
-// 32 lanes x 64 columns of 32 bits, complete when this returns.
-__device__ __forceinline__ void tmem_ld64f(uint32_t addr, float* r) {
+// 32 lanes x 32 columns of 32 bits, begun; the registers hold them after tmem_arrived.
+__device__ __forceinline__ void tmem_begin32(uint32_t addr, float (&r)[32]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
-      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
       : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
         "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
         "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
-        "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31]),
-        "=f"(r[32]), "=f"(r[33]), "=f"(r[34]), "=f"(r[35]), "=f"(r[36]), "=f"(r[37]), "=f"(r[38]), "=f"(r[39]),
-        "=f"(r[40]), "=f"(r[41]), "=f"(r[42]), "=f"(r[43]), "=f"(r[44]), "=f"(r[45]), "=f"(r[46]), "=f"(r[47]),
-        "=f"(r[48]), "=f"(r[49]), "=f"(r[50]), "=f"(r[51]), "=f"(r[52]), "=f"(r[53]), "=f"(r[54]), "=f"(r[55]),
-        "=f"(r[56]), "=f"(r[57]), "=f"(r[58]), "=f"(r[59]), "=f"(r[60]), "=f"(r[61]), "=f"(r[62]), "=f"(r[63])
-      : "r"(addr)
-      : "memory");
+        "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_arrived(float (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
+                 "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]),
+                 "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]),
+                 "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31])
+               :);
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+               "tcgen05.wait::ld.sync.aligned;"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                 "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+               : "r"(addr));
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
                "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-               "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-               : "memory");
+               "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]));
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -212,13 +223,22 @@ __device__ __forceinline__ void put_query(uint32_t base, int row, const uint16_t
                       __byte_perm(x.y, x.w, 0x7632)));
   }
 }
-// K-major operand [128 rows][D]: step of 16 elements; MN-major operand (V): step of 16 keys.
-__device__ __forceinline__ uint64_t k_desc(uint32_t base, int step) {
-  return smem_desc(base + (step >> 2) * (128 * 128) + (step & 3) * 32, 16, 1024, kSw128);
+// Shared-memory descriptors, from the low word of the tile's: one thread issues all
+// products, and forming 64-bit descriptors step by step cost it more time than
+// the products take.  K-major operand (Q, K): a step of 16 elements is 32 bytes in a
+// block of 64 elements; MN-major operand (V): a step of 16 keys is 16 rows of 128 bytes.
+__device__ __forceinline__ uint32_t k_word(uint32_t base) { return (uint32_t)smem_desc(base, 16, 1024, kSw128); }
+__device__ __forceinline__ uint32_t mn_word(uint32_t base) { return (uint32_t)smem_desc(base, 128 * 128, 1024, kSw128); }
+__device__ __forceinline__ uint64_t desc_of(uint32_t word) {
+  constexpr uint32_t kHigh = (uint32_t)(smem_desc(0, 0, 1024, kSw128) >> 32);
+  return (uint64_t)kHigh << 32 | word;
 }
-__device__ __forceinline__ uint64_t mn_desc(uint32_t base, int step) {
-  return smem_desc(base + step * 16 * 128, 128 * 128, 1024, kSw128);
-}
+__device__ __forceinline__ uint64_t k_desc(uint32_t word, int step) { return desc_of(word + (step >> 2) * (128 * 128 / 16) + (step & 3) * 2); }
+__device__ __forceinline__ uint64_t mn_desc(uint32_t word, int step) { return desc_of(word + step * (16 * 128 / 16)); }
+
+// P's column for a step of 16 keys: 32 keys' first terms lie in the first 16 of their scores' 32 columns, the
+// second terms (fp16) behind them.
+__device__ __forceinline__ constexpr uint32_t p_col(int step) { return 32 * (step >> 1) + 8 * (step & 1); }
 
 // ------------------------------------------------------------------ work split
 // Key tiles of row tile rt of sequence z.
@@ -307,8 +327,140 @@ struct Layout {
   static constexpr uint32_t BYTES = BARS + 256 + 1024;  // with room to align the base
 };
 
+// A row of the softmax, held by one thread: maximum (log2), sum, and what O has
+// yet to be multiplied by.
+struct RowState {
+  float m, l, late;
+};
+
+// O times f.  The last product into it is done: this tile's scores were committed after that.
+template <int D>
+__device__ __forceinline__ void scale_out(uint32_t o_at, float f) {
+#pragma unroll 1
+  for (int q = 0; q < D / 32; ++q) {
+    int o[32];
+    tmem_ld32(o_at + 32 * q, o);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) o[i] = __float_as_int(__int_as_float(o[i]) * f);
+    tmem_st32(o_at + 32 * q, o);
+  }
+}
+
+// One tile of 128 scores of a row: P over the scores.  FULL: the row sees all of
+// them, else the first `lim`.  All steps are written over many independent
+// elements: a warp's latencies, not its instructions, are what it waits for.
+template <int D, bool FP16, bool FULL>
+__device__ __forceinline__ void softmax_tile(RowState& r, uint32_t s_at, uint32_t o_at, const float4* ks, const float4* vs,
+                                             int lim, bool first) {
+  // 32 scores against the row's maximum, and the largest difference
+  auto differences = [&](int q, float (&x)[32], float neg) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 f = ks[8 * q + i];
+      fma2(x[4 * i], x[4 * i + 1], f.x, f.y, neg, neg);
+      fma2(x[4 * i + 2], x[4 * i + 3], f.z, f.w, neg, neg);
+    }
+    if (!FULL) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (32 * q + i >= lim) x[i] = -INFINITY;
+    }
+    float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) a[i / 2 & 3] = max3(a[i / 2 & 3], x[i], x[i + 1]);
+    return fmaxf(max3(a[0], a[1], a[2]), a[3]);
+  };
+  if (first) {  // nothing before it: its own maximum
+#pragma unroll 1
+    for (int q = 0; q < 4; ++q) {
+      float x[32];
+      tmem_begin32(s_at + 32 * q, x);
+      tmem_arrived(x);
+      r.m = fmaxf(r.m, differences(q, x, 0.f));
+    }
+  } else if (__any_sync(~0u, r.late != 1.f)) {
+    scale_out<D>(o_at, r.late);
+    r.late = 1.f;
+  }
+  float mx = -INFINITY, ls[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  float neg = r.m == -INFINITY ? 0.f : -r.m, top;
+  float buf[3][32];
+  tmem_begin32(s_at, buf[0]);
+  tmem_arrived(buf[0]);
+  tmem_begin32(s_at + 32, buf[1]);
+  top = differences(0, buf[0], neg);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    float(&x)[32] = buf[q % 3];
+    if (q < 3) tmem_arrived(buf[(q + 1) % 3]);
+    if (q < 2) tmem_begin32(s_at + 32 * (q + 2), buf[(q + 2) % 3]);
+    mx = fmaxf(mx, top);
+    const bool high = top > (r.m == -INFINITY ? -INFINITY : 64.f);
+    if (__any_sync(~0u, high)) {
+      // up by a whole number, or from nothing to the first score
+      const float by = !high ? 0.f : r.m == -INFINITY ? top : ceilf(top);
+      const float f = !high ? 1.f : r.m == -INFINITY ? 0.f : ex2(-by);
+      r.m = !high ? r.m : r.m == -INFINITY ? top : r.m + by;
+      neg = r.m == -INFINITY ? 0.f : -r.m;
+      mx -= by;
+      r.l *= f;
+      if (!first) scale_out<D>(o_at, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ls[i] *= f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) x[i] -= by;
+      tmem_wait_st();
+      const uint32_t ff = pack_bf16(f, f);
+#pragma unroll 1
+      for (int e = 0; e < (FP16 ? 2 : 1) * q; ++e) {
+        uint32_t y[16];
+        const uint32_t at = FP16 ? s_at + 16 * e : s_at + 32 * e;
+        tmem_ld16(at, y);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) asm("mul.bf16x2 %0, %0, %1;" : "+r"(y[i]) : "r"(ff));
+        tmem_st16(at, y);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] = ex2(x[i]);
+    if (q < 3) top = differences(q + 1, buf[(q + 1) % 3], neg);  // under the exponentials
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) add2(ls[i & 6], ls[(i & 6) + 1], x[i], x[i + 1]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 f = vs[8 * q + i];
+      mul2(x[4 * i], x[4 * i + 1], f.x, f.y);
+      mul2(x[4 * i + 2], x[4 * i + 3], f.z, f.w);
+    }
+    if (!FULL) {  // a masked position's scale may be anything
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (32 * q + i >= lim) x[i] = 0.f;
+    }
+    uint32_t y[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) y[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+    tmem_st16(s_at + 32 * q, y);
+    if (FP16) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        add2(x[2 * i], x[2 * i + 1], -__uint_as_float(y[i] << 16), -__uint_as_float(y[i] & 0xffff0000u));
+        y[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+      }
+      tmem_st16(s_at + 32 * q + 16, y);
+    }
+  }
+  r.l += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
+  tmem_wait_st();
+  if (mx > 8.f) {
+    const float by = ceilf(mx), f = ex2(-by);
+    r.m += by;
+    r.l *= f, r.late *= f;
+  }
+}
+
 template <int D, bool FP16>
-__global__ void __launch_bounds__(512, 1) prompt_kernel(PromptArgs p) {
+__global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
   using L = Layout<D>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u;
@@ -325,20 +477,22 @@ __global__ void __launch_bounds__(512, 1) prompt_kernel(PromptArgs p) {
   auto s_full = [&](int t) { return bars + 80 + 8 * t; };
   auto p_full = [&](int t) { return bars + 96 + 8 * t; };
   auto o_full = [&](int t) { return bars + 112 + 8 * t; };
+  auto turn = [&](int t) { return bars + 144 + 8 * t; };
   const uint32_t done = bars + 128, slot = bars + 136;
   volatile uint32_t* abort = reinterpret_cast<volatile uint32_t*>(smem + L::BARS + 140);
   float* const ks_ring = reinterpret_cast<float*>(smem + L::KS);
   float* const vs_ring = reinterpret_cast<float*>(smem + L::VS);
 
-  if (warp == 12) {
+  if (warp == 8) {
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(k_full(i), 128), mbar_init(v_full(i), 128);
-        mbar_init(k_empty(i), 1), mbar_init(v_empty(i), 1);
+        mbar_init(k_empty(i), 2), mbar_init(v_empty(i), 2);
         mbar_init(q_full(i), 128), mbar_init(p_full(i), 128);
         mbar_init(s_full(i), 2), mbar_init(o_full(i), 1);
+        mbar_init(turn(i), 1);
       }
-      mbar_init(done, 1);
+      mbar_init(done, 2);
       *abort = 0;
       fence_mbar_init();
     }
@@ -366,11 +520,28 @@ __global__ void __launch_bounds__(512, 1) prompt_kernel(PromptArgs p) {
 
   if (warp < 8) {
     // ---------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     const int t = warp >> 2, lrow = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
     uint32_t n = 0, pieces = 0;  // key tiles and pieces so far
+    const bool issuer = (warp & 3) == 0;  // its first lane issues the row tile's products
+    constexpr uint32_t IS = idesc_f16(kKeys, !FP16, false), IO = idesc_f16(D, true, true);
+    const uint32_t q_word = k_word(base + L::Q + t * L::TILE), kk_word = k_word(base + L::K), v_word = mn_word(base + L::V);
+    auto scores = [&](uint32_t g) {  // S = Q K^T of key tile g
+      if (!wait(k_full(g & 1), g >> 1 & 1)) return false;
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t kw = kk_word + (g & 1) * (L::TILE / 16);
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) mma_ss(tmem + t * 128, k_desc(q_word, s), k_desc(kw, s), IS, s > 0);
+        tc_commit(s_full(t));
+        tc_commit(k_empty(g & 1));
+        mbar_arrive(s_full(t));  // passes on the scales that k_full's wait made visible here
+      }
+      __syncwarp();
+      return true;
+    };
     while (any) {
       const Span sp = span_of(a, w.z);
       const int row = w.rt * kRows + t * kM + lrow, tok = row / a.rep, head = w.h * a.rep + row % a.rep;
@@ -380,108 +551,63 @@ __global__ void __launch_bounds__(512, 1) prompt_kernel(PromptArgs p) {
                    live ? (const uint16_t*)a.q + (w.z * a.qs[0] + head * a.qs[1] + tok * a.qs[2]) : nullptr, p.vec_q);
       fence_proxy_async_smem();
       mbar_arrive(q_full(t));
-      float m = -INFINITY, l = 0.f;
+      if (issuer && (!wait(q_full(t), pieces & 1) || !scores(n))) goto out;
+      RowState r = {-INFINITY, 0.f, 1.f};
       for (int j = w.t0; j < w.t1; ++j, ++n) {
         if (!wait(s_full(t), n & 1)) goto out;
         tc_fence_after();
         const float4* ks = reinterpret_cast<const float4*>(ks_ring + (n & (kRing - 1)) * kKeys);
         const float4* vs = reinterpret_cast<const float4*>(vs_ring + (n & (kRing - 1)) * kKeys);
         const int lim = limit - j * kKeys;
-        // Every step below is written over many independent elements: a warp's own latencies, not its
-        // instructions, are what this loop waits for.
-        float s[128];
-        const bool full = __all_sync(~0u, lim >= kKeys);
-        tmem_ld64f(s_at, s);
-        tmem_ld64f(s_at + 64, s + 64);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float4 f = ks[i];
-          mul2(s[4 * i], s[4 * i + 1], f.x, f.y);
-          mul2(s[4 * i + 2], s[4 * i + 3], f.z, f.w);
-        }
-        if (!full) {
-#pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (i >= lim) s[i] = -INFINITY;
-        }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int i = 0; i < 128; i += 2) mx[i / 2 & 3] = max3(mx[i / 2 & 3], s[i], s[i + 1]);
-        mx[0] = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
-        const bool up = mx[0] > m + 8.f;
-        if (__any_sync(~0u, up)) {
-          const float f = up ? ex2(m - mx[0]) : 1.f;
-          if (up) m = mx[0];
-          l *= f;
-          if (j > w.t0) {  // the last product into O is done: s_full was committed after it
-#pragma unroll 1
-            for (int q = 0; q < D / 32; ++q) {
-              int o[32];
-              tmem_ld32(o_at + 32 * q, o);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_int(__int_as_float(o[i]) * f);
-              tmem_st32(o_at + 32 * q, o);
-            }
-          }
-        }
-        const float neg = m == -INFINITY ? 0.f : -m;
-        float ls[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float* x = s + 32 * q;
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) add2(x[i], x[i + 1], neg, neg);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] = ex2(x[i]);
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) add2(ls[i & 6], ls[(i & 6) + 1], x[i], x[i + 1]);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 f = vs[8 * q + i];
-            mul2(x[4 * i], x[4 * i + 1], f.x, f.y);
-            mul2(x[4 * i + 2], x[4 * i + 3], f.z, f.w);
-          }
-          if (!full) {  // a masked position's scale may be anything
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (32 * q + i >= lim) x[i] = 0.f;
-          }
-          uint32_t y[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) y[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
-          tmem_st16(s_at + 16 * q, y);
-          if (FP16) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              add2(x[2 * i], x[2 * i + 1], -__uint_as_float(y[i] << 16), -__uint_as_float(y[i] & 0xffff0000u));
-              y[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
-            }
-            tmem_st16(s_at + 64 + 16 * q, y);
-          }
-        }
-        l += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
-        tmem_wait_st();
+        if (__all_sync(~0u, lim >= kKeys))
+          softmax_tile<D, FP16, true>(r, s_at, o_at, ks, vs, lim, j == w.t0);
+        else
+          softmax_tile<D, FP16, false>(r, s_at, o_at, ks, vs, lim, j == w.t0);
         tc_fence_before();
         mbar_arrive(p_full(t));
+        if (issuer) {
+          if (!wait(p_full(t), n & 1) || !wait(v_full(n & 1), n >> 1 & 1)) goto out;
+          // the two row tiles' products take turns: issued side by side they would all end together, and then
+          // both softmaxes would run together and the tensor cores wait for them
+          if ((t || n) && !wait(turn(t), (t ? n : n - 1) & 1)) goto out;
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t vw = v_word + (n & 1) * (L::TILE / 16);
+#pragma unroll
+            for (int s = 0; s < kKeys / 16; ++s)
+              mma_ts(tmem + 256 + t * 128, tmem + t * 128 + p_col(s), mn_desc(vw, s), IO, j > w.t0 || s > 0);
+            if (FP16) {
+#pragma unroll
+              for (int s = 0; s < kKeys / 16; ++s) mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 16 + p_col(s), mn_desc(vw, s), IO, 1);
+            }
+            tc_commit(v_empty(n & 1));
+            if (j + 1 == w.t1) tc_commit(o_full(t));
+          }
+          __syncwarp();
+          if (j + 1 < w.t1 && !scores(n + 1)) goto out;
+          if (lane == 0) mbar_arrive(turn(t ^ 1));
+        }
       }
       if (!wait(o_full(t), pieces & 1)) goto out;
       tc_fence_after();
       {
-        const float inv = 1.f / l;
+        const float inv = 1.f / r.l;
         const bool write = row < p.rows;
         float* part = p.parts + ((size_t)blockIdx.x * 2 + (pieces ? 1 : 0)) * (kRows * (D + 2));
         const size_t to = w.z * a.os[0] + head * a.os[1] + (size_t)tok * a.os[2];
         if (write) {
           if (!w.whole)
-            part[t * kM + lrow] = m, part[kRows + t * kM + lrow] = l;
+            part[t * kM + lrow] = r.m, part[kRows + t * kM + lrow] = r.l;
           else if (p.stats)
-            p.stats[((size_t)w.z * c.H + w.h) * p.rows + row] = make_float2(m, inv);
+            p.stats[((size_t)w.z * c.H + w.h) * p.rows + row] = make_float2(r.m, inv);
         }
 #pragma unroll 1
         for (int q = 0; q < D / 32; ++q) {
           float o[32];
           tmem_ld32f(o_at + 32 * q, o);
           if (!write) continue;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] *= r.late;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const float y[8] = {o[8 * g], o[8 * g + 2], o[8 * g + 4], o[8 * g + 6], o[8 * g + 1], o[8 * g + 3], o[8 * g + 5], o[8 * g + 7]};
@@ -503,9 +629,9 @@ __global__ void __launch_bounds__(512, 1) prompt_kernel(PromptArgs p) {
       ++pieces;
       any = w.next(p);
     }
-  } else if (warp < 12) {
+  } else {
     // ---------------------------------------------------------------- decoding
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     const int key = tid - 256;
     uint32_t n = 0;
     while (any) {
@@ -536,64 +662,10 @@ __global__ void __launch_bounds__(512, 1) prompt_kernel(PromptArgs p) {
       }
       any = w.next(p);
     }
-  } else {
-    // ---------------------------------------------------------------- products
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-    if (warp == 12) {
-      constexpr uint32_t IS = idesc_f16(kKeys, !FP16, false), IO = idesc_f16(D, true, true);
-      uint32_t n = 0, pieces = 0;
-      auto scores = [&](int t, uint32_t g) {
-        if (lane == 0) {
-#pragma unroll
-          for (int s = 0; s < D / 16; ++s)
-            mma_ss(tmem + t * 128, k_desc(base + L::Q + t * L::TILE, s), k_desc(base + L::K + (g & 1) * L::TILE, s), IS, s > 0);
-          tc_commit(s_full(t));
-          mbar_arrive(s_full(t));  // passes on the scales that k_full's wait made visible here
-        }
-        __syncwarp();
-      };
-      while (any) {
-        const int tiles = w.t1 - w.t0;
-        if (!wait(k_full(n & 1), n >> 1 & 1)) goto out;
-        for (int t = 0; t < 2; ++t) {
-          if (!wait(q_full(t), pieces & 1)) goto out;
-          tc_fence_after();
-          scores(t, n);
-        }
-        if (lane == 0) tc_commit(k_empty(n & 1));
-        for (int j = 0; j < tiles; ++j, ++n) {
-          for (int t = 0; t < 2; ++t) {
-            if (!wait(v_full(n & 1), n >> 1 & 1) || !wait(p_full(t), n & 1)) goto out;
-            tc_fence_after();
-            if (lane == 0) {
-#pragma unroll
-              for (int s = 0; s < kKeys / 16; ++s)
-                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * s, mn_desc(base + L::V + (n & 1) * L::TILE, s), IO, j > 0 || s > 0);
-              if (FP16) {
-#pragma unroll
-                for (int s = 0; s < kKeys / 16; ++s)
-                  mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 64 + 8 * s, mn_desc(base + L::V + (n & 1) * L::TILE, s), IO, 1);
-              }
-              if (t == 1) tc_commit(v_empty(n & 1));
-              if (j + 1 == tiles) tc_commit(o_full(t));
-            }
-            __syncwarp();
-            if (j + 1 < tiles) {
-              if (!wait(k_full((n + 1) & 1), (n + 1) >> 1 & 1)) goto out;
-              tc_fence_after();
-              scores(t, n + 1);
-              if (t == 1 && lane == 0) tc_commit(k_empty((n + 1) & 1));
-            }
-          }
-        }
-        ++pieces;
-        any = w.next(p);
-      }
-    }
   }
 out:
   __syncwarp();
-  if (warp == 12) {  // nothing of this CTA's may be under way when its TMEM goes
+  if (warp == 0 || warp == 4) {  // nothing of this CTA's may be under way when its TMEM goes
     if (lane == 0) tc_commit(done);
     __syncwarp();
     mbar_wait(done, 0);
@@ -601,7 +673,7 @@ out:
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(tmem, 512);
+  if (warp == 8) tmem_dealloc(tmem, 512);
 }
 
 // Joins units that several CTAs held: blockIdx.x < 8 grid: 32 rows of the unit that
@@ -799,6 +871,7 @@ __global__ void __launch_bounds__(288, 2) prompt_weights_kernel(PromptArgs p) {
     }
   } else {
     constexpr uint32_t IS = idesc_f16(kM, !FP16, false);
+    const uint32_t kw = k_word(base + L::K), qw = k_word(base + L::Q);
     if (!wait(k_full, 0)) goto out;
     for (int rt = rt0; rt < rt1; ++rt) {
       const int g = rt - rt0, b = g & 1;
@@ -807,7 +880,7 @@ __global__ void __launch_bounds__(288, 2) prompt_weights_kernel(PromptArgs p) {
       if (lane == 0) {
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
-          mma_ss(tmem + b * 128, k_desc(base + L::K, s), k_desc(base + L::Q + b * L::TILE, s), IS, s > 0);
+          mma_ss(tmem + b * 128, k_desc(kw, s), k_desc(qw + b * (L::TILE / 16), s), IS, s > 0);
         tc_commit(s_full(b));
         tc_commit(q_empty(b));
       }
@@ -862,7 +935,7 @@ static int allow_smem(K* kernel, uint32_t bytes) {
 template <int D, bool FP16>
 static int launch_prompt(const PromptArgs& p, cudaStream_t s) {
   if (int rc = allow_smem(prompt_kernel<D, FP16>, Layout<D>::BYTES)) return rc;
-  prompt_kernel<D, FP16><<<p.grid, 512, Layout<D>::BYTES, s>>>(p);
+  prompt_kernel<D, FP16><<<p.grid, kPrompt, Layout<D>::BYTES, s>>>(p);
   if (int rc = check_launch("kv4 prompt", p.grid)) return rc;
   const unsigned n = 8 * p.grid + p.a.c.Z * p.row_tiles;
   prompt_finish_kernel<D, FP16><<<n, 256, 0, s>>>(p);
