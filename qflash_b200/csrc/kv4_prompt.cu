@@ -8,10 +8,10 @@
 //   4 warps decode: a thread owns a key, turns its codes into bf16 (or fp16)
 //     numbers code - zero, exact, and writes them swizzled into shared memory;
 //     scales go to a ring of their own, and stay outside of the products
+//   1 warp issues tcgen05.mma: S = Q K^T into TMEM, O += P V with P from TMEM
 //   2 x 4 warps do the softmax of a row tile each, a thread a row, and write P
-//     over S; a thread of each issues its tile's tcgen05.mma: S = Q K^T into TMEM,
-//     O += P V with P from TMEM.  The two tiles alternate: one's products run
-//     under the other's softmax.
+//     over S.  The two tiles take turns: one's products run under the other's
+//     softmax.
 // P vs goes to the tensor cores as bf16 for bf16 queries, as the sum of two bf16
 // terms for fp16 queries (half steps 2^-8 and 2^-16).  A tile's P is formed against
 // the maximum of the tiles before it, in one pass that takes 32 columns at a time
@@ -40,7 +40,7 @@ constexpr int kM = 128;           // rows of a tile, TMEM lanes
 constexpr int kKeys = 128;        // keys of a tile
 constexpr int kRows = 2 * kM;     // rows of a CTA
 constexpr int kRing = 4;          // tiles of scales
-constexpr int kPrompt = 384;      // threads: 8 warps of softmax, which issue the products, and 4 that decode
+constexpr int kPrompt = 512;      // threads: 8 warps of softmax, 4 that decode, 1 that issues products, 3 idle
 
 struct PromptArgs {
   AttendArgs a;
@@ -59,16 +59,20 @@ __host__ __device__ constexpr uint32_t idesc_f16(int N, bool bf16, bool b_mn_maj
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn_major ? 1u : 0u) << 16) |
          ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kM >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+// Issued by the lane with `on`, which all lanes of a warp reach together: in a branch of one
+// lane's every descriptor would be moved to the uniform registers by itself.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t on) {
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(on)
                : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t on) {
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(on)
                : "memory");
 }
+// The same value in all lanes, known to be.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(~0u, x, 0); }
 __device__ __forceinline__ void tmem_ld32f(uint32_t addr, float* r) {
   int v[32];
   tmem_ld32(addr, v);
@@ -477,22 +481,20 @@ __global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
   auto s_full = [&](int t) { return bars + 80 + 8 * t; };
   auto p_full = [&](int t) { return bars + 96 + 8 * t; };
   auto o_full = [&](int t) { return bars + 112 + 8 * t; };
-  auto turn = [&](int t) { return bars + 144 + 8 * t; };
   const uint32_t done = bars + 128, slot = bars + 136;
   volatile uint32_t* abort = reinterpret_cast<volatile uint32_t*>(smem + L::BARS + 140);
   float* const ks_ring = reinterpret_cast<float*>(smem + L::KS);
   float* const vs_ring = reinterpret_cast<float*>(smem + L::VS);
 
-  if (warp == 8) {
+  if (warp == 12) {
     if (lane == 0) {
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(k_full(i), 128), mbar_init(v_full(i), 128);
-        mbar_init(k_empty(i), 2), mbar_init(v_empty(i), 2);
-        mbar_init(q_full(i), 128), mbar_init(p_full(i), 128);
+      for (int i = 0; i < 2; ++i) {  // arrivals: one per warp that writes
+        mbar_init(k_full(i), 4), mbar_init(v_full(i), 4);
+        mbar_init(k_empty(i), 1), mbar_init(v_empty(i), 1);
+        mbar_init(q_full(i), 4), mbar_init(p_full(i), 4);
         mbar_init(s_full(i), 2), mbar_init(o_full(i), 1);
-        mbar_init(turn(i), 1);
       }
-      mbar_init(done, 2);
+      mbar_init(done, 1);
       *abort = 0;
       fence_mbar_init();
     }
@@ -506,6 +508,10 @@ __global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
   uint32_t tmem = 0;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
   const Waiter wait{abort, c.ctl};
+  auto warp_arrive = [&](uint32_t bar) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+  };
 
   Walk w;
   const long long total = Walk::total_tiles(p);
@@ -520,28 +526,11 @@ __global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
 
   if (warp < 8) {
     // ---------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     const int t = warp >> 2, lrow = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
     uint32_t n = 0, pieces = 0;  // key tiles and pieces so far
-    const bool issuer = (warp & 3) == 0;  // its first lane issues the row tile's products
-    constexpr uint32_t IS = idesc_f16(kKeys, !FP16, false), IO = idesc_f16(D, true, true);
-    const uint32_t q_word = k_word(base + L::Q + t * L::TILE), kk_word = k_word(base + L::K), v_word = mn_word(base + L::V);
-    auto scores = [&](uint32_t g) {  // S = Q K^T of key tile g
-      if (!wait(k_full(g & 1), g >> 1 & 1)) return false;
-      tc_fence_after();
-      if (lane == 0) {
-        const uint32_t kw = kk_word + (g & 1) * (L::TILE / 16);
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s) mma_ss(tmem + t * 128, k_desc(q_word, s), k_desc(kw, s), IS, s > 0);
-        tc_commit(s_full(t));
-        tc_commit(k_empty(g & 1));
-        mbar_arrive(s_full(t));  // passes on the scales that k_full's wait made visible here
-      }
-      __syncwarp();
-      return true;
-    };
     while (any) {
       const Span sp = span_of(a, w.z);
       const int row = w.rt * kRows + t * kM + lrow, tok = row / a.rep, head = w.h * a.rep + row % a.rep;
@@ -550,8 +539,7 @@ __global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
       put_query<D>(base + L::Q + t * L::TILE, lrow,
                    live ? (const uint16_t*)a.q + (w.z * a.qs[0] + head * a.qs[1] + tok * a.qs[2]) : nullptr, p.vec_q);
       fence_proxy_async_smem();
-      mbar_arrive(q_full(t));
-      if (issuer && (!wait(q_full(t), pieces & 1) || !scores(n))) goto out;
+      warp_arrive(q_full(t));
       RowState r = {-INFINITY, 0.f, 1.f};
       for (int j = w.t0; j < w.t1; ++j, ++n) {
         if (!wait(s_full(t), n & 1)) goto out;
@@ -564,29 +552,7 @@ __global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
         else
           softmax_tile<D, FP16, false>(r, s_at, o_at, ks, vs, lim, j == w.t0);
         tc_fence_before();
-        mbar_arrive(p_full(t));
-        if (issuer) {
-          if (!wait(p_full(t), n & 1) || !wait(v_full(n & 1), n >> 1 & 1)) goto out;
-          // the two row tiles' products take turns: issued side by side they would all end together, and then
-          // both softmaxes would run together and the tensor cores wait for them
-          if ((t || n) && !wait(turn(t), (t ? n : n - 1) & 1)) goto out;
-          tc_fence_after();
-          if (lane == 0) {
-            const uint32_t vw = v_word + (n & 1) * (L::TILE / 16);
-#pragma unroll
-            for (int s = 0; s < kKeys / 16; ++s)
-              mma_ts(tmem + 256 + t * 128, tmem + t * 128 + p_col(s), mn_desc(vw, s), IO, j > w.t0 || s > 0);
-            if (FP16) {
-#pragma unroll
-              for (int s = 0; s < kKeys / 16; ++s) mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 16 + p_col(s), mn_desc(vw, s), IO, 1);
-            }
-            tc_commit(v_empty(n & 1));
-            if (j + 1 == w.t1) tc_commit(o_full(t));
-          }
-          __syncwarp();
-          if (j + 1 < w.t1 && !scores(n + 1)) goto out;
-          if (lane == 0) mbar_arrive(turn(t ^ 1));
-        }
+        warp_arrive(p_full(t));
       }
       if (!wait(o_full(t), pieces & 1)) goto out;
       tc_fence_after();
@@ -629,9 +595,9 @@ __global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
       ++pieces;
       any = w.next(p);
     }
-  } else {
+  } else if (warp < 12) {
     // ---------------------------------------------------------------- decoding
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     const int key = tid - 256;
     uint32_t n = 0;
     while (any) {
@@ -654,18 +620,81 @@ __global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
         vs_ring[ring + key] = param_scale(vp);
         put_codes<D, FP16>(base + L::K + st * L::TILE, key, kc, p.magic_k, zero_pair<FP16>(kp));
         fence_proxy_async_smem();
-        mbar_arrive(k_full(st));
+        warp_arrive(k_full(st));
         if (!wait(v_empty(st), (n >> 1 & 1) ^ 1)) goto out;
         put_codes<D, false>(base + L::V + st * L::TILE, key, vc, p.magic_v, zero_pair<false>(vp));
         fence_proxy_async_smem();
-        mbar_arrive(v_full(st));
+        warp_arrive(v_full(st));
       }
       any = w.next(p);
+    }
+  } else {
+    // ---------------------------------------------------------------- products
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == 12) {
+      constexpr uint32_t IS = idesc_f16(kKeys, !FP16, false), IO = idesc_f16(D, true, true);
+      const uint32_t q_word = k_word(base + L::Q), kk_word = k_word(base + L::K), v_word = mn_word(base + L::V);
+      uint32_t n = 0, pieces = 0;
+      // S = Q K^T of row tile t and key tile g
+      auto scores = [&](int t, uint32_t g) {
+        const uint32_t kw = uniform(kk_word + (g & 1) * (L::TILE / 16)), qw = uniform(q_word + t * (L::TILE / 16)), to = uniform(tmem + t * 128);
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) mma_ss(to, k_desc(qw, s), k_desc(kw, s), IS, s > 0, lane == 0);
+        if (lane == 0) {
+          tc_commit(s_full(t));
+          mbar_arrive(s_full(t));  // passes on the scales that k_full's wait made visible here
+        }
+        __syncwarp();
+      };
+      while (any) {
+        const int tiles = w.t1 - w.t0;
+        if (!wait(k_full(n & 1), n >> 1 & 1)) goto out;
+        for (int t = 0; t < 2; ++t) {
+          if (!wait(q_full(t), pieces & 1)) goto out;
+          tc_fence_after();
+          scores(t, n);
+        }
+        if (lane == 0) tc_commit(k_empty(n & 1));
+        __syncwarp();
+        for (int j = 0; j < tiles; ++j, ++n) {
+          // first what is there long before P, so that nothing stands between P and its products
+          if (!wait(v_full(n & 1), n >> 1 & 1)) goto out;
+          if (j + 1 < tiles && !wait(k_full((n + 1) & 1), (n + 1) >> 1 & 1)) goto out;
+          for (int t = 0; t < 2; ++t) {
+            if (!wait(p_full(t), n & 1)) goto out;
+            tc_fence_after();
+            const uint32_t vw = uniform(v_word + (n & 1) * (L::TILE / 16)), to = uniform(tmem + 256 + t * 128), from = uniform(tmem + t * 128);
+            const uint32_t more = uniform(j > 0);
+#pragma unroll
+            for (int s = 0; s < kKeys / 16; ++s) mma_ts(to, from + p_col(s), mn_desc(vw, s), IO, s > 0 ? 1 : more, lane == 0);
+            if (FP16) {
+#pragma unroll
+              for (int s = 0; s < kKeys / 16; ++s) mma_ts(to, from + 16 + p_col(s), mn_desc(vw, s), IO, 1, lane == 0);
+            }
+            if (j + 1 < tiles) {
+              scores(t, n + 1);
+            } else {
+              if (lane == 0) tc_commit(o_full(t));
+              __syncwarp();
+            }
+            if (t == 1) {
+              // Both row tiles are through with this tile's values and the next one's keys when these are.
+              if (lane == 0) {
+                tc_commit(v_empty(n & 1));
+                if (j + 1 < tiles) tc_commit(k_empty((n + 1) & 1));
+              }
+              __syncwarp();
+            }
+          }
+        }
+        ++pieces;
+        any = w.next(p);
+      }
     }
   }
 out:
   __syncwarp();
-  if (warp == 0 || warp == 4) {  // nothing of this CTA's may be under way when its TMEM goes
+  if (warp == 12) {  // nothing of this CTA's may be under way when its TMEM goes
     if (lane == 0) tc_commit(done);
     __syncwarp();
     mbar_wait(done, 0);
@@ -673,7 +702,7 @@ out:
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_dealloc(tmem, 512);
+  if (warp == 12) tmem_dealloc(tmem, 512);
 }
 
 // Joins units that several CTAs held: blockIdx.x < 8 grid: 32 rows of the unit that
@@ -877,10 +906,10 @@ __global__ void __launch_bounds__(288, 2) prompt_weights_kernel(PromptArgs p) {
       const int g = rt - rt0, b = g & 1;
       if (!wait(q_full(b), g >> 1 & 1) || !wait(s_empty(b), (g >> 1 & 1) ^ 1)) goto out;
       tc_fence_after();
-      if (lane == 0) {
+      const uint32_t kb = uniform(kw), qb = uniform(qw + b * (L::TILE / 16)), to = uniform(tmem + b * 128);
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s)
-          mma_ss(tmem + b * 128, k_desc(kw, s), k_desc(qw + b * (L::TILE / 16), s), IS, s > 0);
+      for (int s = 0; s < D / 16; ++s) mma_ss(to, k_desc(kb, s), k_desc(qb, s), IS, s > 0, lane == 0);
+      if (lane == 0) {
         tc_commit(s_full(b));
         tc_commit(q_empty(b));
       }
