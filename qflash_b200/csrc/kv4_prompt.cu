@@ -196,16 +196,19 @@ __device__ __forceinline__ uint32_t zero_pair(uint32_t param) {
 
 // One vector's codes, decoded, as row `row` of a 128-row tile in shared memory:
 // blocks of 64 elements (128 bytes, swizzled by 16-byte chunks over 8 rows).
+// A compact loop that takes codes[0] and rotates them: the warps of a CTA do
+// different things, and together they must not outgrow the instruction caches.
 template <int D, bool FP16>
-__device__ __forceinline__ void put_codes(uint32_t base, int row, const uint4 (&codes)[D / 32], uint32_t magic, uint32_t zero) {
-#pragma unroll
+__device__ __forceinline__ void put_codes(uint32_t base, int row, uint4 (&codes)[D / 32], uint32_t magic, uint32_t zero) {
+  const uint32_t to = base + row * 128, turn = (uint32_t)(row & 7) << 4;
+#pragma unroll 1
   for (int i = 0; i < D / 32; ++i) {
-    const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+    const uint32_t w[4] = {codes[0].x, codes[0].y, codes[0].z, codes[0].w};
+    const uint32_t block = to + (i >> 1) * (128 * 128), chunk = (i & 1) * 64;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int chunk = 4 * i + j;
-      sts128(base + (chunk / 8) * (128 * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), decode8<FP16>(w[j], magic, zero));
-    }
+    for (int j = 0; j < 4; ++j) sts128(block + ((chunk + 16 * j) ^ turn), decode8<FP16>(w[j], magic, zero));
+#pragma unroll
+    for (int e = 0; e + 1 < D / 32; ++e) codes[e] = codes[e + 1];
   }
 }
 // One query row, likewise.
@@ -388,16 +391,12 @@ __device__ __forceinline__ void softmax_tile(RowState& r, uint32_t s_at, uint32_
   }
   float mx = -INFINITY, ls[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   float neg = r.m == -INFINITY ? 0.f : -r.m, top;
-  float buf[3][32];
-  tmem_begin32(s_at, buf[0]);
-  tmem_arrived(buf[0]);
-  tmem_begin32(s_at + 32, buf[1]);
-  top = differences(0, buf[0], neg);
-#pragma unroll
+#pragma unroll 1
   for (int q = 0; q < 4; ++q) {
-    float(&x)[32] = buf[q % 3];
-    if (q < 3) tmem_arrived(buf[(q + 1) % 3]);
-    if (q < 2) tmem_begin32(s_at + 32 * (q + 2), buf[(q + 2) % 3]);
+    float x[32];
+    tmem_begin32(s_at + 32 * q, x);
+    tmem_arrived(x);
+    top = differences(q, x, neg);
     mx = fmaxf(mx, top);
     const bool high = top > (r.m == -INFINITY ? -INFINITY : 64.f);
     if (__any_sync(~0u, high)) {
@@ -427,7 +426,6 @@ __device__ __forceinline__ void softmax_tile(RowState& r, uint32_t s_at, uint32_
     }
 #pragma unroll
     for (int i = 0; i < 32; ++i) x[i] = ex2(x[i]);
-    if (q < 3) top = differences(q + 1, buf[(q + 1) % 3], neg);  // under the exponentials
 #pragma unroll
     for (int i = 0; i < 32; i += 2) add2(ls[i & 6], ls[(i & 6) + 1], x[i], x[i + 1]);
 #pragma unroll
@@ -638,8 +636,11 @@ __global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
       // S = Q K^T of row tile t and key tile g
       auto scores = [&](int t, uint32_t g) {
         const uint32_t kw = uniform(kk_word + (g & 1) * (L::TILE / 16)), qw = uniform(q_word + t * (L::TILE / 16)), to = uniform(tmem + t * 128);
+#pragma unroll 1
+        for (int b = 0; b < D / 64; ++b)
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) mma_ss(to, k_desc(qw, s), k_desc(kw, s), IS, s > 0, lane == 0);
+          for (int s = 0; s < 4; ++s)
+            mma_ss(to, k_desc(qw + b * 1024, s), k_desc(kw + b * 1024, s), IS, s > 0 ? 1 : b, lane == 0);
         if (lane == 0) {
           tc_commit(s_full(t));
           mbar_arrive(s_full(t));  // passes on the scales that k_full's wait made visible here
@@ -665,12 +666,13 @@ __global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
             tc_fence_after();
             const uint32_t vw = uniform(v_word + (n & 1) * (L::TILE / 16)), to = uniform(tmem + 256 + t * 128), from = uniform(tmem + t * 128);
             const uint32_t more = uniform(j > 0);
+#pragma unroll 1
+            for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int s = 0; s < kKeys / 16; ++s) mma_ts(to, from + p_col(s), mn_desc(vw, s), IO, s > 0 ? 1 : more, lane == 0);
-            if (FP16) {
-#pragma unroll
-              for (int s = 0; s < kKeys / 16; ++s) mma_ts(to, from + 16 + p_col(s), mn_desc(vw, s), IO, 1, lane == 0);
-            }
+              for (int s = 0; s < 4; ++s) {
+                mma_ts(to, from + 64 * b + p_col(s), mn_desc(vw + 512 * b, s), IO, s > 0 ? 1 : more | b, lane == 0);
+                if (FP16) mma_ts(to, from + 64 * b + 16 + p_col(s), mn_desc(vw + 512 * b, s), IO, 1, lane == 0);
+              }
             if (j + 1 < tiles) {
               scores(t, n + 1);
             } else {
