@@ -274,6 +274,7 @@ typedef struct qflash_kv4_cache {
   int32_t* lens;
   int32_t* ctl;
   int32_t Z, H, capacity, D;
+  int32_t device; /* that owns the buffers; -1: found out on every call */
 } qflash_kv4_cache;
 
 /*

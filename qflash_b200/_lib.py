@@ -28,7 +28,7 @@ _I64x4 = ctypes.POINTER(ctypes.c_int64)
 class KV4CacheStruct(ctypes.Structure):
     """qflash_kv4_cache."""
     _fields_ = [(n, ctypes.c_void_p) for n in ("k_codes", "v_codes", "k_param", "v_param", "weight", "lens", "ctl")] + [
-        (n, ctypes.c_int32) for n in ("Z", "H", "capacity", "D")]
+        (n, ctypes.c_int32) for n in ("Z", "H", "capacity", "D", "device")]
 
 
 _KV4 = ctypes.POINTER(KV4CacheStruct)
@@ -259,48 +259,69 @@ def fwd_fused_window(q, k, v, table, index, window_mask, num_windows, q8, k8, v8
     _check(rc, "qflash_fwd_fused_window")
 
 
+# The cache's calls are made once per decoding step and layer, so their host time counts: strides are turned
+# into ctypes arrays once per layout, workspace sizes asked for once per shape.
+_A4 = ctypes.c_int64 * 4
+_KV4_STRIDES = {}
+_KV4_DTYPE = {}  # torch dtype -> DTYPES' number (this module does not import torch)
+
+
+def _kv4_strides(t):
+    st = t.stride()
+    a = _KV4_STRIDES.get(st)
+    if a is None:
+        if len(_KV4_STRIDES) > 4096:
+            _KV4_STRIDES.clear()
+        a = _KV4_STRIDES[st] = _A4(*st)
+    return a
+
+
+def _kv4_dtype(dtype) -> int:
+    n = _KV4_DTYPE.get(dtype)
+    if n is None:
+        n = _KV4_DTYPE[dtype] = DTYPES[str(dtype)]
+    return n
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-_KV4_DTYPE = {}  # torch dtype -> DTYPES' number, filled on first use (this module does not import torch)
-
-
-def _kv4_dtype(t) -> int:
-    n = _KV4_DTYPE.get(t.dtype)
-    if n is None:
-        n = _KV4_DTYPE[t.dtype] = DTYPES[str(t.dtype)]
-    return n
-
-
 def kv4_append(cache, k, v, new_lens, at, stream) -> None:
     """Launch qflash_kv4_append; no synchronisation."""
-    _check(load().qflash_kv4_append(cache, k.data_ptr(), v.data_ptr(), _kv4_dtype(k), _strides(k), _strides(v),
-                                    k.shape[2], _ptr(new_lens), _ptr(at), stream), "qflash_kv4_append")
+    rc = load().qflash_kv4_append(cache, k.data_ptr(), v.data_ptr(), _kv4_dtype(k.dtype), _kv4_strides(k),
+                                  _kv4_strides(v), k.shape[2], _ptr(new_lens), _ptr(at), stream)
+    if rc:
+        _check(rc, "qflash_kv4_append")
 
 
 def kv4_read(cache, k, v, count, start, stream) -> None:
     """Launch qflash_kv4_read; no synchronisation."""
-    _check(load().qflash_kv4_read(cache, k.data_ptr(), v.data_ptr(), _kv4_dtype(k), count, _ptr(start), stream),
-           "qflash_kv4_read")
+    rc = load().qflash_kv4_read(cache, k.data_ptr(), v.data_ptr(), _kv4_dtype(k.dtype), count, _ptr(start), stream)
+    if rc:
+        _check(rc, "qflash_kv4_read")
 
 
-def kv4_attend(cache, q, out, new_lens, scale, causal, weights_in, stream) -> None:
-    """Launch qflash_kv4_attend with a workspace of its own; no synchronisation."""
-    import torch
-    lib = load()
+def kv4_attend_workspace(cache, dtype, Hq, N, weights) -> int:
+    """Bytes of workspace a call needs; 0 also for one that kv4_attend will refuse."""
+    return load().qflash_kv4_attend_workspace(cache, _kv4_dtype(dtype), Hq, N, weights)
+
+
+def kv4_attend(cache, q, out, new_lens, scale, causal, weights_in, ws, ws_bytes, stream) -> None:
+    """Launch qflash_kv4_attend; no synchronisation."""
     _, Hq, N, _ = q.shape
-    dtype = _kv4_dtype(q)
-    ws = torch.empty(lib.qflash_kv4_attend_workspace(cache, dtype, Hq, N, weights_in is not None), dtype=torch.uint8,
-                     device=q.device)
-    _check(lib.qflash_kv4_attend(cache, q.data_ptr(), dtype, _strides(q), out.data_ptr(), _strides(out), Hq, N,
-                                 _ptr(new_lens), scale, causal, _ptr(weights_in), ws.data_ptr(), ws.numel(), stream),
-           "qflash_kv4_attend")
+    rc = load().qflash_kv4_attend(cache, q.data_ptr(), _kv4_dtype(q.dtype), _kv4_strides(q), out.data_ptr(),
+                                  _kv4_strides(out), Hq, N, _ptr(new_lens), scale, causal, _ptr(weights_in),
+                                  ws.data_ptr(), ws_bytes, stream)
+    if rc:
+        _check(rc, "qflash_kv4_attend")
 
 
 def kv4_evict(cache, to, budget, recent, kept, stream) -> None:
     """Launch qflash_kv4_evict; no synchronisation."""
-    _check(load().qflash_kv4_evict(cache, to, budget, recent, kept.data_ptr(), stream), "qflash_kv4_evict")
+    rc = load().qflash_kv4_evict(cache, to, budget, recent, kept.data_ptr(), stream)
+    if rc:
+        _check(rc, "qflash_kv4_evict")
 
 
 def fused_workspace_bytes(mask_zb: int, mask_hb: int, N: int) -> int:

@@ -33,7 +33,7 @@ class KV4Cache:
     ``lens`` int32 [Z], all contiguous CUDA tensors on one device."""
 
     __slots__ = ("k_codes", "v_codes", "k_param", "v_param", "weight", "lens", "_ctl", "_c", "_ref",
-                 "shape", "device")
+                 "_index", "_workspace", "_scale", "shape", "device")
 
     def __init__(self, k_codes: Tensor, v_codes: Tensor, k_param: Tensor, v_param: Tensor, weight: Tensor,
                  lens: Tensor):
@@ -57,8 +57,9 @@ class KV4Cache:
         self._ctl = torch.zeros(2, dtype=torch.int32, device=k_codes.device)
         self.shape, self.device = (Z, H, C, 2 * half), k_codes.device
         self._c = _lib.KV4CacheStruct(*(t.data_ptr() for t in (k_codes, v_codes, k_param, v_param, weight, lens,
-                                                               self._ctl)), Z, H, C, 2 * half)
+                                                               self._ctl)), Z, H, C, 2 * half, self.device.index)
         self._ref = ctypes.byref(self._c)
+        self._index, self._workspace, self._scale = self.device.index, {}, 1.0 / (2 * half) ** 0.5
 
     @classmethod
     def empty(cls, batch: int, kv_heads: int, capacity: int, head_dim: int, device="cuda") -> "KV4Cache":
@@ -85,10 +86,10 @@ class KV4Cache:
         if key.dtype not in _FLOATS or value.dtype != key.dtype:
             raise ValueError(f"key and value must be float32, float16 or bfloat16 of one dtype, got {key.dtype}, "
                              f"{value.dtype}")
-        self._same_device(key=key, value=value)
-        key, value = _inner(key), _inner(value)
-        _lib.kv4_append(self._ref, key, value, self._counts("new_lens", new_lens), self._counts("at", at),
-                        torch.cuda.current_stream(self.device).cuda_stream)
+        self._here("key", key)
+        self._here("value", value)
+        _lib.kv4_append(self._ref, _inner(key), _inner(value), self._counts("new_lens", new_lens),
+                        self._counts("at", at), _stream(self._index))
 
     def attend(self, query: Tensor, scale: float | None = None, causal: bool = True, new_lens: Tensor | None = None,
                accumulate: bool = False, weights: Tensor | None = None, out: Tensor | None = None) -> Tensor:
@@ -109,7 +110,7 @@ class KV4Cache:
             raise ValueError(f"query must be [{Z}, a multiple of {H}, N, {D}], got {tuple(query.shape)}")
         if query.dtype not in (torch.float16, torch.bfloat16):
             raise ValueError(f"query must be float16 or bfloat16, got {query.dtype}")
-        self._same_device(query=query)
+        self._here("query", query)
         if weights is None:
             weights = self.weight
         elif not accumulate:
@@ -123,9 +124,17 @@ class KV4Cache:
         elif out.shape != query.shape or out.dtype != query.dtype or out.stride(-1) != 1 or out.device != self.device:
             raise ValueError(f"out must be a {tuple(query.shape)} {query.dtype} tensor on {self.device} with a "
                              "contiguous last dim")
+        shape = (query.dtype, query.shape[1], query.shape[2], accumulate)
+        need = self._workspace.get(shape)
+        if need is None:
+            if len(self._workspace) > 4096:
+                self._workspace.clear()
+            need = self._workspace[shape] = _lib.kv4_attend_workspace(self._ref, *shape)
+        # of this call alone: two calls on one cache may run side by side, on streams or in graphs
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         _lib.kv4_attend(self._ref, query, out, self._counts("new_lens", new_lens),
-                        1.0 / D ** 0.5 if scale is None else scale, causal, weights if accumulate else None,
-                        torch.cuda.current_stream(self.device).cuda_stream)
+                        self._scale if scale is None else scale, causal, weights if accumulate else None, ws, need,
+                        _stream(self._index))
         return out
 
     def evict(self, budget: int, recent: int, out: "KV4Cache") -> Tensor:
@@ -144,7 +153,7 @@ class KV4Cache:
         if not 0 <= recent <= budget:
             raise ValueError(f"recent {recent} not in [0, {budget}]")
         kept = torch.empty((Z, H, budget), dtype=torch.int32, device=self.device)
-        _lib.kv4_evict(self._ref, out._ref, budget, recent, kept, torch.cuda.current_stream(self.device).cuda_stream)
+        _lib.kv4_evict(self._ref, out._ref, budget, recent, kept, _stream(self._index))
         return kept
 
     def read(self, count: int | None = None, start: Tensor | None = None,
@@ -160,7 +169,7 @@ class KV4Cache:
             raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
         k, v = (torch.empty((Z, H, count, D), dtype=dtype, device=self.device) for _ in range(2))
         _lib.kv4_read(self._ref, k, v, count, self._counts("start", start),
-                      torch.cuda.current_stream(self.device).cuda_stream)
+                      _stream(self._index))
         return k, v
 
     def check(self) -> None:
@@ -176,19 +185,19 @@ class KV4Cache:
             raise OverflowError(f"tokens outside the cache's {self.shape[2]} positions were dropped")
 
     def _counts(self, name, t):
-        if t is not None and (tuple(t.shape) != self.shape[:1] or t.dtype != torch.int32 or t.device != self.device
+        if t is not None and (t.shape != self.shape[:1] or t.dtype != torch.int32 or t.device != self.device
                               or not t.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous int32 [{self.shape[0]}] tensor on {self.device}, got "
                              f"{t.dtype} {tuple(t.shape)} on {t.device}")
         return t
 
-    def _same_device(self, **tensors):
-        for name, t in tensors.items():
-            if t.device != self.device:
-                raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
+    def _here(self, name, t):
+        if t.device != self.device:
+            raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
 
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(device).cuda_stream without the object
 
 
 def _inner(t: Tensor) -> Tensor:

@@ -9,6 +9,7 @@
 // rint to even.  A vector of zeros has scale 0; one with an infinity or a NaN
 // has scale NaN (all it stands for is NaN) and codes 0.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "kv4_common.cuh"
@@ -527,6 +528,38 @@ int check_cache(const qflash_kv4_cache* c, const char* what) {
   return QFLASH_OK;
 }
 
+// Makes the cache's device current for a call's launches, and the caller's again behind them.
+struct OnDevice {
+  int prev = -1, dev = 0, rc = QFLASH_OK;
+  explicit OnDevice(const qflash_kv4_cache* c) {
+    int cur = -1;
+    if (cudaGetDevice(&cur) != cudaSuccess) {
+      cudaGetLastError();
+      cur = -1;
+    }
+    if (c->device == cur && cur >= 0 && known(cur)) {
+      dev = cur;
+      return;
+    }
+    prev = cur;
+    rc = select_device(c->k_codes, &dev);
+    if (!rc && c->device >= 0 && c->device != dev)
+      rc = set_err(QFLASH_ERR_ARG, "kv4: the cache's buffers are on device %d, not %d", dev, c->device);
+    if (!rc) seen()[dev].store(true, std::memory_order_relaxed);
+  }
+  ~OnDevice() {
+    if (prev >= 0 && prev != dev) cudaSetDevice(prev);
+  }
+  OnDevice(const OnDevice&) = delete;
+  OnDevice& operator=(const OnDevice&) = delete;
+  static constexpr int kDevices = 64;  // as many as select_device knows
+  static std::atomic<bool>* seen() {  // devices that select_device has accepted
+    static std::atomic<bool> s[kDevices];
+    return s;
+  }
+  static bool known(int d) { return d < kDevices && seen()[d].load(std::memory_order_relaxed); }
+};
+
 static size_t elt(int dtype) { return dtype == kF32 ? 4 : 2; }
 
 // rows of 8-element runs can be loaded 16 bytes at a time
@@ -581,9 +614,9 @@ extern "C" int qflash_kv4_append(const qflash_kv4_cache* cache, const void* k, c
   if (cache->Z == 0 || N == 0) return QFLASH_OK;
   if (!k || !v || !k_strides || !v_strides) return set_err(QFLASH_ERR_ARG, "kv4 append: null pointer");
   if (k_strides[3] != 1 || v_strides[3] != 1) return set_err(QFLASH_ERR_ARG, "kv4 append: innermost (head-dim) stride must be 1");
-  DeviceGuard keep_device;
-  int dev = 0;
-  if (int rc = select_device(cache->k_codes, &dev)) return rc;
+  OnDevice on(cache);
+  if (on.rc) return on.rc;
+  const int dev = on.dev;
   AppendArgs a;
   a.c = view(cache);
   a.x[0] = k, a.x[1] = v;
@@ -603,9 +636,9 @@ extern "C" int qflash_kv4_read(const qflash_kv4_cache* cache, void* k, void* v, 
   if (cache->Z == 0 || N == 0) return QFLASH_OK;
   if (!k || !v) return set_err(QFLASH_ERR_ARG, "kv4 read: null pointer");
   if (((uintptr_t)k | (uintptr_t)v) & 15) return set_err(QFLASH_ERR_ALIGN, "kv4 read: outputs must be 16-byte aligned");
-  DeviceGuard keep_device;
-  int dev = 0;
-  if (int rc = select_device(cache->k_codes, &dev)) return rc;
+  OnDevice on(cache);
+  if (on.rc) return on.rc;
+  const int dev = on.dev;
   ReadArgs a = {view(cache), {k, v}, N, start, {}};
   cudaStream_t s = (cudaStream_t)stream;
   return dtype == kF32 ? launch_read<float>(a, sm_count(dev), s) : dtype == kF16 ? launch_read<__half>(a, sm_count(dev), s) : launch_read<__nv_bfloat16>(a, sm_count(dev), s);
@@ -631,9 +664,9 @@ extern "C" int qflash_kv4_evict(const qflash_kv4_cache* from, const qflash_kv4_c
       if (overlap(x.a, fc * x.bytes, y.b, tc * y.bytes))
         return set_err(QFLASH_ERR_ARG, "kv4 evict: the caches share memory");
   if (overlap(from->lens, 4 * (size_t)from->Z, to->lens, 4 * (size_t)to->Z)) return set_err(QFLASH_ERR_ARG, "kv4 evict: the caches share memory");
-  DeviceGuard keep_device;
-  int dev = 0;
-  if (int rc = select_device(from->k_codes, &dev)) return rc;
+  OnDevice on(from);
+  if (on.rc) return on.rc;
+  const int dev = on.dev;
   const EvictArgs a = {view(from), view(to), budget, recent, kept};
   cudaStream_t s = (cudaStream_t)stream;
   // CTAs per head: as many as have SMs of their own, as long as each has some thousand positions
@@ -701,9 +734,9 @@ extern "C" int qflash_kv4_attend(const qflash_kv4_cache* cache, const void* q, i
   if (!workspace || workspace_bytes < need)
     return set_err(QFLASH_ERR_ARG, "kv4 attend: workspace of %zu bytes, %zu are needed", workspace ? workspace_bytes : 0, need);
   if ((uintptr_t)workspace & 15) return set_err(QFLASH_ERR_ALIGN, "kv4 attend: workspace must be 16-byte aligned");
-  DeviceGuard keep_device;
-  int dev = 0;
-  if (int rc = select_device(cache->k_codes, &dev)) return rc;
+  OnDevice on(cache);
+  if (on.rc) return on.rc;
+  const int dev = on.dev;
   AttendArgs a;
   a.c = view(cache);
   a.q = q, a.out = out;

@@ -29,6 +29,7 @@
 // forms S^T = K Q^T again, a thread a key, and adds up exp(S - m) / l along its
 // row of columns: no sum crosses threads, and no atomics.
 #include <algorithm>
+#include <atomic>
 
 #include "kv4_common.cuh"
 #include "sm100_ptx.cuh"
@@ -946,7 +947,7 @@ static PromptArgs plan_prompt(const AttendArgs& a, bool weights, int sms, size_t
   return p;
 }
 
-constexpr int kSms = 148;
+constexpr int kSms = 148, kDevices = 64;  // as many as select_device knows
 
 size_t prompt_workspace(const qflash_kv4_cache* c, int Hq, int N, bool weights) {
   AttendArgs a;
@@ -956,23 +957,26 @@ size_t prompt_workspace(const qflash_kv4_cache* c, int Hq, int N, bool weights) 
   return n;
 }
 
-template <class K>
-static int allow_smem(K* kernel, uint32_t bytes) {
+template <void (*kernel)(PromptArgs)>
+static int allow_smem(uint32_t bytes, int dev) {
+  static std::atomic<bool> done[kDevices];  // per kernel and device
+  if (done[dev].load(std::memory_order_relaxed)) return QFLASH_OK;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess)
     return set_err(QFLASH_ERR_LAUNCH, "kv4 prompt: shared memory: %s", cudaGetErrorString(cudaGetLastError()));
+  done[dev].store(true, std::memory_order_relaxed);
   return QFLASH_OK;
 }
 
 template <int D, bool FP16>
-static int launch_prompt(const PromptArgs& p, cudaStream_t s) {
-  if (int rc = allow_smem(prompt_kernel<D, FP16>, Layout<D>::BYTES)) return rc;
+static int launch_prompt(const PromptArgs& p, int dev, cudaStream_t s) {
+  if (int rc = allow_smem<prompt_kernel<D, FP16>>(Layout<D>::BYTES, dev)) return rc;
   prompt_kernel<D, FP16><<<p.grid, kPrompt, Layout<D>::BYTES, s>>>(p);
   if (int rc = check_launch("kv4 prompt", p.grid)) return rc;
   const unsigned n = 8 * p.grid + p.a.c.Z * p.row_tiles;
   prompt_finish_kernel<D, FP16><<<n, 256, 0, s>>>(p);
   if (int rc = check_launch("kv4 prompt finish", n)) return rc;
   if (!p.stats) return QFLASH_OK;
-  if (int rc = allow_smem(prompt_weights_kernel<D, FP16>, WLayout<D>::BYTES)) return rc;
+  if (int rc = allow_smem<prompt_weights_kernel<D, FP16>>(WLayout<D>::BYTES, dev)) return rc;
   const unsigned nw = (unsigned)(p.a.c.Z * p.a.c.H) * ((p.a.c.C + kKeys - 1) / kKeys);
   prompt_weights_kernel<D, FP16><<<nw, 288, WLayout<D>::BYTES, s>>>(p);
   return check_launch("kv4 prompt weights", nw);
@@ -986,8 +990,8 @@ int attend_prompt(const AttendArgs& a, bool fp16, void* ws, int dev, cudaStream_
   p.stats = a.weights_in ? (float2*)((uint8_t*)ws + (size_t)p.stats) : nullptr;
   auto aligned = [](const void* q, const int64_t* st) { return (((uintptr_t)q | (st[0] * 2) | (st[1] * 2) | (st[2] * 2)) & 15) == 0; };
   p.vec_q = aligned(a.q, a.qs), p.vec_o = aligned(a.out, a.os);
-  if (a.c.D == 64) return fp16 ? launch_prompt<64, true>(p, s) : launch_prompt<64, false>(p, s);
-  return fp16 ? launch_prompt<128, true>(p, s) : launch_prompt<128, false>(p, s);
+  if (a.c.D == 64) return fp16 ? launch_prompt<64, true>(p, dev, s) : launch_prompt<64, false>(p, dev, s);
+  return fp16 ? launch_prompt<128, true>(p, dev, s) : launch_prompt<128, false>(p, dev, s);
 }
 
 }  // namespace kv4
