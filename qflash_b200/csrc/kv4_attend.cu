@@ -401,6 +401,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
   const uint32_t ring = shared_addr(smem) + warp * (S::COUNT * S::BYTES);
   const AttendArgs& a = p.a;
   const Cache& c = a.c;
+  may_begin();
   long long before, total;
   cost_before(p, 0, &before, &total);
   const int grid = (int)min((long long)p.grid, total);  // no CTA's run is empty
@@ -561,6 +562,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
 // weights (the blocks behind them: kChunk positions of a head each).
 constexpr int kChunk = 1024;
 constexpr int kJoin = 256;  // threads
+constexpr int kPer = (kGridMax + kJoin - 1) / kJoin;
 
 template <int D, int NT, bool FP16>
 __global__ void __launch_bounds__(kJoin) rows_finish_kernel(RowsArgs p) {
@@ -572,6 +574,8 @@ __global__ void __launch_bounds__(kJoin) rows_finish_kernel(RowsArgs p) {
   const AttendArgs& a = p.a;
   const Cache& c = a.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // one block at least waits, whatever it has to do: the kernels behind this one go by its end
+  if (blockIdx.x == 0) wait_for_previous();
   const int joins = c.Z * c.H * p.rows;
   const bool weigh = (int)blockIdx.x >= joins;
   const int chunks = (c.C + kChunk - 1) / kChunk;
@@ -595,37 +599,51 @@ __global__ void __launch_bounds__(kJoin) rows_finish_kernel(RowsArgs p) {
     const int c0 = tiles ? holder(first + kBegin) : 0, n = tiles ? holder(first + cost - 1) - c0 + 1 : 0;
     if (n == 1) return;  // written by its holder
     constexpr int G = kJoin / D;  // groups of threads that share a row's pieces
+    constexpr int kAhead = 4;     // pieces whose part of O is on its way before the maximum is known
     const int d = tid % D, group = tid / D;
     float y = 0.f;
+    wait_for_previous();
     if (seen) {
-      float mx = -INFINITY;
-      for (int k = tid; k < n; k += kJoin) mx = fmaxf(mx, part_of(first, c0, c0 + k)[r]);
+      auto piece = [&](int k) { return part_of(first, c0, c0 + k); };
+      float pre[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) pre[i] = group + i * G < n ? piece(group + i * G)[2 * R + r * D + d] : 0.f;
+      float pm[kPer], pl[kPer], mx = -INFINITY;  // this thread's pieces: tid, tid + kJoin ..
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int k = tid + i * kJoin;
+        pm[i] = k < n ? piece(k)[r] : -INFINITY;
+        pl[i] = k < n ? piece(k)[R + r] : 0.f;
+        mx = fmaxf(mx, pm[i]);
+      }
 #pragma unroll
       for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
       if (lane == 0) red[warp] = mx;
       __syncthreads();
 #pragma unroll
       for (int w = 0; w < kJoin / 32; ++w) mx = fmaxf(mx, red[w]);
-      __syncthreads();
       float l = 0.f;
-      for (int k = tid; k < n; k += kJoin) {
-        const float* part = part_of(first, c0, c0 + k);
-        const float f = part[r] == -INFINITY ? 1.f : ex2(part[r] - mx);
-        sf[k] = f;
-        l += f * part[R + r];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const float f = pm[i] == -INFINITY ? 1.f : ex2(pm[i] - mx);
+        if (tid + i * kJoin < n) sf[tid + i * kJoin] = f;
+        l += f * pl[i];
       }
 #pragma unroll
       for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
-      if (lane == 0) red[warp] = l;
+      if (lane == 0) sums[warp] = l;
       __syncthreads();
       l = 0.f;
 #pragma unroll
-      for (int w = 0; w < kJoin / 32; ++w) l += red[w];
+      for (int w = 0; w < kJoin / 32; ++w) l += sums[w];
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (group + i * G < n) y += sf[group + i * G] * pre[i];
       // all but the first piece lie in their CTAs' slot 0
-      if (group == 0) y = sf[0] * part_of(first, c0, c0)[2 * R + r * D + d];
       const float* part = p.parts + (size_t)2 * c0 * kPart + 2 * R + r * D + d;
 #pragma unroll 8
-      for (int k = 1 + group; k < n; k += G) y += sf[k] * part[(size_t)2 * k * kPart];
+      for (int k = group + kAhead * G; k < n; k += G) y += sf[k] * part[(size_t)2 * k * kPart];
       sums[tid] = y;
       __syncthreads();
 #pragma unroll
@@ -644,6 +662,18 @@ __global__ void __launch_bounds__(kJoin) rows_finish_kernel(RowsArgs p) {
   // weights: w_j += sum over rows of 2^(S_rj - m_r) / l_r
   const int j0 = (blockIdx.x - joins) % chunks * kChunk, j1 = min(sp.len, j0 + kChunk);
   if (j0 >= j1) return;
+  constexpr int kKeysPer = kChunk / kJoin;
+  float old[kKeysPer];
+#pragma unroll
+  for (int i = 0; i < kKeysPer; ++i) old[i] = j0 + tid + i * kJoin < j1 ? a.weights_in[(size_t)zh * c.C + j0 + tid + i * kJoin] : 0.f;
+  wait_for_previous();
+  const float* scores = p.scores + (size_t)zh * c.C * p.score_rows;
+  float4 ahead[kKeysPer];  // the scores of up to 4 rows, on their way before the rows' maxima are known
+#pragma unroll
+  for (int i = 0; i < kKeysPer; ++i) {
+    const int j = j0 + tid + i * kJoin;
+    ahead[i] = p.score_rows == 4 && j < min(j1, most) ? *reinterpret_cast<const float4*>(scores + (size_t)j * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
   for (int row = warp; row < p.rows; row += kJoin / 32) {
     float mx = -INFINITY, l = 0.f;
     const bool seen = tiles && sp.limit(a, a.tok0 + row / a.rep) > 0;
@@ -669,16 +699,25 @@ __global__ void __launch_bounds__(kJoin) rows_finish_kernel(RowsArgs p) {
     if (lane == 0) sm[row] = mx == -INFINITY ? 0.f : mx, sinv[row] = seen ? 1.f / l : 0.f;
   }
   __syncthreads();
-  for (int j = j0 + tid; j < j1; j += kJoin) {
+#pragma unroll
+  for (int i = 0; i < kKeysPer; ++i) {
+    const int j = j0 + tid + i * kJoin;
+    if (j >= j1) break;
     float add = 0.f;
     if (j < most) {
-      const float* s = p.scores + ((size_t)zh * c.C + j) * p.score_rows;
+      const float* s = scores + (size_t)j * p.score_rows;
+      const float x[4] = {ahead[i].x, ahead[i].y, ahead[i].z, ahead[i].w};
+      if (p.score_rows == 4) {
+#pragma unroll
+        for (int row = 0; row < 4; ++row)
+          if (row < p.rows && j < sp.limit(a, a.tok0 + row / a.rep)) add += ex2(x[row] - sm[row]) * sinv[row];
+      } else {
 #pragma unroll 4
-      for (int row = 0; row < p.rows; ++row)
-        if (j < sp.limit(a, a.tok0 + row / a.rep)) add += ex2(s[row] - sm[row]) * sinv[row];
+        for (int row = 0; row < p.rows; ++row)
+          if (j < sp.limit(a, a.tok0 + row / a.rep)) add += ex2(s[row] - sm[row]) * sinv[row];
+      }
     }
-    const size_t w = (size_t)zh * c.C + j;
-    c.weight[w] = a.weights_in[w] + add;
+    c.weight[(size_t)zh * c.C + j] = old[i] + add;
   }
 }
 
@@ -728,7 +767,7 @@ static int launch_rows(RowsArgs r, int dev, cudaStream_t s) {
   rows_kernel<D, NT, FP16><<<r.grid, kWarps * 32, smem, s>>>(r);
   if (int rc = check_launch("kv4 rows", r.grid)) return rc;
   const unsigned grid = (unsigned)(c.Z * c.H) * (r.rows + (r.scores ? (c.C + kChunk - 1) / kChunk : 0));
-  rows_finish_kernel<D, NT, FP16><<<grid, kJoin, 0, s>>>(r);
+  launch_behind(rows_finish_kernel<D, NT, FP16>, grid, kJoin, s, r);
   return check_launch("kv4 rows finish", grid);
 }
 

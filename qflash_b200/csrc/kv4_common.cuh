@@ -81,6 +81,22 @@ __device__ __forceinline__ void store8(T* p, bool vec, const float (&x)[8]) {
   }
 }
 
+// A kernel that begins while the one before it in the stream still runs: what it does before
+// wait_for_previous may read nothing that one writes.  The one before says may_begin
+// once all its CTAs are resident, so the second kernel's blocks take no place from it.
+__device__ __forceinline__ void may_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <class A>
+inline void launch_behind(void (*kernel)(A), unsigned grid, unsigned threads, cudaStream_t s, const A& args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid), cfg.blockDim = dim3(threads), cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, args);
+}
+
 int check_cache(const qflash_kv4_cache* c, const char* what);
 int check_launch(const char* what, unsigned grid);
 

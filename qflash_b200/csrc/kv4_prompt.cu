@@ -212,7 +212,44 @@ __device__ __forceinline__ void put_codes(uint32_t base, int row, uint4 (&codes)
     for (int e = 0; e + 1 < D / 32; ++e) codes[e] = codes[e + 1];
   }
 }
-// One query row, likewise.
+// The same in the elements' own order: an exchange of halves more per word.
+template <int D, bool FP16>
+__device__ __forceinline__ void put_codes_plain(uint32_t base, int row, uint4 (&codes)[D / 32], uint32_t magic, uint32_t zero) {
+  const uint32_t to = base + row * 128, turn = (uint32_t)(row & 7) << 4;
+#pragma unroll 1
+  for (int i = 0; i < D / 32; ++i) {
+    const uint32_t w[4] = {codes[0].x, codes[0].y, codes[0].z, codes[0].w};
+    const uint32_t block = to + (i >> 1) * (128 * 128), chunk = (i & 1) * 64;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint4 y = decode8<FP16>(w[j], magic, zero);  // 0 4, 1 5, 2 6, 3 7
+      sts128(block + ((chunk + 16 * j) ^ turn), make_uint4(__byte_perm(y.x, y.y, 0x5410), __byte_perm(y.z, y.w, 0x5410),
+                                                           __byte_perm(y.x, y.y, 0x7632), __byte_perm(y.z, y.w, 0x7632)));
+    }
+#pragma unroll
+    for (int e = 0; e + 1 < D / 32; ++e) codes[e] = codes[e + 1];
+  }
+}
+// One query row in its own order, copied past the registers where it starts on a
+// 16-byte boundary (complete after the copies' wait), zeros for one that is not there.
+template <int D>
+__device__ __forceinline__ void copy_query(uint32_t base, int row, const uint16_t* q, const uint16_t* any, bool vec) {
+#pragma unroll 4
+  for (int chunk = 0; chunk < D / 8; ++chunk) {
+    const uint32_t to = base + (chunk / 8) * (128 * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+    if (vec) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(q ? q + 8 * chunk : any), "r"(q ? 16 : 0) : "memory");
+    } else {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (q) {
+        const uint16_t* p = q + 8 * chunk;
+        x = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
+      }
+      sts128(to, x);
+    }
+  }
+}
+// One query row in the order of put_codes.
 template <int D>
 __device__ __forceinline__ void put_query(uint32_t base, int row, const uint16_t* q, bool vec) {
 #pragma unroll 4
@@ -512,6 +549,7 @@ __global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
     if (lane == 0) mbar_arrive(bar);
   };
 
+  may_begin();
   Walk w;
   const long long total = Walk::total_tiles(p);
   const int grid = (int)min((long long)p.grid, total);
@@ -716,6 +754,8 @@ __global__ void __launch_bounds__(256) prompt_finish_kernel(PromptArgs p) {
   const AttendArgs& a = p.a;
   const Cache& c = a.c;
   constexpr int kPart = kRows * (D + 2);
+  // one block at least waits, whatever it has to do: the kernels behind this one go by its end
+  if (blockIdx.x == 0) wait_for_previous();
   auto put = [&](int z, int h, int row, int col, const float (&x)[8]) {
     const int tok = row / a.rep;
     const size_t to = z * a.os[0] + (h * a.rep + row % a.rep) * a.os[1] + (size_t)tok * a.os[2] + col;
@@ -727,6 +767,7 @@ __global__ void __launch_bounds__(256) prompt_finish_kernel(PromptArgs p) {
   if ((int)blockIdx.x >= 8 * p.grid) {
     const int i = blockIdx.x - 8 * p.grid, z = i / p.row_tiles, rt = i % p.row_tiles;
     if (unit_tiles(p, z, rt) > 0) return;
+    wait_for_previous();
     const float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     for (int e = threadIdx.x; e < kRows * (D / 8); e += 256) {
       const int row = rt * kRows + e / (D / 8);
@@ -745,6 +786,7 @@ __global__ void __launch_bounds__(256) prompt_finish_kernel(PromptArgs p) {
   const long long end = w.first + w.tiles;
   const Span sp = span_of(a, w.z);
   const int first = run_begin(total, grid, k - 1) < w.first ? 2 * (k - 1) + 1 : 2 * (k - 1);
+  wait_for_previous();
   for (int e = threadIdx.x; e < 32 * (D / 8); e += 256) {
     const int r = (blockIdx.x & 7) * 32 + e / (D / 8), col = e % (D / 8) * 8, row = w.rt * kRows + r;
     if (row >= p.rows) break;
@@ -773,6 +815,7 @@ __global__ void __launch_bounds__(256) prompt_finish_kernel(PromptArgs p) {
 }
 
 // ------------------------------------------------------------------ weights
+constexpr int kWeigh = 416;
 template <int D>
 struct WLayout {
   static constexpr uint32_t TILE = 128 * D * 2;
@@ -780,10 +823,12 @@ struct WLayout {
   static constexpr uint32_t BYTES = BARS + 128 + 1024;
 };
 
-// One CTA per 128 positions of a head: warps 0-3 add up (a thread a position),
-// warps 4-7 bring query tiles, warp 8 issues the products.
+// One CTA per 128 positions of a head: warps 0-7 add up (two threads a position,
+// for 64 columns of a tile each), warps 8-11 bring query tiles, warp 12 issues the
+// products.  What bounds it is exponentials, and with one thread a position the
+// latencies of 4 warps.
 template <int D, bool FP16>
-__global__ void __launch_bounds__(288, 2) prompt_weights_kernel(PromptArgs p) {
+__global__ void __launch_bounds__(kWeigh, 2) prompt_weights_kernel(PromptArgs p) {
   using L = WLayout<D>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u;
@@ -791,8 +836,8 @@ __global__ void __launch_bounds__(288, 2) prompt_weights_kernel(PromptArgs p) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const AttendArgs& a = p.a;
   const Cache& c = a.c;
-  const int key_tiles = (c.C + kKeys - 1) / kKeys;
-  const int zh = blockIdx.x / key_tiles, key0 = blockIdx.x % key_tiles * kKeys, z = zh / c.H, h = zh % c.H;
+  // the first positions first: with a causal limit most rows see them
+  const int heads = c.Z * c.H, zh = blockIdx.x % heads, key0 = blockIdx.x / heads * kKeys, z = zh / c.H, h = zh % c.H;
   const Span sp = span_of(a, z);
   if (key0 >= sp.len) return;
   // rows that see position key0: from token `first` on
@@ -811,14 +856,15 @@ __global__ void __launch_bounds__(288, 2) prompt_weights_kernel(PromptArgs p) {
   auto s_empty = [&](int i) { return bars + 48 + 8 * i; };
   const uint32_t k_full = bars + 64, done = bars + 72, slot = bars + 80;
   volatile uint32_t* abort = reinterpret_cast<volatile uint32_t*>(smem + L::BARS + 84);
+  __shared__ float other[kKeys];
   float* const col = reinterpret_cast<float*>(smem + L::COL);  // [2][3][128]: maximum, 1 / sum, limit
-  if (warp == 8) {
+  if (warp == 12) {
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
-        mbar_init(q_full(i), 128), mbar_init(q_empty(i), 129);
-        mbar_init(s_full(i), 1), mbar_init(s_empty(i), 128);
+        mbar_init(q_full(i), 4), mbar_init(q_empty(i), 9);
+        mbar_init(s_full(i), 1), mbar_init(s_empty(i), 8);
       }
-      mbar_init(k_full, 128), mbar_init(done, 1);
+      mbar_init(k_full, 4), mbar_init(done, 1);
       *abort = 0;
       fence_mbar_init();
     }
@@ -833,73 +879,95 @@ __global__ void __launch_bounds__(288, 2) prompt_weights_kernel(PromptArgs p) {
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
   const Waiter wait{abort, c.ctl};
 
-  if (warp < 4) {
-    const int key = key0 + tid, at = min(key, sp.len - 1);
+  auto warp_arrive = [&](uint32_t bar) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+  };
+  const int key = key0 + (tid & 127);
+  float sum0 = 0.f, sum1 = 0.f;
+  if (warp < 8) {
+    const int at = min(key, sp.len - 1), half = warp >> 2;
     const uint32_t kp = key < sp.len ? __ldg(c.param[0] + head + at) : 0u;
     const float ks = param_scale(kp) * a.scale_log2e;
-    uint4 kc[D / 32];
-    const uint4* src = reinterpret_cast<const uint4*>(c.codes[0] + (head + at) * (D / 2));
+    if (half == 0) {
+      uint4 kc[D / 32];
+      const uint4* src = reinterpret_cast<const uint4*>(c.codes[0] + (head + at) * (D / 2));
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) kc[i] = __ldg(src + i);
-    put_codes<D, FP16>(base + L::K, tid, kc, p.magic_k, zero_pair<FP16>(kp));
-    fence_proxy_async_smem();
-    mbar_arrive(k_full);
-    const uint32_t s_at = tmem + ((uint32_t)(warp * 32) << 16);
-    float sum0 = 0.f, sum1 = 0.f;
+      for (int i = 0; i < D / 32; ++i) kc[i] = __ldg(src + i);
+      put_codes_plain<D, FP16>(base + L::K, tid, kc, p.magic_k, zero_pair<FP16>(kp));
+      fence_proxy_async_smem();
+      warp_arrive(k_full);
+    }
+    const uint32_t s_at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 64 * half;
     for (int rt = rt0; rt < rt1; ++rt) {
       const int g = rt - rt0, b = g & 1;
       if (!wait(s_full(b), g >> 1 & 1) || !wait(q_full(b), g >> 1 & 1)) goto out;
       tc_fence_after();
-      const float4* cm = reinterpret_cast<const float4*>(col + b * 384);
+      const float4* cm = reinterpret_cast<const float4*>(col + b * 384) + 16 * half;
       const float4* ci = cm + 32;
       const int4* cl = reinterpret_cast<const int4*>(cm + 64);
       // every row of the tile is there and sees all 128 positions
       const bool full = (rt + 1) * kM <= sp.fresh * a.rep && sp.limit(a, rt * kM / a.rep) >= key0 + kKeys;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float s[32];
-        tmem_ld32f(s_at + b * 128 + 32 * q, s);
+#pragma unroll 1
+      for (int q = 0; q < 2; ++q) {
+        float x[32];
+        tmem_begin32(s_at + b * 128 + 32 * q, x);
+        tmem_arrived(x);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float4 m = cm[8 * q + i], v = ci[8 * q + i];
-          float* x = s + 4 * i;
-          fma2(x[0], x[1], ks, ks, -m.x, -m.y);
-          fma2(x[2], x[3], ks, ks, -m.z, -m.w);
+          const float4 m = cm[8 * q + i];
+          fma2(x[4 * i], x[4 * i + 1], ks, ks, -m.x, -m.y);
+          fma2(x[4 * i + 2], x[4 * i + 3], ks, ks, -m.z, -m.w);
+        }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = ex2(x[e]);
-          if (!full) {
+        for (int i = 0; i < 32; ++i) x[i] = ex2(x[i]);
+        if (full) {
+          float t0 = 0.f, t1 = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 v = ci[8 * q + i];
+            fma2(x[4 * i], x[4 * i + 1], v.x, v.y, sum0, sum1);
+            fma2(x[4 * i + 2], x[4 * i + 3], v.z, v.w, t0, t1);
+            sum0 = x[4 * i], sum1 = x[4 * i + 1], t0 = x[4 * i + 2], t1 = x[4 * i + 3];
+          }
+          add2(sum0, sum1, t0, t1);
+        } else {  // a row that does not see the position may have any sum
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
             const int4 lim = cl[8 * q + i];
-            sum0 += key < lim.x ? x[0] * v.x : 0.f;
-            sum1 += key < lim.y ? x[1] * v.y : 0.f;
-            sum0 += key < lim.z ? x[2] * v.z : 0.f;
-            sum1 += key < lim.w ? x[3] * v.w : 0.f;
-          } else {
-            fma2(x[0], x[1], v.x, v.y, sum0, sum1);
-            fma2(x[2], x[3], v.z, v.w, x[0], x[1]);
-            sum0 = x[2], sum1 = x[3];
+            const float4 v = ci[8 * q + i];
+            sum0 += key < lim.x ? x[4 * i] * v.x : 0.f;
+            sum1 += key < lim.y ? x[4 * i + 1] * v.y : 0.f;
+            sum0 += key < lim.z ? x[4 * i + 2] * v.z : 0.f;
+            sum1 += key < lim.w ? x[4 * i + 3] * v.w : 0.f;
           }
         }
       }
       tc_fence_before();
-      mbar_arrive(s_empty(b));
-      mbar_arrive(q_empty(b));
+      warp_arrive(s_empty(b));
+      if (lane == 0) mbar_arrive(q_empty(b));
     }
-    if (key < sp.len) c.weight[head + key] = a.weights_in[head + key] + (sum0 + sum1);
-  } else if (warp < 8) {
-    const int r = tid - 128;
-    for (int rt = rt0; rt < rt1; ++rt) {
+  } else if (warp < 12) {
+    const int r = tid - 256;
+    const uint16_t* const q0 = (const uint16_t*)a.q;
+    for (int rt = rt0; rt <= rt1; ++rt) {  // one tile behind: the last one's copies have arrived
       const int g = rt - rt0, b = g & 1, row = rt * kM + r, tok = row / a.rep;
-      const int limit = row < p.rows && tok < sp.fresh ? sp.limit(a, tok) : 0;
-      const float2 st = limit > 0 ? __ldg(p.stats + (size_t)zh * p.rows + row) : make_float2(0.f, 0.f);
-      if (!wait(q_empty(b), (g >> 1 & 1) ^ 1)) goto out;
-      put_query<D>(base + L::Q + b * L::TILE, r,
-                   limit > 0 ? (const uint16_t*)a.q + (z * a.qs[0] + (h * a.rep + row % a.rep) * a.qs[1] + tok * a.qs[2]) : nullptr,
-                   p.vec_q);
-      col[b * 384 + r] = st.x == -INFINITY ? 0.f : st.x;
-      col[b * 384 + 128 + r] = st.y;
-      reinterpret_cast<int*>(col)[b * 384 + 256 + r] = limit;
-      fence_proxy_async_smem();
-      mbar_arrive(q_full(b));
+      if (rt < rt1) {
+        const int limit = row < p.rows && tok < sp.fresh ? sp.limit(a, tok) : 0;
+        const float2 st = limit > 0 ? __ldg(p.stats + (size_t)zh * p.rows + row) : make_float2(0.f, 0.f);
+        if (!wait(q_empty(b), (g >> 1 & 1) ^ 1)) goto out;
+        copy_query<D>(base + L::Q + b * L::TILE, r,
+                      limit > 0 ? q0 + (z * a.qs[0] + (h * a.rep + row % a.rep) * a.qs[1] + tok * a.qs[2]) : nullptr, q0, p.vec_q);
+        col[b * 384 + r] = st.x == -INFINITY ? 0.f : st.x;
+        col[b * 384 + 128 + r] = st.y;
+        reinterpret_cast<int*>(col)[b * 384 + 256 + r] = limit;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      if (rt > rt0) {
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        fence_proxy_async_smem();
+        warp_arrive(q_full(b ^ 1));
+      }
     }
   } else {
     constexpr uint32_t IS = idesc_f16(kM, !FP16, false);
@@ -921,15 +989,17 @@ __global__ void __launch_bounds__(288, 2) prompt_weights_kernel(PromptArgs p) {
   }
 out:
   __syncwarp();
-  if (warp == 8) {
+  if (warp == 12) {
     if (lane == 0) tc_commit(done);
     __syncwarp();
     mbar_wait(done, 0);
   }
+  if (warp >= 4 && warp < 8) other[tid - 128] = sum0 + sum1;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_dealloc(tmem, 256);
+  if (warp == 12) tmem_dealloc(tmem, 256);
+  if (tid < kKeys && key < sp.len) c.weight[head + key] = a.weights_in[head + key] + ((sum0 + sum1) + other[tid]);
 }
 
 // ------------------------------------------------------------------ host
@@ -973,12 +1043,12 @@ static int launch_prompt(const PromptArgs& p, int dev, cudaStream_t s) {
   prompt_kernel<D, FP16><<<p.grid, kPrompt, Layout<D>::BYTES, s>>>(p);
   if (int rc = check_launch("kv4 prompt", p.grid)) return rc;
   const unsigned n = 8 * p.grid + p.a.c.Z * p.row_tiles;
-  prompt_finish_kernel<D, FP16><<<n, 256, 0, s>>>(p);
+  launch_behind(prompt_finish_kernel<D, FP16>, n, 256, s, p);
   if (int rc = check_launch("kv4 prompt finish", n)) return rc;
   if (!p.stats) return QFLASH_OK;
   if (int rc = allow_smem<prompt_weights_kernel<D, FP16>>(WLayout<D>::BYTES, dev)) return rc;
   const unsigned nw = (unsigned)(p.a.c.Z * p.a.c.H) * ((p.a.c.C + kKeys - 1) / kKeys);
-  prompt_weights_kernel<D, FP16><<<nw, 288, WLayout<D>::BYTES, s>>>(p);
+  prompt_weights_kernel<D, FP16><<<nw, kWeigh, WLayout<D>::BYTES, s>>>(p);
   return check_launch("kv4 prompt weights", nw);
 }
 
