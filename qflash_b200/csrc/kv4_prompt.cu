@@ -819,7 +819,9 @@ constexpr int kWeigh = 416;
 template <int D>
 struct WLayout {
   static constexpr uint32_t TILE = 128 * D * 2;
-  static constexpr uint32_t K = 0, Q = TILE, COL = 3 * TILE, BARS = COL + 2 * 3 * 512;
+  // query tiles: 3 where two CTAs' fit into an SM
+  static constexpr int COUNT = D == 64 ? 3 : 2;
+  static constexpr uint32_t K = 0, Q = TILE, COL = (1 + COUNT) * TILE, BARS = COL + COUNT * 3 * 512;
   static constexpr uint32_t BYTES = BARS + 128 + 1024;
 };
 
@@ -851,19 +853,17 @@ __global__ void __launch_bounds__(kWeigh, 2) prompt_weights_kernel(PromptArgs p)
   }
   const uint32_t bars = base + L::BARS;
   auto q_full = [&](int i) { return bars + 8 * i; };
-  auto q_empty = [&](int i) { return bars + 16 + 8 * i; };
-  auto s_full = [&](int i) { return bars + 32 + 8 * i; };
-  auto s_empty = [&](int i) { return bars + 48 + 8 * i; };
-  const uint32_t k_full = bars + 64, done = bars + 72, slot = bars + 80;
-  volatile uint32_t* abort = reinterpret_cast<volatile uint32_t*>(smem + L::BARS + 84);
+  auto q_empty = [&](int i) { return bars + 24 + 8 * i; };
+  auto s_full = [&](int i) { return bars + 48 + 8 * i; };
+  auto s_empty = [&](int i) { return bars + 64 + 8 * i; };
+  const uint32_t k_full = bars + 80, done = bars + 88, slot = bars + 96;
+  volatile uint32_t* abort = reinterpret_cast<volatile uint32_t*>(smem + L::BARS + 100);
   __shared__ float other[kKeys];
   float* const col = reinterpret_cast<float*>(smem + L::COL);  // [2][3][128]: maximum, 1 / sum, limit
   if (warp == 12) {
     if (lane == 0) {
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(q_full(i), 4), mbar_init(q_empty(i), 9);
-        mbar_init(s_full(i), 1), mbar_init(s_empty(i), 8);
-      }
+      for (int i = 0; i < L::COUNT; ++i) mbar_init(q_full(i), 4), mbar_init(q_empty(i), 9);
+      for (int i = 0; i < 2; ++i) mbar_init(s_full(i), 1), mbar_init(s_empty(i), 8);
       mbar_init(k_full, 4), mbar_init(done, 1);
       *abort = 0;
       fence_mbar_init();
@@ -900,10 +900,10 @@ __global__ void __launch_bounds__(kWeigh, 2) prompt_weights_kernel(PromptArgs p)
     }
     const uint32_t s_at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 64 * half;
     for (int rt = rt0; rt < rt1; ++rt) {
-      const int g = rt - rt0, b = g & 1;
-      if (!wait(s_full(b), g >> 1 & 1) || !wait(q_full(b), g >> 1 & 1)) goto out;
+      const int g = rt - rt0, b = g & 1, qb = g % L::COUNT;
+      if (!wait(s_full(b), g >> 1 & 1) || !wait(q_full(qb), g / L::COUNT & 1)) goto out;
       tc_fence_after();
-      const float4* cm = reinterpret_cast<const float4*>(col + b * 384) + 16 * half;
+      const float4* cm = reinterpret_cast<const float4*>(col + qb * 384) + 16 * half;
       const float4* ci = cm + 32;
       const int4* cl = reinterpret_cast<const int4*>(cm + 64);
       // every row of the tile is there and sees all 128 positions
@@ -945,17 +945,18 @@ __global__ void __launch_bounds__(kWeigh, 2) prompt_weights_kernel(PromptArgs p)
       }
       tc_fence_before();
       warp_arrive(s_empty(b));
-      if (lane == 0) mbar_arrive(q_empty(b));
+      if (lane == 0) mbar_arrive(q_empty(qb));
     }
   } else if (warp < 12) {
     const int r = tid - 256;
     const uint16_t* const q0 = (const uint16_t*)a.q;
-    for (int rt = rt0; rt <= rt1; ++rt) {  // one tile behind: the last one's copies have arrived
-      const int g = rt - rt0, b = g & 1, row = rt * kM + r, tok = row / a.rep;
+    constexpr int kLag = L::COUNT - 2;  // tiles whose copies are still under way when the next are begun
+    for (int rt = rt0; rt < rt1 + kLag; ++rt) {
+      const int g = rt - rt0, b = g % L::COUNT, row = rt * kM + r, tok = row / a.rep;
       if (rt < rt1) {
         const int limit = row < p.rows && tok < sp.fresh ? sp.limit(a, tok) : 0;
         const float2 st = limit > 0 ? __ldg(p.stats + (size_t)zh * p.rows + row) : make_float2(0.f, 0.f);
-        if (!wait(q_empty(b), (g >> 1 & 1) ^ 1)) goto out;
+        if (!wait(q_empty(b), (g / L::COUNT & 1) ^ 1)) goto out;
         copy_query<D>(base + L::Q + b * L::TILE, r,
                       limit > 0 ? q0 + (z * a.qs[0] + (h * a.rep + row % a.rep) * a.qs[1] + tok * a.qs[2]) : nullptr, q0, p.vec_q);
         col[b * 384 + r] = st.x == -INFINITY ? 0.f : st.x;
@@ -963,10 +964,10 @@ __global__ void __launch_bounds__(kWeigh, 2) prompt_weights_kernel(PromptArgs p)
         reinterpret_cast<int*>(col)[b * 384 + 256 + r] = limit;
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
-      if (rt > rt0) {
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
+      if (g >= kLag) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
         fence_proxy_async_smem();
-        warp_arrive(q_full(b ^ 1));
+        warp_arrive(q_full((g - kLag) % L::COUNT));
       }
     }
   } else {
@@ -974,15 +975,15 @@ __global__ void __launch_bounds__(kWeigh, 2) prompt_weights_kernel(PromptArgs p)
     const uint32_t kw = k_word(base + L::K), qw = k_word(base + L::Q);
     if (!wait(k_full, 0)) goto out;
     for (int rt = rt0; rt < rt1; ++rt) {
-      const int g = rt - rt0, b = g & 1;
-      if (!wait(q_full(b), g >> 1 & 1) || !wait(s_empty(b), (g >> 1 & 1) ^ 1)) goto out;
+      const int g = rt - rt0, b = g & 1, qs = g % L::COUNT;
+      if (!wait(q_full(qs), g / L::COUNT & 1) || !wait(s_empty(b), (g >> 1 & 1) ^ 1)) goto out;
       tc_fence_after();
-      const uint32_t kb = uniform(kw), qb = uniform(qw + b * (L::TILE / 16)), to = uniform(tmem + b * 128);
+      const uint32_t kb = uniform(kw), qb = uniform(qw + qs * (L::TILE / 16)), to = uniform(tmem + b * 128);
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) mma_ss(to, k_desc(kb, s), k_desc(qb, s), IS, s > 0, lane == 0);
       if (lane == 0) {
         tc_commit(s_full(b));
-        tc_commit(q_empty(b));
+        tc_commit(q_empty(qs));
       }
       __syncwarp();
     }
