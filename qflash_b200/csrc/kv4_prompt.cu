@@ -293,28 +293,34 @@ __device__ __forceinline__ int unit_tiles(const PromptArgs& p, int z, int rt) {
   const int first = rt * kRows / a.rep, last = min(min(a.N, sp.fresh), (rt * kRows + kRows - 1) / a.rep + 1);
   return first >= last ? 0 : (sp.limit(a, last - 1) + kKeys - 1) / kKeys;
 }
+// What a unit counts for in the split: its queries and its output take the time of kBegin tiles.
+constexpr int kBegin = 2;
+__device__ __forceinline__ int cost_of(int tiles) { return tiles ? tiles + kBegin : 0; }
 
 // Where a CTA is in its run.  All lanes of a warp hold the same.
 struct Walk {
   int z, rt, h, tiles;   // the unit
-  long long first;       // its first tile
+  long long first;       // where it begins: kBegin places, then its tiles
   long long at, stop;    // the run
   int t0, t1;            // the piece: key tiles of the unit
+  int places;            // what of the run it takes
   bool whole;
 
   __device__ __forceinline__ void cut() {
-    t0 = (int)(at - first);
-    t1 = (int)min((long long)tiles, t0 + (stop - at));
+    const int u0 = (int)(at - first), u1 = (int)min((long long)cost_of(tiles), u0 + (stop - at));
+    places = u1 - u0;
+    t0 = max(0, u0 - kBegin);
+    t1 = max(0, u1 - kBegin);
     whole = t0 == 0 && t1 == tiles;
   }
-  // The unit that holds tile `where` (of `total`).  One warp together.
+  // The unit that holds a place.  One warp together.
   __device__ __forceinline__ bool seek(const PromptArgs& p, long long where) {
     const int lane = threadIdx.x & 31, n = p.a.c.Z * p.row_tiles, H = p.a.c.H;
     long long base = 0;
     for (int i0 = 0; i0 < n; i0 += 32) {
       const int i = i0 + lane;
       const int t = i < n ? unit_tiles(p, i / p.row_tiles, i % p.row_tiles) : 0;
-      const long long mine = (long long)t * H;
+      const long long mine = (long long)cost_of(t) * H;
       long long sum = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -327,38 +333,46 @@ struct Walk {
         tiles = __shfl_sync(~0u, t, l);
         first = base + __shfl_sync(~0u, sum - mine, l);
         z = (i0 + l) / p.row_tiles, rt = (i0 + l) % p.row_tiles;
-        h = (int)((where - first) / tiles);
-        first += (long long)h * tiles;
+        h = (int)((where - first) / cost_of(tiles));
+        first += (long long)h * cost_of(tiles);
         return true;
       }
       base += __shfl_sync(~0u, sum, 31);
     }
     return false;
   }
-  __device__ static long long total_tiles(const PromptArgs& p) {
+  __device__ static long long total_cost(const PromptArgs& p) {
     const int lane = threadIdx.x & 31, n = p.a.c.Z * p.row_tiles;
     long long sum = 0;
-    for (int i = lane; i < n; i += 32) sum += unit_tiles(p, i / p.row_tiles, i % p.row_tiles);
+    for (int i = lane; i < n; i += 32) sum += cost_of(unit_tiles(p, i / p.row_tiles, i % p.row_tiles));
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
     return sum * p.a.c.H;
   }
-  // On to the run's next piece; false behind its end.
-  __device__ __forceinline__ bool next(const PromptArgs& p) {
-    at += t1 - t0;
-    if (at >= stop) return false;
-    first += tiles;
-    if (++h == p.a.c.H) {
-      h = 0;
-      do {
-        if (++rt == p.row_tiles) {
-          rt = 0;
-          if (++z >= p.a.c.Z) return false;  // only if lens changed meanwhile
-        }
-        tiles = unit_tiles(p, z, rt);
-      } while (tiles == 0);
-    }
+  // The run's first piece with tiles in it, from `at` on.  One warp together.
+  __device__ __forceinline__ bool begin(const PromptArgs& p) {
+    if (!seek(p, at)) return false;  // only if lens changed meanwhile
     cut();
+    return t1 > t0 || next(p);
+  }
+  // On to the run's next piece with tiles in it; false behind its end.
+  __device__ __forceinline__ bool next(const PromptArgs& p) {
+    do {
+      at += places;
+      if (at >= stop) return false;
+      first += cost_of(tiles);
+      if (++h == p.a.c.H) {
+        h = 0;
+        do {
+          if (++rt == p.row_tiles) {
+            rt = 0;
+            if (++z >= p.a.c.Z) return false;  // only if lens changed meanwhile
+          }
+          tiles = unit_tiles(p, z, rt);
+        } while (tiles == 0);
+      }
+      cut();
+    } while (t1 <= t0);
     return true;
   }
 };
@@ -551,14 +565,13 @@ __global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
 
   may_begin();
   Walk w;
-  const long long total = Walk::total_tiles(p);
+  const long long total = Walk::total_cost(p);
   const int grid = (int)min((long long)p.grid, total);
   bool any = (int)blockIdx.x < grid;
   if (any) {
     w.at = run_begin(total, grid, blockIdx.x);
     w.stop = run_begin(total, grid, blockIdx.x + 1);
-    any = w.seek(p, w.at);  // false only if lens changed meanwhile
-    if (any) w.cut();
+    any = w.begin(p);
   }
 
   if (warp < 8) {
@@ -568,15 +581,23 @@ __global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
     uint32_t n = 0, pieces = 0;  // key tiles and pieces so far
-    while (any) {
+    // this thread's row of a unit: queries into shared memory
+    auto bring_query = [&] {
       const Span sp = span_of(a, w.z);
       const int row = w.rt * kRows + t * kM + lrow, tok = row / a.rep, head = w.h * a.rep + row % a.rep;
       const bool live = row < p.rows && tok < sp.fresh;
-      const int limit = live ? sp.limit(a, tok) : 0;
       put_query<D>(base + L::Q + t * L::TILE, lrow,
                    live ? (const uint16_t*)a.q + (w.z * a.qs[0] + head * a.qs[1] + tok * a.qs[2]) : nullptr, p.vec_q);
       fence_proxy_async_smem();
       warp_arrive(q_full(t));
+    };
+    if (any) bring_query();
+    while (any) {
+      const Span sp = span_of(a, w.z);
+      const int row = w.rt * kRows + t * kM + lrow, tok = row / a.rep, head = w.h * a.rep + row % a.rep;
+      const int limit = row < p.rows && tok < sp.fresh ? sp.limit(a, tok) : 0;
+      const bool whole = w.whole;
+      const int z = w.z, h = w.h;
       RowState r = {-INFINITY, 0.f, 1.f};
       for (int j = w.t0; j < w.t1; ++j, ++n) {
         if (!wait(s_full(t), n & 1)) goto out;
@@ -591,18 +612,22 @@ __global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
         tc_fence_before();
         warp_arrive(p_full(t));
       }
+      // the last scores are made, so the next unit's queries may come: their products with the first keys run
+      // under this unit's output
+      any = w.next(p);
+      if (any) bring_query();
       if (!wait(o_full(t), pieces & 1)) goto out;
       tc_fence_after();
       {
         const float inv = 1.f / r.l;
         const bool write = row < p.rows;
         float* part = p.parts + ((size_t)blockIdx.x * 2 + (pieces ? 1 : 0)) * (kRows * (D + 2));
-        const size_t to = w.z * a.os[0] + head * a.os[1] + (size_t)tok * a.os[2];
+        const size_t to = z * a.os[0] + head * a.os[1] + (size_t)tok * a.os[2];
         if (write) {
-          if (!w.whole)
+          if (!whole)
             part[t * kM + lrow] = r.m, part[kRows + t * kM + lrow] = r.l;
           else if (p.stats)
-            p.stats[((size_t)w.z * c.H + w.h) * p.rows + row] = make_float2(r.m, inv);
+            p.stats[((size_t)z * c.H + h) * p.rows + row] = make_float2(r.m, inv);
         }
 #pragma unroll 1
         for (int q = 0; q < D / 32; ++q) {
@@ -614,7 +639,7 @@ __global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const float y[8] = {o[8 * g], o[8 * g + 2], o[8 * g + 4], o[8 * g + 6], o[8 * g + 1], o[8 * g + 3], o[8 * g + 5], o[8 * g + 7]};
-            if (w.whole) {
+            if (whole) {
               float x[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) x[e] = limit > 0 ? y[e] * inv : 0.f;
@@ -630,7 +655,6 @@ __global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
         tc_fence_before();
       }
       ++pieces;
-      any = w.next(p);
     }
   } else if (warp < 12) {
     // ---------------------------------------------------------------- decoding
@@ -777,13 +801,14 @@ __global__ void __launch_bounds__(256) prompt_finish_kernel(PromptArgs p) {
     return;
   }
   const int k = blockIdx.x / 8;
-  const long long total = Walk::total_tiles(p);
+  const long long total = Walk::total_cost(p);
   const int grid = (int)min((long long)p.grid, total);
   if (k == 0 || k >= grid) return;
   Walk w;
   const long long cut = run_begin(total, grid, k);
-  if (!w.seek(p, cut) || w.first == cut || run_begin(total, grid, k - 1) > w.first) return;
-  const long long end = w.first + w.tiles;
+  // a cut that has tiles of its unit before it, and is the first to
+  if (!w.seek(p, cut) || cut <= w.first + kBegin || run_begin(total, grid, k - 1) > w.first + kBegin) return;
+  const long long end = w.first + cost_of(w.tiles);
   const Span sp = span_of(a, w.z);
   const int first = run_begin(total, grid, k - 1) < w.first ? 2 * (k - 1) + 1 : 2 * (k - 1);
   wait_for_previous();
