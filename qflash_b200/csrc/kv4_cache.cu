@@ -342,11 +342,35 @@ __device__ __forceinline__ uint32_t peer_word(const uint32_t* p, uint32_t rank) 
   return v;
 }
 
+// A word of CTA `rank` of the cluster, or of this one if it is alone.
+__device__ __forceinline__ uint32_t word_of(const uint32_t* p, int rank, int cs) { return cs > 1 ? peer_word(p, rank) : *p; }
+
+// The sum of a word over the cluster, all loads under way before the first is added.
+__device__ __forceinline__ uint32_t cluster_sum(const uint32_t* p, int cs) {
+  uint32_t x[kCluster], sum = 0;
+#pragma unroll
+  for (int r = 0; r < kCluster; ++r) x[r] = r < cs ? word_of(p, r, cs) : 0;
+#pragma unroll
+  for (int r = 0; r < kCluster; ++r) sum += x[r];
+  return sum;
+}
+
+__device__ __forceinline__ uint32_t warp_scan(uint32_t x) {  // of this lane and those below
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t up = __shfl_up_sync(~0u, x, o);
+    if ((threadIdx.x & 31) >= o) x += up;
+  }
+  return x;
+}
+
 __global__ void __launch_bounds__(kSelect) evict_select_kernel(EvictArgs a) {
-  constexpr int W = kSelect / 32, PER = kDigits / kSelect, TILE = kSelect * kKeep;
+  constexpr int W = kSelect / 32, GROUPS = kDigits / 32;
   __shared__ uint32_t hist[2][kDigits];  // of even and odd passes: peers may still read the last pass's
-  __shared__ uint32_t sums[W], counts[2], s_digit, s_left;
+  __shared__ uint32_t coarse[2][GROUPS];  // sums of 32 digits
+  __shared__ uint32_t counts[2], s_digit, s_left;
   __shared__ uint32_t warp_more[W], warp_same[W];
+  may_begin();
   const int cs = (int)cluster_size(), rank = (int)cluster_rank();
   const int zh = blockIdx.x / cs, z = zh / a.from.H, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n = length_of(a.from, z);
@@ -362,87 +386,70 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(EvictArgs a) {
   for (int i = mine; i < a.recent; i += stride) kept[need + i] = old + i;
   if (need == 0) return;
   const int run = (old + cs - 1) / cs, i0 = min(old, rank * run), i1 = min(old, i0 + run);
-  const bool once = run <= TILE;
-  // a warp holds kKeep * 32 neighbouring positions: position at(t, j) of tile t in u[j]
+  // a thread holds `keep` positions of a tile in u, a warp's are neighbours: at(t, j), j < keep
+  const int keep = min(kKeep, (run + kSelect - 1) / kSelect), tile = kSelect * keep;
+  const bool once = run <= tile;
   uint32_t u[kKeep];
-  auto at = [&](int t, int j) { return i0 + t * TILE + (warp * kKeep + j) * 32 + lane; };
+  auto at = [&](int t, int j) { return i0 + t * tile + (warp * keep + j) * 32 + lane; };
   auto load = [&](int t) {
     float w[kKeep];
 #pragma unroll
-    for (int j = 0; j < kKeep; ++j) w[j] = at(t, j) < i1 ? __ldg(weight + at(t, j)) : 0.f;
+    for (int j = 0; j < kKeep; ++j) w[j] = j < keep && at(t, j) < i1 ? __ldg(weight + at(t, j)) : 0.f;
 #pragma unroll
     for (int j = 0; j < kKeep; ++j) u[j] = order_of(w[j]);
   };
-  const int tiles = (i1 - i0 + TILE - 1) / TILE;
+  const int tiles = (i1 - i0 + tile - 1) / tile;
   uint32_t prefix = 0, left = need;  // among weights that begin with prefix, the left-th largest is looked for
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-    uint32_t* h = hist[pass & 1];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) h[i * kSelect + tid] = 0;
+    uint32_t *h = hist[pass & 1], *hc = coarse[pass & 1];
+    for (int i = tid; i < kDigits; i += kSelect) h[i] = 0;
     if (tid < 2) counts[tid] = 0;
     __syncthreads();
     for (int t = 0; t < tiles; ++t) {
       if (pass == 0 || !once) load(t);
 #pragma unroll
-      for (int j = 0; j < kKeep; ++j)
+      for (int j = 0; j < kKeep; ++j) {
+        if (j >= keep) break;
         if (at(t, j) < i1 && (pass == 0 || u[j] >> (shift + bits) == prefix >> (shift + bits)))
           atomicAdd(&h[u[j] >> shift & ((1 << bits) - 1)], 1u);
+      }
+    }
+    __syncthreads();
+    for (int i = warp; i < GROUPS; i += W) {
+      const uint32_t sum = __reduce_add_sync(~0u, h[32 * i + lane]);
+      if (lane == 0) hc[i] = sum;
     }
     if (cs > 1) cluster_sync(); else __syncthreads();
-    // thread t holds digits from the top: kDigits - 1 - PER t downwards
-    uint32_t d[PER], sum = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) d[i] = 0;
-    if (cs == 1) {
-#pragma unroll
-      for (int i = 0; i < PER; ++i) d[i] = h[kDigits - 1 - PER * tid - i];
-    } else {
-      uint32_t x[kCluster][PER];  // all on their way before the first is added
-#pragma unroll
-      for (int r = 0; r < kCluster; ++r)
-#pragma unroll
-        for (int i = 0; i < PER; ++i) x[r][i] = r < cs ? peer_word(h + kDigits - 1 - PER * tid - i, r) : 0;
-#pragma unroll
-      for (int r = 0; r < kCluster; ++r)
-#pragma unroll
-        for (int i = 0; i < PER; ++i) d[i] += x[r][i];
-    }
-#pragma unroll
-    for (int i = 0; i < PER; ++i) sum += d[i];
-    uint32_t upto = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t up = __shfl_up_sync(~0u, upto, o);
-      if (lane >= o) upto += up;
-    }
-    if (lane == 31) sums[warp] = upto;
-    __syncthreads();
-    upto += __reduce_add_sync(~0u, lane < warp ? sums[lane] : 0u);
-    uint32_t above = upto - sum;
-    if (above < left && left <= upto) {
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        if (above < left && left <= above + d[i]) s_digit = kDigits - 1 - PER * tid - i, s_left = left - above;
-        above += d[i];
-      }
+    if (warp == 0) {
+      // from the top: the group of 32 digits, two to a lane, then the digit, so that little crosses the cluster
+      const uint32_t g0 = cluster_sum(hc + GROUPS - 1 - 2 * lane, cs), g1 = cluster_sum(hc + GROUPS - 2 - 2 * lane, cs);
+      const uint32_t upto = warp_scan(g0 + g1), before = upto - g0 - g1;
+      const bool first = before < left && left <= before + g0, second = before + g0 < left && left <= upto;
+      const int l = __ffs(__ballot_sync(~0u, first || second)) - 1;
+      const int group = __shfl_sync(~0u, GROUPS - 1 - 2 * lane - (second ? 1 : 0), l);
+      const uint32_t above = __shfl_sync(~0u, before + (second ? g0 : 0), l);
+      const int digit = 32 * group + 31 - lane;
+      const uint32_t d = cluster_sum(h + digit, cs), to = above + warp_scan(d);
+      if (to - d < left && left <= to) s_digit = digit, s_left = left - (to - d);
     }
     __syncthreads();
     prefix |= s_digit << shift, left = s_left;
   }
   // heavier and equal positions of a warp's part of a tile
   auto count = [&](int t, uint32_t& more, uint32_t& same) {
-    more = same = 0;
+    uint32_t m = 0, e = 0;
 #pragma unroll
     for (int j = 0; j < kKeep; ++j) {
-      const bool in = at(t, j) < i1;
-      more += __popc(__ballot_sync(~0u, in && u[j] > prefix));
-      same += __popc(__ballot_sync(~0u, in && u[j] == prefix));
+      if (j >= keep) break;
+      m += at(t, j) < i1 && u[j] > prefix;
+      e += at(t, j) < i1 && u[j] == prefix;
     }
+    more = __reduce_add_sync(~0u, m), same = __reduce_add_sync(~0u, e);
   };
   // how many of them the CTAs before this one have
-  uint32_t done = 0, equal = 0, more, same;
+  uint32_t done = 0, equal = 0, more = 0, same = 0;
   if (cs > 1) {
     for (int t = 0; t < tiles; ++t) {
       if (!once) load(t);
@@ -450,11 +457,13 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(EvictArgs a) {
       if (lane == 0) atomicAdd(&counts[0], more), atomicAdd(&counts[1], same);
     }
     cluster_sync();
-    for (int r = 0; r < rank; ++r) done += peer_word(&counts[0], r), equal += peer_word(&counts[1], r);
+    uint32_t x[2] = {0, 0};
+    if (lane < 2 * rank) x[lane & 1] = peer_word(&counts[lane & 1], lane >> 1);
+    done = __reduce_add_sync(~0u, x[0]), equal = __reduce_add_sync(~0u, x[1]);
   }
   for (int t = 0; t < tiles; ++t) {
     if (!once) load(t);
-    count(t, more, same);
+    if (cs == 1 || !once) count(t, more, same);
     if (lane == 0) warp_more[warp] = more, warp_same[warp] = same;
     __syncthreads();
     const uint32_t m = warp_more[lane], e = warp_same[lane];  // kSelect / 32 is 32
@@ -463,6 +472,7 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(EvictArgs a) {
     const unsigned below = (1u << lane) - 1;
 #pragma unroll
     for (int j = 0; j < kKeep; ++j) {
+      if (j >= keep) break;
       const bool in = at(t, j) < i1, heavy = in && u[j] > prefix, even = in && u[j] == prefix;
       const unsigned bm = __ballot_sync(~0u, heavy), be = __ballot_sync(~0u, even);
       const uint32_t em = pm + __popc(bm & below), es = ps + __popc(be & below);
@@ -488,12 +498,13 @@ __global__ void __launch_bounds__(kThreads) evict_move_kernel(EvictArgs a) {
   uint4* to = reinterpret_cast<uint4*>(kv ? t.codes[1] : t.codes[0]) + (size_t)zh * t.C * (D / 32) + part;
   const uint32_t* from_param = (kv ? f.param[1] : f.param[0]) + (size_t)zh * f.C;
   uint32_t* to_param = (kv ? t.param[1] : t.param[0]) + (size_t)zh * t.C;
+  wait_for_previous();
   int src[kMove];
   uint4 x[kMove];
   uint32_t p[kMove];
   float w[kMove];
 #pragma unroll
-  for (int k = 0; k < kMove; ++k) src[k] = i0 + k * G < a.budget ? __ldg(a.kept + (size_t)zh * a.budget + i0 + k * G) : -1;
+  for (int k = 0; k < kMove; ++k) src[k] = i0 + k * G < a.budget ? a.kept[(size_t)zh * a.budget + i0 + k * G] : -1;
 #pragma unroll
   for (int k = 0; k < kMove; ++k)
     if (src[k] >= 0) {
@@ -690,10 +701,11 @@ extern "C" int qflash_kv4_evict(const qflash_kv4_cache* from, const qflash_kv4_c
       b.from.param[i] += h0 * from->capacity, b.to.param[i] += h0 * to->capacity;
     }
     b.from.weight += h0 * from->capacity, b.to.weight += h0 * to->capacity, b.kept += h0 * budget;
-    if (from->D == 64)
-      evict_move_kernel<64><<<dim3(nx, (unsigned)n), kThreads, 0, s>>>(b);
+    const dim3 grid(nx, (unsigned)n);
+    if (h0)  // behind another part of itself
+      from->D == 64 ? evict_move_kernel<64><<<grid, kThreads, 0, s>>>(b) : evict_move_kernel<128><<<grid, kThreads, 0, s>>>(b);
     else
-      evict_move_kernel<128><<<dim3(nx, (unsigned)n), kThreads, 0, s>>>(b);
+      launch_behind(from->D == 64 ? evict_move_kernel<64> : evict_move_kernel<128>, grid, kThreads, s, b);
     if (int rc = check_launch("kv4 evict move", nx)) return rc;
   }
   return QFLASH_OK;

@@ -87,9 +87,9 @@ __device__ __forceinline__ void store8(T* p, bool vec, const float (&x)[8]) {
 __device__ __forceinline__ void may_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 template <class A>
-inline void launch_behind(void (*kernel)(A), unsigned grid, unsigned threads, cudaStream_t s, const A& args) {
+inline void launch_behind(void (*kernel)(A), dim3 grid, unsigned threads, cudaStream_t s, const A& args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid), cfg.blockDim = dim3(threads), cfg.stream = s;
+  cfg.gridDim = grid, cfg.blockDim = dim3(threads), cfg.stream = s;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
