@@ -55,6 +55,7 @@ struct RowsArgs {
   int row_tiles;  // ceil(rows / (8 NT))
   int grid;       // CTAs of the first kernel
   uint32_t magic_k, magic_v;
+  bool single;    // a CTA per unit, no second kernel
   bool vec_q;     // query rows start on 16-byte boundaries
   int score_rows; // rows rounded up to even: the score buffer's row length
   float* parts;   // [grid][2][8 NT (D + 2)]: m, l, O of a piece
@@ -156,6 +157,39 @@ __device__ __forceinline__ int sequence_of(const RowsArgs& p, long long at, long
   }
   *first = base;
   return p.a.c.Z;
+}
+
+// What both give for the place a CTA's run begins at, lengths loaded once where
+// one warp holds them all.  `place_of`: the run's beginning from the total.
+struct Place {
+  long long total, at, first;  // first: where sequence z begins
+  int z, grid;
+};
+__device__ __forceinline__ Place begin_of(const RowsArgs& p, int cta) {
+  Place r;
+  const int lane = threadIdx.x & 31;
+  if (p.a.c.Z > 32) {
+    long long before;
+    cost_before(p, 0, &before, &r.total);
+    r.grid = (int)min((long long)p.grid, r.total);
+    r.at = r.grid ? r.total * min(cta, r.grid) / r.grid : 0;
+    r.z = cta < r.grid ? sequence_of(p, r.at, &r.first) : p.a.c.Z;
+    return r;
+  }
+  const long long mine = lane < p.a.c.Z ? (long long)cost_of(span_of(p.a, lane).most(p.a)) * p.a.c.H * p.row_tiles : 0;
+  long long sum = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long up = __shfl_up_sync(~0u, sum, o);
+    if (lane >= o) sum += up;
+  }
+  r.total = __shfl_sync(~0u, sum, 31);
+  r.grid = (int)min((long long)p.grid, r.total);  // no CTA's run is empty
+  r.at = r.grid ? r.total * min(cta, r.grid) / r.grid : 0;
+  const unsigned hit = __ballot_sync(~0u, r.at >= sum - mine && r.at < sum);
+  r.z = hit ? __ffs(hit) - 1 : p.a.c.Z;
+  r.first = __shfl_sync(~0u, sum - mine, r.z & 31);
+  return r;
 }
 
 __device__ __forceinline__ long long run_start(long long total, int grid, int cta) { return total * cta / grid; }
@@ -402,19 +436,39 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
   const AttendArgs& a = p.a;
   const Cache& c = a.c;
   may_begin();
-  long long before, total;
-  cost_before(p, 0, &before, &total);
-  const int grid = (int)min((long long)p.grid, total);  // no CTA's run is empty
-  if ((int)blockIdx.x >= grid) return;
-  long long at = run_start(total, grid, blockIdx.x);
-  const long long stop = run_start(total, grid, blockIdx.x + 1);
-  long long zfirst;
-  int z = sequence_of(p, at, &zfirst);
-  if (z >= c.Z) return;  // only if lens changed meanwhile
+  long long at, stop, zfirst;
+  int z;
+  if (p.single) {  // one unit, whole
+    z = blockIdx.x / (c.H * p.row_tiles);
+    zfirst = 0;
+  } else {
+    const Place me = begin_of(p, blockIdx.x);
+    if ((int)blockIdx.x >= me.grid || me.z >= c.Z) return;  // the latter only if lens changed meanwhile
+    at = me.at, zfirst = me.first, z = me.z;
+    stop = run_start(me.total, me.grid, blockIdx.x + 1);
+  }
   Span sp = span_of(a, z);
   int most = sp.most(a);
   int piece = 0;  // the first piece of a CTA goes to slot 0, a later cut one (its last) to slot 1
   const int units = c.H * p.row_tiles;
+  if (p.single) {
+    const int cost = cost_of(most);
+    at = (long long)(blockIdx.x % units) * cost, stop = at + cost;
+    if (most <= 0) {  // nothing to see
+      const int row0 = (int)(blockIdx.x % p.row_tiles) * R, h = (int)(blockIdx.x % units) / p.row_tiles;
+      for (int e = tid; e < R * D; e += kWarps * 32) {
+        const int row = row0 + e / D;
+        if (row >= p.rows) break;
+        const size_t to = z * a.os[0] + (h * a.rep + row % a.rep) * a.os[1] + (a.tok0 + row / a.rep) * a.os[2] + e % D;
+        ((uint16_t*)a.out)[to] = 0;
+      }
+      if (p.scores) {
+        const size_t head = (size_t)z * c.H + h;
+        for (int j = tid; j < sp.len; j += kWarps * 32) c.weight[head * c.C + j] = a.weights_in[head * c.C + j];
+      }
+      return;
+    }
+  }
   while (at < stop) {
     long long in_z = at - zfirst;
     while (most <= 0 || in_z >= (long long)units * cost_of(most)) {  // on to the next sequence that shows anything
@@ -546,7 +600,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
           else
             ((__nv_bfloat16*)a.out)[to + i] = __float2bfloat16_rn(y[i]);
         }
-        if (d == 0 && p.scores) p.stats[(head * p.row_tiles + unit % p.row_tiles) * R + r] = make_float2(mm, ll);
+        if (d == 0 && p.scores && !p.single) p.stats[(head * p.row_tiles + unit % p.row_tiles) * R + r] = make_float2(mm, ll);
       } else {
         *reinterpret_cast<float4*>(part + 2 * R + r * D + d) = oo;
         if (d == 0) part[r] = mm, part[R + r] = ll;
@@ -554,6 +608,28 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
     }
     __syncthreads();
     ++piece;
+    if (p.single && p.scores) {  // weights of a head that is this CTA's alone: its scores are behind the barriers above
+      if (tid < R) {
+        float mm = sm[0][tid], ll = 0.f;
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) mm = fmaxf(mm, sm[w][tid]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) ll += sl[w][tid] * (sm[w][tid] == -INFINITY ? 1.f : ex2(sm[w][tid] - mm));
+        const int tok = a.tok0 + tid / a.rep;
+        const bool seen = tid < p.rows && sp.limit(a, tok) > 0;
+        so[0][tid][0] = mm == -INFINITY ? 0.f : mm, so[0][tid][1] = seen ? 1.f / ll : 0.f;
+        so[0][tid][2] = __int_as_float(seen ? sp.limit(a, tok) : 0);
+      }
+      __syncthreads();
+      const float* s = p.scores + head * c.C * p.score_rows;
+      for (int j = tid; j < sp.len; j += kWarps * 32) {
+        float add = 0.f;
+        if (j < most)
+          for (int row = 0; row < p.rows; ++row)
+            if (j < __float_as_int(so[0][row][2])) add += ex2(s[(size_t)j * p.score_rows + row] - so[0][row][0]) * so[0][row][1];
+        c.weight[head * c.C + j] = a.weights_in[head * c.C + j] + add;
+      }
+    }
   }
 }
 
@@ -762,8 +838,18 @@ static int launch_rows(RowsArgs r, int dev, cudaStream_t s) {
       return set_err(QFLASH_ERR_LAUNCH, "kv4 rows: occupancy: %s", cudaGetErrorString(cudaGetLastError()));
     per_sm.store(n);
   }
-  const long long tiles = (long long)c.Z * c.H * r.row_tiles * ((c.C + kTile - 1) / kTile);
-  r.grid = (int)std::min<long long>(std::min<long long>((long long)sm_count(dev) * per_sm.load(), kGridMax), tiles);
+  const long long units = (long long)c.Z * c.H * r.row_tiles, tiles = (c.C + kTile - 1) / kTile;
+  // Short caches: a unit to a CTA, since joining costs a kernel; with longer ones, or few units that have their
+  // weights to add up, SMs would idle for too long.  One kernel and two, us at rep 4: 8 heads of 333 positions
+  // 5.2 and 8.1, of 1024 10.2 and 9.0 (which the launch saved makes up for), with weights 14.8 and 10.6; 128 heads of
+  // 1024 10.9 and 17.8, 512 heads 22.6 and 38.5; 8 heads of 2048 16.9 and 10.3.
+  r.single = (tiles <= (r.scores && units < 64 ? 4 : 8) || (units >= 256 && tiles <= 16)) && (!r.scores || r.row_tiles == 1);
+  if (r.single) {
+    r.grid = (int)units;
+    rows_kernel<D, NT, FP16><<<r.grid, kWarps * 32, smem, s>>>(r);
+    return check_launch("kv4 rows", r.grid);
+  }
+  r.grid = (int)std::min<long long>(std::min<long long>((long long)sm_count(dev) * per_sm.load(), kGridMax), units * tiles);
   rows_kernel<D, NT, FP16><<<r.grid, kWarps * 32, smem, s>>>(r);
   if (int rc = check_launch("kv4 rows", r.grid)) return rc;
   const unsigned grid = (unsigned)(c.Z * c.H) * (r.rows + (r.scores ? (c.C + kChunk - 1) / kChunk : 0));
