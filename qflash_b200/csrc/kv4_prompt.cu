@@ -14,10 +14,11 @@
 //     softmax.
 // P vs goes to the tensor cores as bf16 for bf16 queries, as the sum of two bf16
 // terms for fp16 queries (half steps 2^-8 and 2^-16).  A tile's P is formed against
-// the maximum of the tiles before it, in one pass that takes 32 columns at a time
-// and overwrites them: P of any size costs no bits in floating point.  The new
-// maximum counts from the next tile on, if it is larger by 8 (in log2) or more; only a
-// score that is larger by 64 stops the pass, and what the tile has so far is scaled.
+// a reference from the tiles before it (at first the first tile's maximum), in one
+// pass that takes 32 columns at a time and overwrites them: P of any size costs no
+// bits in floating point.  Where a tile's P add up to more than 2^16 the reference is
+// raised for the next; only sums above 2^64 stop the pass, and what the tile has so
+// far is scaled.
 // The order of d within each 8 is 0 4 1 5 2 6 3 7 everywhere (codes d and d + 4
 // of a word come out of one mask): Q is stored so, and the epilogue undoes it.
 //
@@ -386,8 +387,8 @@ struct Layout {
   static constexpr uint32_t BYTES = BARS + 256 + 1024;  // with room to align the base
 };
 
-// A row of the softmax, held by one thread: maximum (log2), sum, and what O has
-// yet to be multiplied by.
+// A row of the softmax, held by one thread: the reference of its exponentials
+// (log2), their sum, and what O has yet to be multiplied by.
 struct RowState {
   float m, l, late;
 };
@@ -405,81 +406,99 @@ __device__ __forceinline__ void scale_out(uint32_t o_at, float f) {
   }
 }
 
+// 32 scores against a row's reference; those from `lim` on (of the tile's 128) masked.
+template <bool FULL>
+__device__ __forceinline__ void differences(uint32_t s_at, const float4* ks, int q, int lim, float neg, float (&x)[32]) {
+  tmem_begin32(s_at + 32 * q, x);
+  tmem_arrived(x);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float4 f = ks[8 * q + i];
+    fma2(x[4 * i], x[4 * i + 1], f.x, f.y, neg, neg);
+    fma2(x[4 * i + 2], x[4 * i + 3], f.z, f.w, neg, neg);
+  }
+  if (!FULL) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (32 * q + i >= lim) x[i] = -INFINITY;
+  }
+}
+__device__ __forceinline__ float largest(const float (&x)[32]) {
+  float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) a[i / 2 & 3] = max3(a[i / 2 & 3], x[i], x[i + 1]);
+  return fmaxf(max3(a[0], a[1], a[2]), a[3]);
+}
+// The first tile's own maximum is the reference to begin with.
+__device__ __noinline__ float first_reference(uint32_t s_at, const float4* ks, int lim) {
+  float m = -INFINITY;
+#pragma unroll 1
+  for (int q = 0; q < 4; ++q) {
+    float x[32];
+    differences<false>(s_at, ks, q, lim, 0.f, x);
+    m = fmaxf(m, largest(x));
+  }
+  return m;
+}
+// Raises the reference of rows for which chunk q is `high` to the chunk's maximum,
+// by a whole number (or from nothing to the first score), and scales O and the P of
+// this tile's chunks before q.  Returns the reference and what the sums are to be
+// multiplied by.  Out of line, as its registers would burden every tile's loop.
+template <int D, bool FP16>
+__device__ __noinline__ float2 raise_reference(float m, uint32_t s_at, uint32_t o_at, const float4* ks, int q, int lim,
+                                               bool high, bool first) {
+  float x[32];
+  differences<false>(s_at, ks, q, lim, m == -INFINITY ? 0.f : -m, x);
+  const float top = largest(x);
+  const bool up = high && top > (m == -INFINITY ? -INFINITY : 0.f);
+  const float by = !up ? 0.f : m == -INFINITY ? top : ceilf(top);
+  const float f = !up ? 1.f : m == -INFINITY ? 0.f : ex2(-by);
+  m = !up ? m : m == -INFINITY ? top : m + by;
+  if (!first) scale_out<D>(o_at, f);
+  tmem_wait_st();
+  const uint32_t ff = pack_bf16(f, f);
+#pragma unroll 1
+  for (int e = 0; e < (FP16 ? 2 : 1) * q; ++e) {
+    uint32_t y[16];
+    const uint32_t at = FP16 ? s_at + 16 * e : s_at + 32 * e;
+    tmem_ld16(at, y);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) asm("mul.bf16x2 %0, %0, %1;" : "+r"(y[i]) : "r"(ff));
+    tmem_st16(at, y);
+  }
+  return make_float2(m, f);
+}
+
 // One tile of 128 scores of a row: P over the scores.  FULL: the row sees all of
 // them, else the first `lim`.  All steps are written over many independent
 // elements: a warp's latencies, not its instructions, are what it waits for.
+// For the same reason no maximum stands before the exponentials: their sum says
+// afterwards, before P is stored, whether the reference is still good enough, and
+// what it has to become.
 template <int D, bool FP16, bool FULL>
 __device__ __forceinline__ void softmax_tile(RowState& r, uint32_t s_at, uint32_t o_at, const float4* ks, const float4* vs,
                                              int lim, bool first) {
-  // 32 scores against the row's maximum, and the largest difference
-  auto differences = [&](int q, float (&x)[32], float neg) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float4 f = ks[8 * q + i];
-      fma2(x[4 * i], x[4 * i + 1], f.x, f.y, neg, neg);
-      fma2(x[4 * i + 2], x[4 * i + 3], f.z, f.w, neg, neg);
-    }
-    if (!FULL) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (32 * q + i >= lim) x[i] = -INFINITY;
-    }
-    float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-    for (int i = 0; i < 32; i += 2) a[i / 2 & 3] = max3(a[i / 2 & 3], x[i], x[i + 1]);
-    return fmaxf(max3(a[0], a[1], a[2]), a[3]);
-  };
-  if (first) {  // nothing before it: its own maximum
-#pragma unroll 1
-    for (int q = 0; q < 4; ++q) {
-      float x[32];
-      tmem_begin32(s_at + 32 * q, x);
-      tmem_arrived(x);
-      r.m = fmaxf(r.m, differences(q, x, 0.f));
-    }
+  if (first) {
+    r.m = first_reference(s_at, ks, lim);
   } else if (__any_sync(~0u, r.late != 1.f)) {
     scale_out<D>(o_at, r.late);
     r.late = 1.f;
   }
-  float mx = -INFINITY, ls[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  float neg = r.m == -INFINITY ? 0.f : -r.m, top;
+  float total = 0.f;
+  bool raised = false;
 #pragma unroll 1
   for (int q = 0; q < 4; ++q) {
     float x[32];
-    tmem_begin32(s_at + 32 * q, x);
-    tmem_arrived(x);
-    top = differences(q, x, neg);
-    mx = fmaxf(mx, top);
-    const bool high = top > (r.m == -INFINITY ? -INFINITY : 64.f);
-    if (__any_sync(~0u, high)) {
-      // up by a whole number, or from nothing to the first score
-      const float by = !high ? 0.f : r.m == -INFINITY ? top : ceilf(top);
-      const float f = !high ? 1.f : r.m == -INFINITY ? 0.f : ex2(-by);
-      r.m = !high ? r.m : r.m == -INFINITY ? top : r.m + by;
-      neg = r.m == -INFINITY ? 0.f : -r.m;
-      mx -= by;
-      r.l *= f;
-      if (!first) scale_out<D>(o_at, f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ls[i] *= f;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) x[i] -= by;
-      tmem_wait_st();
-      const uint32_t ff = pack_bf16(f, f);
-#pragma unroll 1
-      for (int e = 0; e < (FP16 ? 2 : 1) * q; ++e) {
-        uint32_t y[16];
-        const uint32_t at = FP16 ? s_at + 16 * e : s_at + 32 * e;
-        tmem_ld16(at, y);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) asm("mul.bf16x2 %0, %0, %1;" : "+r"(y[i]) : "r"(ff));
-        tmem_st16(at, y);
-      }
-    }
+    differences<FULL>(s_at, ks, q, lim, r.m == -INFINITY ? 0.f : -r.m, x);
 #pragma unroll
     for (int i = 0; i < 32; ++i) x[i] = ex2(x[i]);
+    float c[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) add2(ls[i & 6], ls[(i & 6) + 1], x[i], x[i + 1]);
+    for (int i = 0; i < 32; i += 2) add2(c[i & 6], c[(i & 6) + 1], x[i], x[i + 1]);
+    add2(c[0], c[1], c[2], c[3]);
+    add2(c[4], c[5], c[6], c[7]);
+    add2(c[0], c[1], c[4], c[5]);
+    const float sum = c[0] + c[1];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float4 f = vs[8 * q + i];
@@ -491,23 +510,37 @@ __device__ __forceinline__ void softmax_tile(RowState& r, uint32_t s_at, uint32_
       for (int i = 0; i < 32; ++i)
         if (32 * q + i >= lim) x[i] = 0.f;
     }
-    uint32_t y[16];
+    uint32_t hi[16], lo[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) y[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
-    tmem_st16(s_at + 32 * q, y);
+    for (int i = 0; i < 16; ++i) hi[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
     if (FP16) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        add2(x[2 * i], x[2 * i + 1], -__uint_as_float(y[i] << 16), -__uint_as_float(y[i] & 0xffff0000u));
-        y[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+        add2(x[2 * i], x[2 * i + 1], -__uint_as_float(hi[i] << 16), -__uint_as_float(hi[i] & 0xffff0000u));
+        lo[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
       }
-      tmem_st16(s_at + 32 * q + 16, y);
     }
+    // Too large to go on with (or, for a row without a score above -inf so far, not to be judged by the sum):
+    // the chunk again, against a higher reference.  Asked only here, so that nothing above waits for the answer.
+    const bool high = !raised && (sum > 1.8446744e19f || (r.m == -INFINITY && lim > 32 * q));  // 2^64
+    if (__any_sync(~0u, high)) {
+      const float2 up = raise_reference<D, FP16>(r.m, s_at, o_at, ks, q, lim, high, first);
+      r.m = up.x;
+      r.l *= up.y, total *= up.y;
+      raised = true;
+      --q;
+      continue;
+    }
+    raised = false;
+    total += sum;
+    tmem_st16(s_at + 32 * q, hi);
+    if (FP16) tmem_st16(s_at + 32 * q + 16, lo);
   }
-  r.l += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
+  r.l += total;
   tmem_wait_st();
-  if (mx > 8.f) {
-    const float by = ceilf(mx), f = ex2(-by);
+  // The tile's sum is its largest P up to a factor of 128: a reference raised to it leaves that 2^-7 at least.
+  if (total > 65536.f && total < INFINITY) {
+    const float by = (float)((int)(__float_as_uint(total) >> 23) - 127), f = ex2(-by);
     r.m += by;
     r.l *= f, r.late *= f;
   }
@@ -576,7 +609,7 @@ __global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
 
   if (warp < 8) {
     // ---------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
     const int t = warp >> 2, lrow = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
@@ -691,7 +724,7 @@ __global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
     }
   } else {
     // ---------------------------------------------------------------- products
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     if (warp == 12) {
       constexpr uint32_t IS = idesc_f16(kKeys, !FP16, false), IO = idesc_f16(D, true, true);
       const uint32_t q_word = k_word(base + L::Q), kk_word = k_word(base + L::K), v_word = mn_word(base + L::V);
