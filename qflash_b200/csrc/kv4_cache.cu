@@ -321,27 +321,6 @@ constexpr int kKeep = 16;  // positions per thread and tile
 constexpr int kDigits = 2048;
 constexpr int kCluster = 8;
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// CTA `rank`'s copy of a word of shared memory
-__device__ __forceinline__ uint32_t peer_word(const uint32_t* p, uint32_t rank) {
-  uint32_t at, v;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at));
-  return v;
-}
-
 // A word of CTA `rank` of the cluster, or of this one if it is alone.
 __device__ __forceinline__ uint32_t word_of(const uint32_t* p, int rank, int cs) { return cs > 1 ? peer_word(p, rank) : *p; }
 

@@ -81,6 +81,27 @@ __device__ __forceinline__ void store8(T* p, bool vec, const float (&x)[8]) {
   }
 }
 
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// CTA `rank`'s copy of a word of shared memory
+__device__ __forceinline__ uint32_t peer_word(const uint32_t* p, uint32_t rank) {
+  uint32_t at, v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at));
+  return v;
+}
+
 // A kernel that begins while the one before it in the stream still runs: what it does before
 // wait_for_previous may read nothing that one writes.  The one before says may_begin
 // once all its CTAs are resident, so the second kernel's blocks take no place from it.

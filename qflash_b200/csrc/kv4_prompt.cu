@@ -27,8 +27,8 @@
 // joined by a second kernel.
 //
 // The attention weights need the rows' final maximum and sum, so a third kernel
-// forms S^T = K Q^T again, a thread a key, and adds up exp(S - m) / l along its
-// row of columns: no sum crosses threads, and no atomics.
+// forms S^T = K Q^T again, keys in rows, and adds up exp(S - m) / l along its
+// columns in a fixed order: no atomics.
 #include <algorithm>
 #include <atomic>
 
@@ -883,12 +883,13 @@ struct WLayout {
   static constexpr uint32_t BYTES = BARS + 128 + 1024;
 };
 
-// One CTA per 128 positions of a head: warps 0-7 add up (two threads a position,
-// for 64 columns of a tile each), warps 8-11 bring query tiles, warp 12 issues the
-// products.  What bounds it is exponentials, and with one thread a position the
+// Two CTAs (a cluster) per 128 positions of a head, with every other row tile each,
+// as the first positions of a prompt are seen by all its rows, one tile after
+// the other.  Warps 0-7 add up (two threads a position, for 64 columns of a tile
+// each), warps 8-11 bring query tiles, warp 12 issues the products.  What bounds it is exponentials, and with one thread a position the
 // latencies of 4 warps.
 template <int D, bool FP16>
-__global__ void __launch_bounds__(kWeigh, 2) prompt_weights_kernel(PromptArgs p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeigh, 2) prompt_weights_kernel(PromptArgs p) {
   using L = WLayout<D>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u;
@@ -897,18 +898,20 @@ __global__ void __launch_bounds__(kWeigh, 2) prompt_weights_kernel(PromptArgs p)
   const AttendArgs& a = p.a;
   const Cache& c = a.c;
   // the first positions first: with a causal limit most rows see them
-  const int heads = c.Z * c.H, zh = blockIdx.x % heads, key0 = blockIdx.x / heads * kKeys, z = zh / c.H, h = zh % c.H;
+  const int rank = (int)cluster_rank(), unit = blockIdx.x / 2;
+  const int heads = c.Z * c.H, zh = unit % heads, key0 = unit / heads * kKeys, z = zh / c.H, h = zh % c.H;
   const Span sp = span_of(a, z);
-  if (key0 >= sp.len) return;
+  if (key0 >= sp.len) return;  // both CTAs together, here and below
   // rows that see position key0: from token `first` on
   const int first = a.causal ? max(0, key0 - (sp.len - sp.fresh)) : 0;
   const int rt0 = first < sp.fresh ? first * a.rep / kM : 0, rt1 = first < sp.fresh ? (sp.fresh * a.rep + kM - 1) / kM : 0;
   const size_t head = (size_t)zh * c.C;
   if (rt0 >= rt1) {
     const int key = key0 + tid;
-    if (tid < kKeys && key < sp.len) c.weight[head + key] = a.weights_in[head + key];
+    if (rank == 0 && tid < kKeys && key < sp.len) c.weight[head + key] = a.weights_in[head + key];
     return;
   }
+  const int tiles = max(0, (rt1 - rt0 - rank + 1) / 2);  // this CTA's: rt0 + rank, and every second from there on
   const uint32_t bars = base + L::BARS;
   auto q_full = [&](int i) { return bars + 8 * i; };
   auto q_empty = [&](int i) { return bars + 24 + 8 * i; };
@@ -957,8 +960,8 @@ __global__ void __launch_bounds__(kWeigh, 2) prompt_weights_kernel(PromptArgs p)
       warp_arrive(k_full);
     }
     const uint32_t s_at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 64 * half;
-    for (int rt = rt0; rt < rt1; ++rt) {
-      const int g = rt - rt0, b = g & 1, qb = g % L::COUNT;
+    for (int g = 0; g < tiles; ++g) {
+      const int rt = rt0 + rank + 2 * g, b = g & 1, qb = g % L::COUNT;
       if (!wait(s_full(b), g >> 1 & 1) || !wait(q_full(qb), g / L::COUNT & 1)) goto out;
       tc_fence_after();
       const float4* cm = reinterpret_cast<const float4*>(col + qb * 384) + 16 * half;
@@ -1009,9 +1012,9 @@ __global__ void __launch_bounds__(kWeigh, 2) prompt_weights_kernel(PromptArgs p)
     const int r = tid - 256;
     const uint16_t* const q0 = (const uint16_t*)a.q;
     constexpr int kLag = L::COUNT - 2;  // tiles whose copies are still under way when the next are begun
-    for (int rt = rt0; rt < rt1 + kLag; ++rt) {
-      const int g = rt - rt0, b = g % L::COUNT, row = rt * kM + r, tok = row / a.rep;
-      if (rt < rt1) {
+    for (int g = 0; g < tiles + kLag; ++g) {
+      const int b = g % L::COUNT, row = (rt0 + rank + 2 * g) * kM + r, tok = row / a.rep;
+      if (g < tiles) {
         const int limit = row < p.rows && tok < sp.fresh ? sp.limit(a, tok) : 0;
         const float2 st = limit > 0 ? __ldg(p.stats + (size_t)zh * p.rows + row) : make_float2(0.f, 0.f);
         if (!wait(q_empty(b), (g / L::COUNT & 1) ^ 1)) goto out;
@@ -1022,7 +1025,7 @@ __global__ void __launch_bounds__(kWeigh, 2) prompt_weights_kernel(PromptArgs p)
         reinterpret_cast<int*>(col)[b * 384 + 256 + r] = limit;
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
-      if (g >= kLag) {
+      if (g >= kLag && tiles) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
         fence_proxy_async_smem();
         warp_arrive(q_full((g - kLag) % L::COUNT));
@@ -1032,8 +1035,8 @@ __global__ void __launch_bounds__(kWeigh, 2) prompt_weights_kernel(PromptArgs p)
     constexpr uint32_t IS = idesc_f16(kM, !FP16, false);
     const uint32_t kw = k_word(base + L::K), qw = k_word(base + L::Q);
     if (!wait(k_full, 0)) goto out;
-    for (int rt = rt0; rt < rt1; ++rt) {
-      const int g = rt - rt0, b = g & 1, qs = g % L::COUNT;
+    for (int g = 0; g < tiles; ++g) {
+      const int b = g & 1, qs = g % L::COUNT;
       if (!wait(q_full(qs), g / L::COUNT & 1) || !wait(s_empty(b), (g >> 1 & 1) ^ 1)) goto out;
       tc_fence_after();
       const uint32_t kb = uniform(kw), qb = uniform(qw + qs * (L::TILE / 16)), to = uniform(tmem + b * 128);
@@ -1058,7 +1061,12 @@ out:
   __syncthreads();
   tc_fence_after();
   if (warp == 12) tmem_dealloc(tmem, 256);
-  if (tid < kKeys && key < sp.len) c.weight[head + key] = a.weights_in[head + key] + ((sum0 + sum1) + other[tid]);
+  const float sum = (sum0 + sum1) + (tid < kKeys ? other[tid] : 0.f);
+  if (rank == 1 && tid < kKeys) other[tid] = sum;  // each thread's own word
+  cluster_sync();
+  if (rank == 0 && tid < kKeys && key < sp.len)
+    c.weight[head + key] = a.weights_in[head + key] + (sum + __uint_as_float(peer_word(reinterpret_cast<const uint32_t*>(other) + tid, 1)));
+  cluster_sync();  // the second CTA's shared memory stays until it was read
 }
 
 // ------------------------------------------------------------------ host
@@ -1106,7 +1114,7 @@ static int launch_prompt(const PromptArgs& p, int dev, cudaStream_t s) {
   if (int rc = check_launch("kv4 prompt finish", n)) return rc;
   if (!p.stats) return QFLASH_OK;
   if (int rc = allow_smem<prompt_weights_kernel<D, FP16>>(WLayout<D>::BYTES, dev)) return rc;
-  const unsigned nw = (unsigned)(p.a.c.Z * p.a.c.H) * ((p.a.c.C + kKeys - 1) / kKeys);
+  const unsigned nw = 2u * (unsigned)(p.a.c.Z * p.a.c.H) * ((p.a.c.C + kKeys - 1) / kKeys);
   prompt_weights_kernel<D, FP16><<<nw, kWeigh, WLayout<D>::BYTES, s>>>(p);
   return check_launch("kv4 prompt weights", nw);
 }
