@@ -45,7 +45,7 @@ namespace kv4 {
 constexpr int kTile = 128;        // keys per CTA tile: 4 warps of 32
 constexpr int kWarps = 4;
 constexpr int kGridMax = 148 * 5;  // CTAs of one resident wave at most
-constexpr int kRowsMax = 64;      // query rows (tokens x rep) per launch that accumulates weights
+constexpr int kRowsMax = 64;      // query rows (tokens x rep) per launch that accumulates weights (with rep <= 64)
 
 constexpr int kBegin = 2;
 

@@ -700,11 +700,21 @@ static int check_attend(const qflash_kv4_cache* cache, int dtype, int Hq, int N)
   return QFLASH_OK;
 }
 
-// Rows of a head from which the kernel for many rows is used.
-static bool many_rows(const qflash_kv4_cache* c, int Hq, int N) { return (long long)Hq / c->H * N > 64; }
+// Whether the kernel for many rows (R per key/value head) is the faster one.  It begins with
+// some 25 us more (128 decoded positions and 256 rows at a time), the other reads the
+// cache once per 16 rows.  us at head dim 128, this one and the other:
+//   8 heads of 4000 positions   64 rows 38 and 23, 256 rows 45 and 48
+//   64 heads of 4000            32 rows 62 and 48,  64 rows 63 and 85
+//   8 heads of 30000            64 rows 70 and 58, 128 rows 73 and 98
+// With weights the other kernel goes by groups of rows and stores their scores:
+//   8 heads of 4000             24 rows 53 and 32,  64 rows 54 and 106
+static bool many_rows(const qflash_kv4_cache* c, int Hq, int N, bool weights) {
+  const long long rows = (long long)Hq / c->H * N, passes = (rows + 15) / 16, positions = (long long)c->Z * c->H * c->capacity;
+  return weights ? rows > 32 : 2 * passes * positions > 800000 + 5 * positions;
+}
 
 static size_t attend_workspace(const qflash_kv4_cache* c, int Hq, int N, bool weights) {
-  return many_rows(c, Hq, N) ? prompt_workspace(c, Hq, N, weights) : rows_workspace(c, Hq, N, weights);
+  return many_rows(c, Hq, N, weights) ? prompt_workspace(c, Hq, N, weights) : rows_workspace(c, Hq, N, weights);
 }
 
 extern "C" size_t qflash_kv4_attend_workspace(const qflash_kv4_cache* cache, int dtype, int Hq, int N, int weights) {
@@ -736,6 +746,6 @@ extern "C" int qflash_kv4_attend(const qflash_kv4_cache* cache, const void* q, i
   a.scale_log2e = (float)(scale * 1.4426950408889634);
   a.weights_in = weights_in;
   a.tok0 = 0, a.ntok = N;
-  return many_rows(cache, Hq, N) ? attend_prompt(a, dtype == kF16, workspace, dev, (cudaStream_t)stream)
+  return many_rows(cache, Hq, N, weights_in != nullptr) ? attend_prompt(a, dtype == kF16, workspace, dev, (cudaStream_t)stream)
                                  : attend_rows(a, dtype == kF16, workspace, dev, (cudaStream_t)stream);
 }

@@ -605,3 +605,244 @@ def test_two_streams_read_one_cache():
                 g.append(cache.attend(q))
     torch.cuda.synchronize()
     assert all(torch.equal(x, w) for g, w in zip(got, want) for x in g)
+
+
+# ------------------------------------------------------------------ the kernel for many rows
+# (accumulate, or a large cache, leads there; the tests above reach it with accumulate only)
+def both_ways(cache, q, scale=None, causal=True, new_lens=None):
+    """attend with weights, from zeros; the weight buffer behind the stored tokens stays as it was."""
+    w = torch.zeros_like(cache.weight)
+    out = cache.attend(q, scale=scale, causal=causal, new_lens=new_lens, accumulate=True, weights=w)
+    return out, cache.weight
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("Z, H, rep, N, lens, causal", [
+    (2, 8, 4, 70, [4000, 1], True), (3, 8, 3, 129, [2500, 129, 0], True), (1, 16, 16, 33, [3001], False),
+    (5, 4, 1, 300, [4099, 300, 0, 7, 2048], True)])
+def test_many_rows_over_a_large_cache(D, dtype, Z, H, rep, N, lens, causal):
+    C = max(lens) + 1
+    cache = make_cache(Z, H, C, D, lens, seed=N)
+    q = queries(Z, H * rep, N, D, dtype, seed=N)
+    new = [min(N, n) for n in lens]
+    nl = torch.tensor(new, dtype=torch.int32, device="cuda")
+    want, spread, cols, size = attend64(cache, q, new, causal)
+    close_out(cache.attend(q, causal=causal, new_lens=nl), want, spread, size, D, C)
+    out, weight = both_ways(cache, q, causal=causal, new_lens=nl)
+    close_out(out, want, spread, size, D, C)
+    live = (torch.arange(C, device="cuda") < cache.lens[:, None])[:, None, :].expand(Z, H, C)
+    tol = (2 * score_error(size.max(), D) + (rep * N + 4) * 2.0 ** -24) * cols + 1e-30
+    assert (((weight.double() - cols).abs() / tol)[live] <= 1).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("rep, N, lens", [(64, 3, [500, 2]), (7, 37, [260, 259]), (5, 101, [101, 50]), (1, 257, [257, 1000])])
+def test_many_rows_odd_groups(dtype, rep, N, lens):
+    """Row tiles that end inside a token's heads, and sequences shorter than the query tensor."""
+    C = max(lens)
+    cache = make_cache(2, 2, C, 64, lens, seed=rep)
+    q = queries(2, 2 * rep, N, 64, dtype, seed=rep)
+    want, spread, _, size = attend64(cache, q, [N, N], True)
+    out, _ = both_ways(cache, q)
+    close_out(out, want, spread, size, 64, C)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_many_rows_values_of_any_size(dtype):
+    for f in (1e-6, 1e-3, 300.0):
+        cache = make_cache(2, 1, 300, 64, [300, 250])
+        cache.v_param[..., 0] = (cache.v_param[..., 0].float() * f).bfloat16()
+        q = queries(2, 4, 200, 64, dtype, seed=2)
+        want, spread, _, size = attend64(cache, q, [200, 200], True)
+        close_out(both_ways(cache, q)[0], want, spread, size, 64, 300)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("rising", [0, 30, 90, 300])
+def test_many_rows_moving_reference(dtype, rising):
+    """Scores that grow along the keys, by up to some hundred (log2) within a tile: the reference has to follow, before
+    and after P was stored, and what was summed up against the old one must not be lost or overflow."""
+    D, n, N = 64, 700, 120
+    cache = make_cache(1, 1, n, D, [n], garbage=False)
+    q = torch.zeros(1, 2, N, D, dtype=dtype, device="cuda")
+    q[..., 0] = 1.0
+    cache.k_codes.fill_(0)
+    cache.k_codes[0, 0, :, 0] = 1  # element 0 is the key's scale, the others 0
+    ramp = torch.arange(n, device="cuda") / n * rising * math.log(2)
+    jump = torch.where(torch.arange(n, device="cuda") % 64 == 37, 5.0 * (rising > 0), 0.0)
+    cache.k_param[0, 0, :, 0], cache.k_param[0, 0, :, 1] = (ramp + jump).bfloat16(), 0.0
+    want, spread, _, size = attend64(cache, q, [N], True, 1.0)
+    assert 2 * score_error(size.max().item(), D) < 0.125
+    close_out(both_ways(cache, q, scale=1.0)[0], want, spread * 1.1, size, D, n)
+    q[:, 1] = -q[:, 1]  # falling scores: nothing behind the first tile counts
+    want, spread, _, size = attend64(cache, q, [N], True, 1.0)
+    close_out(both_ways(cache, q, scale=1.0)[0], want, spread * 1.1, size, D, n)
+
+
+def test_many_rows_scale_and_sharp_rows():
+    cache = make_cache(2, 2, 400, 128, [400, 211], strength=3.0)
+    for scale in (0.7, 3.0, -0.5, 0.0):
+        q = queries(2, 8, 100, 128, FP16, seed=4)
+        want, spread, _, size = attend64(cache, q, [100, 100], True, scale)
+        assert 2 * score_error(size.max().item(), 128) < 0.125
+        close_out(both_ways(cache, q, scale=scale)[0], want, spread * 1.1, size, 128, 400)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_many_rows_poisoned_token(dtype):
+    cache = make_cache(1, 2, 260, 64, [260])
+    cache.k_param[0, 0, 255, 0] = math.nan
+    cache.v_param[0, 1, 256, 0] = math.nan
+    q = queries(1, 4, 130, 64, dtype, seed=8)
+    out, weight = both_ways(cache, q)
+    seen = torch.arange(130, 260, device="cuda")
+    assert torch.equal(torch.isnan(out[0, 0]).all(-1), seen >= 255) and torch.equal(torch.isnan(out[0, 2]).all(-1), seen >= 256)
+    assert torch.isfinite(out[0, :2, :125]).all() and torch.isfinite(out[0, 2:, :126]).all()
+    # rows that see the poisoned key have no weights to give, so no position that they see has one
+    assert torch.isnan(weight[0, 0]).all() and torch.isfinite(weight[0, 1]).all()
+
+
+def test_many_rows_infinite_queries():
+    D = 64
+    cache = make_cache(1, 1, 140, D, [140])
+    cache.k_codes.fill_(0x88)
+    cache.k_param[..., 0], cache.k_param[..., 1] = 1.0, 7.0
+    cache.k_codes[0, 0, 5] = 0x66
+    q = torch.zeros(1, 2, 100, D, dtype=BF16, device="cuda")
+    q[:, 0] = -math.inf
+    q[:, 1] = math.inf
+    assert torch.isnan(both_ways(cache, q, causal=False)[0]).all()
+
+
+@pytest.mark.parametrize("N", [40, 160])
+def test_many_rows_strides(N):
+    Z, H, rep, D = 2, 2, 3, 64
+    cache = make_cache(Z, H, 333, D, [333, 170])
+    q = queries(Z, H * rep, N, D, BF16, seed=3)
+    want, _ = both_ways(cache, q)
+    buf = torch.full((Z, N + 2, H * rep, D + 16), 7.0, dtype=BF16, device="cuda")
+    view = buf[:, 1:1 + N, :, 8:8 + D].transpose(1, 2)
+    assert torch.equal(cache.attend(q, accumulate=True, out=view), want)
+    buf[:, 1:1 + N, :, 8:8 + D] = 7.0
+    assert (buf == 7).all()
+    odd = torch.empty(Z * N * H * rep * D + 1, dtype=BF16, device="cuda")[1:].view(Z, N, H * rep, D).transpose(1, 2)
+    odd.copy_(q)
+    assert torch.equal(both_ways(cache, odd)[0], want)
+    out = torch.empty(Z * N * H * rep * D + 1, dtype=BF16, device="cuda")[1:].view(Z, N, H * rep, D).transpose(1, 2)
+    assert torch.equal(cache.attend(odd, accumulate=True, out=out), want)
+
+
+def test_many_rows_same_result_every_time_and_side_by_side():
+    cache = make_cache(3, 4, 1500, 128, [1500, 411, 5])
+    qs = [queries(3, 16, n, 128, BF16, seed=n) for n in (150, 90)]
+    want = [cache.attend(q) for q in qs]
+    again = [both_ways(cache, q) for q in qs][1][1].clone()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    got = [[], []]
+    for _ in range(8):
+        for s, q, g in zip(streams, qs, got):
+            with torch.cuda.stream(s):
+                g.append(cache.attend(q))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, w) for g, w in zip(got, want) for x in g)
+    for _ in range(3):
+        assert torch.equal(both_ways(cache, qs[1])[1], again)
+    cache.check()
+
+
+def test_captured_prompt_then_decoding():
+    """A padded prompt with weights, then an eviction, in a graph whose lengths change between replays."""
+    from qflash_b200 import KV4Cache
+    Z, H, rep, D, N = 2, 2, 4, 64, 90
+    g = gen(31)
+    caches = [KV4Cache.empty(Z, H, 500, D) for _ in range(2)]
+    small = [KV4Cache.empty(Z, H, 60, D) for _ in range(2)]
+    k, v = (torch.zeros(Z, H, N, D, dtype=BF16, device="cuda") for _ in range(2))
+    q = torch.zeros(Z, H * rep, N, D, dtype=BF16, device="cuda")
+    new = torch.zeros(Z, dtype=torch.int32, device="cuda")
+
+    def step(i):
+        caches[i].append(k, v, new_lens=new)
+        out = caches[i].attend(q, new_lens=new, accumulate=True)
+        return out, caches[i].evict(50, 10, out=small[i])
+
+    graph, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=s):
+        out, kept = step(0)
+    for counts in ([90, 13], [0, 90], [77, 1], [1, 0]):
+        for t in (k, v, q):
+            t.copy_(torch.randn(t.shape, generator=g, device="cuda"))
+        new.copy_(torch.tensor(counts, dtype=torch.int32))
+        graph.replay()
+        want, want_kept = step(1)
+        assert torch.equal(out, want) and torch.equal(kept, want_kept)
+        assert torch.equal(caches[0].weight, caches[1].weight) and torch.equal(caches[0].lens, caches[1].lens)
+        assert torch.equal(small[0].v_codes, small[1].v_codes)
+
+
+def test_another_current_device_and_thread():
+    """The calls go by the cache's device and restore the caller's; two threads may share the library."""
+    import threading
+    from qflash_b200 import KV4Cache
+    results = {}
+
+    def work(i):
+        c = KV4Cache.empty(1, 1, 200, 64, device="cuda:0")
+        x = torch.randn(1, 1, 150, 64, generator=gen(i), device="cuda").half()
+        c.append(x, x)
+        results[i] = c.attend(x), c.weight
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(4):
+        x = torch.randn(1, 1, 150, 64, generator=gen(i), device="cuda").half()
+        c = KV4Cache.empty(1, 1, 200, 64)
+        c.append(x, x)
+        assert torch.equal(c.attend(x), results[i][0])
+    assert torch.cuda.current_device() == 0
+
+
+def test_lengths_outside_the_cache_read_as_its_ends():
+    cache = make_cache(2, 1, 100, 64, [100, 0], garbage=False)
+    q = queries(2, 2, 1, 64, FP16, seed=1)
+    want = cache.attend(q)
+    cache.lens.copy_(torch.tensor([2 ** 31 - 1, -5], dtype=torch.int32))
+    assert torch.equal(cache.attend(q), want)
+    k, _ = cache.read(100)
+    assert k[0].any() and not k[1].any()
+
+
+def test_positions_behind_2_to_the_31_bytes():
+    """Codes, parameters and weights of the last head lie behind 2^32 bytes of the buffers."""
+    from qflash_b200 import KV4Cache
+    H, C, D = 3, 1 << 24, 128  # 2^30 bytes of codes per head
+    cache = KV4Cache.empty(1, H, C, D)
+    at = torch.tensor([C - 3], dtype=torch.int32, device="cuda")
+    x = torch.randn(1, H, 3, D, generator=gen(1), device="cuda").half()
+    cache.append(x, x.flip(2), at=at)
+    assert cache.lens.item() == C
+    k, v = cache.read(3, start=at, dtype=FP32)
+    for t, got in ((x, k), (x.flip(2), v)):
+        code, p = quantise(t)
+        assert torch.equal(got.double(), p[..., :1].double() * (code.double() - p[..., 1:].double()))
+    # all other positions are zeros with scale 0: scores 0, values 0
+    q = queries(1, H, 1, D, FP16, seed=2) * 40
+    out = cache.attend(q, accumulate=True)
+    s = torch.einsum("hd,hjd->hj", q[0, :, 0].double(), k[0].double()) / D ** 0.5
+    z = torch.exp(s).sum(-1) + (C - 3)
+    want = torch.einsum("hj,hjd->hd", torch.exp(s) / z[:, None], v[0].double())
+    spread = torch.einsum("hj,hjd->hd", torch.exp(s) / z[:, None], v[0].double().abs())
+    # the sums of 2^24 exponentials are added up in 512 parts of 2^15, each by 8 threads: 2^12 steps of 2^-24
+    assert ((out[0, :, 0].double() - want).abs() <= (2.0 ** -11) * spread + 2.0 ** -25).all()
+    assert ((cache.weight[0, :, -3:].double() - torch.exp(s) / z[:, None]).abs() <= 2.0 ** -11 * torch.exp(s) / z[:, None]).all()
+    small = KV4Cache.empty(1, H, 8, D)
+    cache.weight[0, :, 77] = 5.0
+    kept = cache.evict(4, 3, out=small)
+    assert kept.tolist() == [[[77, C - 3, C - 2, C - 1]] * H]
+    assert torch.equal(small.read(4, dtype=FP32)[0][:, :, 1:], k)
