@@ -281,8 +281,10 @@ typedef struct qflash_kv4_cache {
  * Quantises keys and values [Z, H, N, D] (dtype 0 fp32, 1 fp16, 2 bf16; strides in
  * elements, innermost 1) into the cache.  Row i of sequence z goes to position
  * at[z] + i (NULL: lens[z] + i) for i < new_lens[z] (NULL: N; clamped to [0, N]);
- * its weight becomes 0 and lens[z] becomes at[z] + new_lens[z].  Tokens outside
- * [0, capacity) are dropped, lens stops at capacity, and bit 0 of ctl[1] is set.
+ * its weight becomes 0 and lens[z] becomes at[z] + new_lens[z] (also where that is
+ * less than before, and with N = 0: tokens are taken back; positions that an `at`
+ * behind lens skips keep what they hold).  Tokens outside [0, capacity) are dropped,
+ * lens stops at its ends, and bit 0 of ctl[1] is set.
  *   lo = min(x, 0), hi = max(x, 0), scale = bf16(fp32((hi - lo) / 15)),
  *   zero = clamp(rint(-lo / scale), 0, 15), code = clamp(rint(x / scale) + zero, 0, 15)
  * with fp32 quotients.  A vector with an infinity or a NaN gets scale NaN.
@@ -305,7 +307,7 @@ int qflash_kv4_read(const qflash_kv4_cache* cache, void* k, void* v, int dtype, 
  * i < new_lens[z] (NULL: N) are the sequence's last tokens: with `causal`, row i sees
  * the positions up to lens[z] - new_lens[z] + i, else all lens[z].  Rows that see
  * nothing, and rows i >= new_lens[z], are written as zeros.
- * With weights_in ([Z, H, capacity] fp32; it may be cache->weight), cache->weight of
+ * With weights_in ([Z, H, capacity] fp32; cache->weight itself, or apart from it), cache->weight of
  * every stored position j becomes weights_in[j] + the sum over rows and query heads
  * of the probability that position j received.
  * `workspace` holds qflash_kv4_attend_workspace(...) bytes, 16-byte aligned, for this

@@ -11,8 +11,10 @@ the reference, whose ``qflash.forward`` attends over floats in one call).
 Every vector is held as codes 0..15, a bfloat16 scale and a zero point
 (``scale * (code - zero)``); include/qflash_b200.h states the layout and the
 rounding.  Sequences of a batch have lengths of their own (``lens``, on the
-device); no call synchronises with the host, and all can be captured into CUDA
-graphs.  Gradients are not computed.
+device); no call but ``check`` synchronises with the host, and all others can be
+captured into CUDA graphs.  Calls that write a cache (``append``, ``attend`` with
+``accumulate``, ``evict`` into it) must be ordered with all others on it, by one
+stream or by events; others may run side by side.  Gradients are not computed.
 """
 from __future__ import annotations
 
@@ -24,6 +26,7 @@ from torch import Tensor
 from . import _lib
 
 HEAD_DIMS = (64, 128)
+MAX_CAPACITY, MAX_HEADS = 1 << 24, 1 << 20
 
 
 class KV4Cache:
@@ -32,14 +35,18 @@ class KV4Cache:
     bfloat16 [Z, H, C, 2] (scale, zero point), ``weight`` float32 [Z, H, C] and
     ``lens`` int32 [Z], all contiguous CUDA tensors on one device."""
 
-    __slots__ = ("k_codes", "v_codes", "k_param", "v_param", "weight", "lens", "_ctl", "_c", "_ref",
-                 "_index", "_workspace", "_scale", "shape", "device")
+    __slots__ = ("_buffers", "_ctl", "_c", "_ref", "_index", "_workspace", "_scale", "shape", "device")
+    # the calls go by the buffers' addresses, so the tensors can be written but not replaced
+    k_codes, v_codes, k_param, v_param, weight, lens = (property(lambda self, i=i: self._buffers[i]) for i in range(6))
 
     def __init__(self, k_codes: Tensor, v_codes: Tensor, k_param: Tensor, v_param: Tensor, weight: Tensor,
                  lens: Tensor):
         if k_codes.dim() != 4:
             raise ValueError(f"k_codes must be [Z, H, C, D / 2], got {tuple(k_codes.shape)}")
         Z, H, C, half = k_codes.shape
+        if not (H >= 1 and 1 <= C <= MAX_CAPACITY and Z * H <= MAX_HEADS):
+            raise ValueError(f"at least one head and position, at most {MAX_CAPACITY} positions and {MAX_HEADS} heads "
+                             f"in all: got Z, H, C = {Z}, {H}, {C}")
         if 2 * half not in HEAD_DIMS:
             raise ValueError(f"head dim {2 * half} not in {HEAD_DIMS}")
         buffers = (("k_codes", k_codes, (Z, H, C, half), torch.uint8), ("v_codes", v_codes, (Z, H, C, half), torch.uint8),
@@ -52,8 +59,9 @@ class KV4Cache:
         for name, t, _, _ in buffers:
             if not t.is_cuda or t.device != k_codes.device:
                 raise ValueError(f"{name} must be on the CUDA device of k_codes, got {t.device}")
-        self.k_codes, self.v_codes, self.k_param, self.v_param = k_codes, v_codes, k_param, v_param
-        self.weight, self.lens = weight, lens
+        self._buffers = (k_codes, v_codes, k_param, v_param, weight, lens)
+        if Z and len({t.data_ptr() for t in self._buffers}) < 6:
+            raise ValueError("the buffers must be six different ones")
         self._ctl = torch.zeros(2, dtype=torch.int32, device=k_codes.device)
         self.shape, self.device = (Z, H, C, 2 * half), k_codes.device
         self._c = _lib.KV4CacheStruct(*(t.data_ptr() for t in (k_codes, v_codes, k_param, v_param, weight, lens,
@@ -78,8 +86,8 @@ class KV4Cache:
         tokens.  ``new_lens`` int32 [Z]: how many of the N rows each sequence
         brings (default all).  ``at`` int32 [Z]: where its first one goes
         (default ``lens``); ``lens`` becomes ``at + new_lens``, so an ``at``
-        below ``lens`` takes tokens back.  Tokens past the capacity are
-        dropped, which ``check`` reports."""
+        below ``lens`` takes tokens back (with N = 0 nothing else).  Tokens
+        past the capacity are dropped, which ``check`` reports."""
         Z, H, _, D = self.shape
         if key.dim() != 4 or key.shape != value.shape or key.shape[:2] != (Z, H) or key.shape[3] != D:
             raise ValueError(f"key and value must be [{Z}, {H}, N, {D}], got {tuple(key.shape)}, {tuple(value.shape)}")
@@ -104,7 +112,7 @@ class KV4Cache:
         ``weights`` (float32 [Z, H, C], default ``weight`` itself) plus the
         probabilities that the position received, over rows and the heads of
         its group.  ``out``: the output tensor (any strides over a contiguous
-        head dim, not sharing elements with the query)."""
+        head dim, each element once, none of them the query's)."""
         Z, H, C, D = self.shape
         if query.dim() != 4 or query.shape[0] != Z or query.shape[3] != D or query.shape[1] % H or not query.shape[1]:
             raise ValueError(f"query must be [{Z}, a multiple of {H}, N, {D}], got {tuple(query.shape)}")
@@ -124,6 +132,8 @@ class KV4Cache:
         elif out.shape != query.shape or out.dtype != query.dtype or out.stride(-1) != 1 or out.device != self.device:
             raise ValueError(f"out must be a {tuple(query.shape)} {query.dtype} tensor on {self.device} with a "
                              "contiguous last dim")
+        elif out.data_ptr() == query.data_ptr() and out.numel() or any(n > 1 and not s for n, s in zip(out.shape, out.stride())):
+            raise ValueError("out must have elements of its own")
         shape = (query.dtype, query.shape[1], query.shape[2], accumulate)
         need = self._workspace.get(shape)
         if need is None:

@@ -45,19 +45,18 @@ namespace kv4 {
 constexpr int kTile = 128;        // keys per CTA tile: 4 warps of 32
 constexpr int kWarps = 4;
 constexpr int kGridMax = 148 * 5;  // CTAs of one resident wave at most
-constexpr int kRowsMax = 64;      // query rows (tokens x rep) per launch that accumulates weights (with rep <= 64)
 
 constexpr int kBegin = 2;
 
 struct RowsArgs {
   AttendArgs a;
-  int rows;       // ntok * rep
+  int rows;       // N * rep
   int row_tiles;  // ceil(rows / (8 NT))
   int grid;       // CTAs of the first kernel
   uint32_t magic_k, magic_v;
   bool single;    // a CTA per unit, no second kernel
   bool vec_q;     // query rows start on 16-byte boundaries
-  int score_rows; // rows rounded up to even: the score buffer's row length
+  int score_rows; // 2, or rows rounded up to fours: the score buffer's row length
   float* parts;   // [grid][2][8 NT (D + 2)]: m, l, O of a piece
   float2* stats;  // [Z H row_tiles][8 NT]: m, l of units that one CTA held
   float* scores;  // [Z H][C][score_rows], in units of log2; null without weights
@@ -459,7 +458,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
       for (int e = tid; e < R * D; e += kWarps * 32) {
         const int row = row0 + e / D;
         if (row >= p.rows) break;
-        const size_t to = z * a.os[0] + (h * a.rep + row % a.rep) * a.os[1] + (a.tok0 + row / a.rep) * a.os[2] + e % D;
+        const size_t to = z * a.os[0] + (h * a.rep + row % a.rep) * a.os[1] + (row / a.rep) * a.os[2] + e % D;
         ((uint16_t*)a.out)[to] = 0;
       }
       if (p.scores) {
@@ -508,7 +507,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
     int least = INT_MAX;  // positions that every row sees
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int row = row0 + 8 * n + g, tok = a.tok0 + row / a.rep;
+      const int row = row0 + 8 * n + g, tok = row / a.rep;
       const bool live = row < p.rows && tok < sp.fresh;
       const uint16_t* q = (const uint16_t*)a.q + (live ? z * a.qs[0] + (h * a.rep + row % a.rep) * a.qs[1] + tok * a.qs[2] : 0) + t * (D / 4);
 #pragma unroll
@@ -525,7 +524,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int r = row0 + 8 * n + 2 * t + j, tk = a.tok0 + r / a.rep;
+        const int r = row0 + 8 * n + 2 * t + j, tk = r / a.rep;
         // rows that are not there see everything: nothing of them is used, and they must not keep the others from FULL
         st.limit[n][j] = r < p.rows && tk < sp.fresh ? sp.limit(a, tk) : INT_MAX;
         least = min(least, st.limit[n][j]);
@@ -589,7 +588,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
         oo.x += x.x * f, oo.y += x.y * f, oo.z += x.z * f, oo.w += x.w * f;
       }
       if (whole) {
-        const int tok = a.tok0 + row / a.rep;
+        const int tok = row / a.rep;
         const bool seen = sp.limit(a, tok) > 0;
         const float inv = 1.f / ll, y[4] = {seen ? oo.x * inv : 0.f, seen ? oo.y * inv : 0.f, seen ? oo.z * inv : 0.f, seen ? oo.w * inv : 0.f};
         const size_t to = z * a.os[0] + (h * a.rep + row % a.rep) * a.os[1] + tok * a.os[2] + d;
@@ -615,7 +614,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
         for (int w = 1; w < kWarps; ++w) mm = fmaxf(mm, sm[w][tid]);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) ll += sl[w][tid] * (sm[w][tid] == -INFINITY ? 1.f : ex2(sm[w][tid] - mm));
-        const int tok = a.tok0 + tid / a.rep;
+        const int tok = tid / a.rep;
         const bool seen = tid < p.rows && sp.limit(a, tok) > 0;
         so[0][tid][0] = mm == -INFINITY ? 0.f : mm, so[0][tid][1] = seen ? 1.f / ll : 0.f;
         so[0][tid][2] = __int_as_float(seen ? sp.limit(a, tok) : 0);
@@ -638,6 +637,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
 // weights (the blocks behind them: kChunk positions of a head each).
 constexpr int kChunk = 1024;
 constexpr int kJoin = 256;  // threads
+
+// The scores of 4 rows (2, if there are no more) from the first one's.
+__device__ __forceinline__ float4 scores_of(const float* s, int score_rows) {
+  if (score_rows > 2) return *reinterpret_cast<const float4*>(s);
+  const float2 x = *reinterpret_cast<const float2*>(s);
+  return make_float4(x.x, x.y, 0.f, 0.f);
+}
 constexpr int kPer = (kGridMax + kJoin - 1) / kJoin;
 
 template <int D, int NT, bool FP16>
@@ -646,7 +652,8 @@ __global__ void __launch_bounds__(kJoin) rows_finish_kernel(RowsArgs p) {
   constexpr int kPart = R * (D + 2);
   __shared__ float sf[kGridMax];
   __shared__ float red[kJoin / 32], sums[kJoin];
-  __shared__ float sm[kRowsMax], sinv[kRowsMax];
+  __shared__ __align__(16) float sm[kWeightRows], sinv[kWeightRows];
+  __shared__ __align__(16) int seen_to[kWeightRows];
   const AttendArgs& a = p.a;
   const Cache& c = a.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -668,7 +675,7 @@ __global__ void __launch_bounds__(kJoin) rows_finish_kernel(RowsArgs p) {
   };
 
   if (!weigh) {
-    const int row = blockIdx.x % p.rows, u = row / R, r = row % R, tok = a.tok0 + row / a.rep;
+    const int row = blockIdx.x % p.rows, u = row / R, r = row % R, tok = row / a.rep;
     const size_t to = z * a.os[0] + (h * a.rep + row % a.rep) * a.os[1] + tok * a.os[2];
     const bool seen = sp.limit(a, tok) > 0;
     const long long first = before + ((long long)h * p.row_tiles + u) * cost;
@@ -744,15 +751,16 @@ __global__ void __launch_bounds__(kJoin) rows_finish_kernel(RowsArgs p) {
   for (int i = 0; i < kKeysPer; ++i) old[i] = j0 + tid + i * kJoin < j1 ? a.weights_in[(size_t)zh * c.C + j0 + tid + i * kJoin] : 0.f;
   wait_for_previous();
   const float* scores = p.scores + (size_t)zh * c.C * p.score_rows;
-  float4 ahead[kKeysPer];  // the scores of up to 4 rows, on their way before the rows' maxima are known
+  float4 x[kKeysPer];  // those of the first 4 rows are on their way before the rows' maxima are known
 #pragma unroll
   for (int i = 0; i < kKeysPer; ++i) {
     const int j = j0 + tid + i * kJoin;
-    ahead[i] = p.score_rows == 4 && j < min(j1, most) ? *reinterpret_cast<const float4*>(scores + (size_t)j * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    x[i] = j < min(j1, most) ? scores_of(scores + (size_t)j * p.score_rows, p.score_rows) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  for (int row = warp; row < p.rows; row += kJoin / 32) {
+  for (int row = warp; row < (p.rows + 3) / 4 * 4; row += kJoin / 32) {
     float mx = -INFINITY, l = 0.f;
-    const bool seen = tiles && sp.limit(a, a.tok0 + row / a.rep) > 0;
+    const int limit = tiles && row < p.rows ? sp.limit(a, row / a.rep) : 0;
+    const bool seen = limit > 0;
     if (seen) {
       const int u = row / R, r = row % R;
       const long long first = before + ((long long)h * p.row_tiles + u) * cost;
@@ -772,46 +780,47 @@ __global__ void __launch_bounds__(kJoin) rows_finish_kernel(RowsArgs p) {
         for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
       }
     }
-    if (lane == 0) sm[row] = mx == -INFINITY ? 0.f : mx, sinv[row] = seen ? 1.f / l : 0.f;
+    if (lane == 0) sm[row] = mx == -INFINITY ? 0.f : mx, sinv[row] = seen ? 1.f / l : 0.f, seen_to[row] = limit;
   }
   __syncthreads();
+  float add[kKeysPer] = {};
+  for (int row = 0; row < p.rows; row += 4) {
+    const float4 m = *reinterpret_cast<const float4*>(sm + row), w = *reinterpret_cast<const float4*>(sinv + row);
+    const int4 to = *reinterpret_cast<const int4*>(seen_to + row);
+#pragma unroll
+    for (int i = 0; i < kKeysPer; ++i) {
+      const int j = j0 + tid + i * kJoin;
+      if (row && j < min(j1, most)) x[i] = scores_of(scores + (size_t)j * p.score_rows + row, p.score_rows);
+    }
+#pragma unroll
+    for (int i = 0; i < kKeysPer; ++i) {
+      const int j = j0 + tid + i * kJoin;
+      if (j < to.x) add[i] += ex2(x[i].x - m.x) * w.x;
+      if (j < to.y) add[i] += ex2(x[i].y - m.y) * w.y;
+      if (j < to.z) add[i] += ex2(x[i].z - m.z) * w.z;
+      if (j < to.w) add[i] += ex2(x[i].w - m.w) * w.w;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < kKeysPer; ++i) {
     const int j = j0 + tid + i * kJoin;
-    if (j >= j1) break;
-    float add = 0.f;
-    if (j < most) {
-      const float* s = scores + (size_t)j * p.score_rows;
-      const float x[4] = {ahead[i].x, ahead[i].y, ahead[i].z, ahead[i].w};
-      if (p.score_rows == 4) {
-#pragma unroll
-        for (int row = 0; row < 4; ++row)
-          if (row < p.rows && j < sp.limit(a, a.tok0 + row / a.rep)) add += ex2(x[row] - sm[row]) * sinv[row];
-      } else {
-#pragma unroll 4
-        for (int row = 0; row < p.rows; ++row)
-          if (j < sp.limit(a, a.tok0 + row / a.rep)) add += ex2(s[row] - sm[row]) * sinv[row];
-      }
-    }
-    c.weight[(size_t)zh * c.C + j] = old[i] + add;
+    if (j < j1) c.weight[(size_t)zh * c.C + j] = old[i] + add[i];
   }
 }
 
 // ------------------------------------------------------------------ host
-static int tokens_per_launch(int rep, int N, bool weights) { return weights ? std::max(1, std::min(N, kRowsMax / rep)) : N; }
-
 struct RowsPlan {
   int nt, row_tiles, rows, score_rows;
   long long parts, stats, scores;  // floats
 };
 constexpr int kDevices = 64;  // as many as select_device knows
 
-static RowsPlan plan_rows(const Cache& c, int rep, int ntok, bool weights) {
+static RowsPlan plan_rows(const Cache& c, int rep, int N, bool weights) {
   RowsPlan p;
-  p.rows = rep * ntok;
+  p.rows = rep * N;
   p.nt = p.rows <= 8 ? 1 : 2;
   p.row_tiles = (p.rows + 8 * p.nt - 1) / (8 * p.nt);
-  p.score_rows = (p.rows + 1) / 2 * 2;
+  p.score_rows = p.rows <= 2 ? 2 : (p.rows + 3) / 4 * 4;
   p.parts = 2LL * kGridMax * 8 * p.nt * (c.D + 2);
   p.stats = weights ? 2LL * c.Z * c.H * p.row_tiles * 8 * p.nt : 0;
   p.scores = weights ? (long long)c.Z * c.H * c.C * p.score_rows : 0;
@@ -819,8 +828,7 @@ static RowsPlan plan_rows(const Cache& c, int rep, int ntok, bool weights) {
 }
 
 size_t rows_workspace(const qflash_kv4_cache* c, int Hq, int N, bool weights) {
-  const int rep = Hq / c->H, n = tokens_per_launch(rep, N, weights);
-  const RowsPlan p = plan_rows(view(c), rep, n, weights);
+  const RowsPlan p = plan_rows(view(c), Hq / c->H, N, weights);
   return (size_t)(p.parts + p.stats + p.scores) * 4;
 }
 
@@ -857,36 +865,25 @@ static int launch_rows(RowsArgs r, int dev, cudaStream_t s) {
   return check_launch("kv4 rows finish", grid);
 }
 
-int attend_rows(const AttendArgs& a0, bool fp16, void* ws, int dev, cudaStream_t s) {
-  const bool weights = a0.weights_in != nullptr;
-  const int step = tokens_per_launch(a0.rep, a0.N, weights);
-  const RowsPlan most = plan_rows(a0.c, a0.rep, step, weights);
-  for (int t0 = 0; t0 < a0.N; t0 += step) {
-    RowsArgs r;
-    r.a = a0;
-    r.a.tok0 = t0;
-    r.a.ntok = std::min(step, a0.N - t0);
-    if (t0 && weights) r.a.weights_in = a0.c.weight;  // the launches before this one have added theirs
-    const RowsPlan p = plan_rows(a0.c, a0.rep, r.a.ntok, weights);
-    r.rows = p.rows;
-    r.row_tiles = p.row_tiles;
-    r.score_rows = p.score_rows;
-    r.magic_k = fp16 ? kMagicFp16 : kMagicBf16;
-    r.magic_v = kMagicBf16;
-    r.vec_q = (((uintptr_t)a0.q | (a0.qs[0] * 2) | (a0.qs[1] * 2) | (a0.qs[2] * 2)) & 15) == 0;
-    r.parts = (float*)ws;
-    r.stats = (float2*)(r.parts + most.parts);
-    r.scores = weights ? r.parts + most.parts + most.stats : nullptr;
-    int rc;
-    if (a0.c.D == 64)
-      rc = p.nt == 1 ? (fp16 ? launch_rows<64, 1, true>(r, dev, s) : launch_rows<64, 1, false>(r, dev, s))
+int attend_rows(const AttendArgs& a, bool fp16, void* ws, int dev, cudaStream_t s) {
+  const bool weights = a.weights_in != nullptr;
+  const RowsPlan p = plan_rows(a.c, a.rep, a.N, weights);
+  RowsArgs r;
+  r.a = a;
+  r.rows = p.rows;
+  r.row_tiles = p.row_tiles;
+  r.score_rows = p.score_rows;
+  r.magic_k = fp16 ? kMagicFp16 : kMagicBf16;
+  r.magic_v = kMagicBf16;
+  r.vec_q = (((uintptr_t)a.q | (a.qs[0] * 2) | (a.qs[1] * 2) | (a.qs[2] * 2)) & 15) == 0;
+  r.parts = (float*)ws;
+  r.stats = (float2*)(r.parts + p.parts);
+  r.scores = weights ? r.parts + p.parts + p.stats : nullptr;
+  if (a.c.D == 64)
+    return p.nt == 1 ? (fp16 ? launch_rows<64, 1, true>(r, dev, s) : launch_rows<64, 1, false>(r, dev, s))
                      : (fp16 ? launch_rows<64, 2, true>(r, dev, s) : launch_rows<64, 2, false>(r, dev, s));
-    else
-      rc = p.nt == 1 ? (fp16 ? launch_rows<128, 1, true>(r, dev, s) : launch_rows<128, 1, false>(r, dev, s))
-                     : (fp16 ? launch_rows<128, 2, true>(r, dev, s) : launch_rows<128, 2, false>(r, dev, s));
-    if (rc) return rc;
-  }
-  return QFLASH_OK;
+  return p.nt == 1 ? (fp16 ? launch_rows<128, 1, true>(r, dev, s) : launch_rows<128, 1, false>(r, dev, s))
+                   : (fp16 ? launch_rows<128, 2, true>(r, dev, s) : launch_rows<128, 2, false>(r, dev, s));
 }
 
 }  // namespace kv4

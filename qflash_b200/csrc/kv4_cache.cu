@@ -39,7 +39,7 @@ struct Share {
     const long long group = 1LL << log_group;
     const unsigned x = (unsigned)((units + (kThreads >> log_group) - 1) / (kThreads >> log_group));
     const long long parts = (work + group * per_thread - 1) / (group * per_thread);
-    return dim3(x, (unsigned)std::min<long long>(std::min<long long>(parts, 65535), std::max(1u, blocks / x)));
+    return dim3(x, (unsigned)std::max(1LL, std::min<long long>(std::min<long long>(parts, 65535), blocks / x)));
   }
 };
 static Share share(long long work, long long units, int least) {
@@ -601,9 +601,9 @@ extern "C" int qflash_kv4_append(const qflash_kv4_cache* cache, const void* k, c
   if (N < 0) return set_err(QFLASH_ERR_ARG, "kv4 append: negative N");
   if (dtype != kF32 && dtype != kF16 && dtype != kBF16) return set_err(QFLASH_ERR_ARG, "kv4 append: dtype %d", dtype);
   if (2LL * cache->Z * cache->H * N >= 1LL << 31) return set_err(QFLASH_ERR_UNSUPPORTED, "kv4 append: 2^31 vectors or more");
-  if (cache->Z == 0 || N == 0) return QFLASH_OK;
-  if (!k || !v || !k_strides || !v_strides) return set_err(QFLASH_ERR_ARG, "kv4 append: null pointer");
-  if (k_strides[3] != 1 || v_strides[3] != 1) return set_err(QFLASH_ERR_ARG, "kv4 append: innermost (head-dim) stride must be 1");
+  if (cache->Z == 0 || (N == 0 && !at)) return QFLASH_OK;
+  if ((N && (!k || !v)) || !k_strides || !v_strides) return set_err(QFLASH_ERR_ARG, "kv4 append: null pointer");
+  if (N && (k_strides[3] != 1 || v_strides[3] != 1)) return set_err(QFLASH_ERR_ARG, "kv4 append: innermost (head-dim) stride must be 1");
   OnDevice on(cache);
   if (on.rc) return on.rc;
   const int dev = on.dev;
@@ -641,6 +641,8 @@ extern "C" int qflash_kv4_evict(const qflash_kv4_cache* from, const qflash_kv4_c
   if (from->Z != to->Z || from->H != to->H || from->D != to->D)
     return set_err(QFLASH_ERR_ARG, "kv4 evict: caches of %d x %d heads of %d and of %d x %d heads of %d", from->Z, from->H,
                    from->D, to->Z, to->H, to->D);
+  if (from->device >= 0 && to->device >= 0 && from->device != to->device)
+    return set_err(QFLASH_ERR_ARG, "kv4 evict: caches on devices %d and %d", from->device, to->device);
   if (budget < 1 || budget > to->capacity) return set_err(QFLASH_ERR_ARG, "kv4 evict: budget %d of a capacity of %d", budget, to->capacity);
   if (recent < 0 || recent > budget) return set_err(QFLASH_ERR_ARG, "kv4 evict: %d recent tokens of a budget of %d", recent, budget);
   if (from->Z == 0) return QFLASH_OK;
@@ -657,6 +659,13 @@ extern "C" int qflash_kv4_evict(const qflash_kv4_cache* from, const qflash_kv4_c
   OnDevice on(from);
   if (on.rc) return on.rc;
   const int dev = on.dev;
+  if (to->device != dev) {
+    int there = -1;
+    const int rc = select_device(to->k_codes, &there);  // which makes it the current one
+    if (there != dev) cudaSetDevice(dev);
+    if (rc) return rc;
+    if (there != dev) return set_err(QFLASH_ERR_ARG, "kv4 evict: caches on devices %d and %d", dev, there);
+  }
   const EvictArgs a = {view(from), view(to), budget, recent, kept};
   cudaStream_t s = (cudaStream_t)stream;
   // CTAs per head: as many as have SMs of their own, as long as each has some thousand positions
@@ -706,11 +715,13 @@ static int check_attend(const qflash_kv4_cache* cache, int dtype, int Hq, int N)
 //   8 heads of 4000 positions   64 rows 38 and 23, 256 rows 45 and 48
 //   64 heads of 4000            32 rows 62 and 48,  64 rows 63 and 85
 //   8 heads of 30000            64 rows 70 and 58, 128 rows 73 and 98
-// With weights the other kernel goes by groups of rows and stores their scores:
-//   8 heads of 4000             24 rows 53 and 32,  64 rows 54 and 106
+// With weights the other one also stores all scores and reads them back, this one computes them twice:
+//   8 heads of 4000 positions   33 rows 55 and 44,  48 rows 54 and 42,  64 rows 55 and 68
+//   64 heads of 4000            33 rows 165 and 106, 48 rows 166 and 118, 64 rows 168 and 154
+//   256 heads of 1000           33 rows 172 and 137, 48 rows 173 and 176, 64 rows 174 and 229
 static bool many_rows(const qflash_kv4_cache* c, int Hq, int N, bool weights) {
   const long long rows = (long long)Hq / c->H * N, passes = (rows + 15) / 16, positions = (long long)c->Z * c->H * c->capacity;
-  return weights ? rows > 32 : 2 * passes * positions > 800000 + 5 * positions;
+  return weights ? rows > kWeightRows : 2 * passes * positions > 800000 + 5 * positions;
 }
 
 static size_t attend_workspace(const qflash_kv4_cache* c, int Hq, int N, bool weights) {
@@ -731,6 +742,9 @@ extern "C" int qflash_kv4_attend(const qflash_kv4_cache* cache, const void* q, i
   if (cache->Z == 0 || N == 0) return QFLASH_OK;
   if (!q || !out || !q_strides || !out_strides) return set_err(QFLASH_ERR_ARG, "kv4 attend: null pointer");
   if (q_strides[3] != 1 || out_strides[3] != 1) return set_err(QFLASH_ERR_ARG, "kv4 attend: innermost (head-dim) stride must be 1");
+  const size_t weight_bytes = (size_t)cache->Z * cache->H * cache->capacity * 4;
+  if (weights_in && weights_in != cache->weight && overlap(weights_in, weight_bytes, cache->weight, weight_bytes))
+    return set_err(QFLASH_ERR_ARG, "kv4 attend: weights_in overlaps the cache's weights");
   const size_t need = attend_workspace(cache, Hq, N, weights_in != nullptr);
   if (!workspace || workspace_bytes < need)
     return set_err(QFLASH_ERR_ARG, "kv4 attend: workspace of %zu bytes, %zu are needed", workspace ? workspace_bytes : 0, need);
@@ -745,7 +759,6 @@ extern "C" int qflash_kv4_attend(const qflash_kv4_cache* cache, const void* q, i
   a.rep = Hq / cache->H, a.N = N, a.new_lens = new_lens, a.causal = causal;
   a.scale_log2e = (float)(scale * 1.4426950408889634);
   a.weights_in = weights_in;
-  a.tok0 = 0, a.ntok = N;
   return many_rows(cache, Hq, N, weights_in != nullptr) ? attend_prompt(a, dtype == kF16, workspace, dev, (cudaStream_t)stream)
                                  : attend_rows(a, dtype == kF16, workspace, dev, (cudaStream_t)stream);
 }

@@ -121,7 +121,7 @@ inline void launch_behind(void (*kernel)(A), dim3 grid, unsigned threads, cudaSt
 int check_cache(const qflash_kv4_cache* c, const char* what);
 int check_launch(const char* what, unsigned grid);
 
-// Attention of `ntok` tokens from token tok0 on; see qflash_kv4_attend.
+// See qflash_kv4_attend.
 struct AttendArgs {
   Cache c;
   const void* q;
@@ -132,18 +132,19 @@ struct AttendArgs {
   int causal;
   float scale_log2e;
   const float* weights_in;  // null: no weights are accumulated
-  int tok0, ntok;
 };
 
-// The rows of one sequence that a launch over tokens [tok0, tok0 + ntok) takes,
-// and how many stored tokens they see at most.
+// Rows (tokens x rep) up to which the kernel for few rows also adds up weights.
+constexpr int kWeightRows = 48;
+
+// The rows of one sequence, and how many stored tokens they see at most.
 struct Span {
   int len, fresh;  // stored tokens; rows of the query tensor that the sequence brings
   __device__ __forceinline__ int limit(const AttendArgs& a, int i) const {  // positions that token i sees
     return i >= fresh ? 0 : a.causal ? max(0, len - fresh + i + 1) : len;
   }
   __device__ __forceinline__ int most(const AttendArgs& a) const {
-    return a.tok0 >= fresh ? 0 : limit(a, min(fresh, a.tok0 + a.ntok) - 1);
+    return fresh ? limit(a, fresh - 1) : 0;
   }
 };
 __device__ __forceinline__ Span span_of(const AttendArgs& a, int z) {

@@ -846,3 +846,55 @@ def test_positions_behind_2_to_the_31_bytes():
     kept = cache.evict(4, 3, out=small)
     assert kept.tolist() == [[[77, C - 3, C - 2, C - 1]] * H]
     assert torch.equal(small.read(4, dtype=FP32)[0][:, :, 1:], k)
+
+
+def test_append_of_no_rows_takes_tokens_back():
+    cache = make_cache(3, 1, 20, 64, [20, 7, 0], garbage=False)
+    none = torch.empty(3, 1, 0, 64, dtype=BF16, device="cuda")
+    codes = cache.k_codes.clone()
+    cache.append(none, none)
+    assert cache.lens.tolist() == [20, 7, 0]
+    cache.append(none, none, at=torch.tensor([5, 7, 25], dtype=torch.int32, device="cuda"))
+    assert cache.lens.tolist() == [5, 7, 20] and torch.equal(cache.k_codes, codes)
+    with pytest.raises(OverflowError):
+        cache.check()
+
+
+def test_buffers_cannot_be_replaced_or_shared():
+    from qflash_b200 import KV4Cache
+    cache = make_cache(1, 1, 20, 64, [20])
+    with pytest.raises(AttributeError):
+        cache.weight = torch.zeros_like(cache.weight)
+    with pytest.raises(ValueError, match="different"):
+        KV4Cache(cache.k_codes, cache.k_codes, cache.k_param, cache.v_param, cache.weight, cache.lens)
+
+
+def test_out_must_not_be_the_query_or_expanded():
+    cache = make_cache(1, 2, 20, 64, [20])
+    q = torch.randn(1, 2, 3, 64, device="cuda").half()
+    with pytest.raises(ValueError, match="its own"):
+        cache.attend(q, out=q)
+    with pytest.raises(ValueError, match="its own"):
+        cache.attend(q, out=torch.empty(1, 2, 1, 64, dtype=q.dtype, device="cuda").expand_as(q))
+    both = torch.stack((q, q), dim=2)  # the query's rows between the output's
+    assert torch.equal(cache.attend(both[:, :, 0], out=both[:, :, 1]), cache.attend(q))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("C", [150, 1400])
+@pytest.mark.parametrize("rep, N", [(1, 1), (2, 1), (3, 1), (1, 5), (7, 1), (3, 3), (1, 11), (6, 3), (5, 6), (9, 4), (47, 1), (4, 12), (7, 7)])
+def test_weights_of_any_number_of_rows(rep, N, C, dtype):
+    """Scores are stored in twos or fours of rows, and read back as such; above 48 rows they are computed again."""
+    lens, new = [C - 1, 3, C // 2, 0], [N, min(N, 3), (N + 1) // 2, 0]
+    cache = make_cache(4, 2, C, 64, lens, seed=rep)
+    q = queries(4, 2 * rep, N, 64, dtype, seed=N)
+    want, spread, cols, size = attend64(cache, q, new, True)
+    start, before = torch.rand(4, 2, C, generator=gen(3), device="cuda"), cache.weight.clone()
+    out = cache.attend(q, new_lens=torch.tensor(new, dtype=torch.int32, device="cuda"), accumulate=True, weights=start)
+    close_out(out, want, spread, size, 64, C)
+    live = (torch.arange(C, device="cuda") < cache.lens[:, None])[:, None, :].expand(4, 2, C)
+    # as in test_attend: p by twice its score error, fp32 sums over the rows by half a step each
+    tol = (2 * score_error(size.max(), 64) + (rep * N + 2) * 2.0 ** -24) * cols + 2.0 ** -23 * (start.double() + cols) + 1e-30
+    off = (cache.weight.double() - start.double() - cols).abs()
+    assert ((off / tol)[live] <= 1).all(), (off / tol)[live].max()
+    assert same(cache.weight[~live], before[~live])

@@ -120,3 +120,21 @@ def test_handle_refuses_bad_buffers():
             KV4Cache(*b)
     with pytest.raises(ValueError, match="k_codes"):
         KV4Cache(torch.zeros(2, 16, 32, dtype=torch.uint8), *buffers()[1:])
+
+
+def test_handle_refuses_sizes_and_shared_buffers():
+    for shape in ((1, 0, 16), (1, 1, 0)):
+        with pytest.raises(ValueError, match="at least one"):
+            KV4Cache(torch.zeros(*shape, 32, dtype=torch.uint8), *buffers()[1:])
+    with pytest.raises(ValueError, match="at least one"):
+        KV4Cache(torch.zeros(1, dtype=torch.uint8).expand(1, 1, (1 << 24) + 1, 32), *buffers()[1:])
+    with pytest.raises(AttributeError):  # the calls go by the buffers' addresses
+        KV4Cache.weight.__set__(object.__new__(KV4Cache), None)
+
+
+def test_caches_on_two_devices_and_overlapping_weights():
+    lib, c = _lib.load(), cache()
+    big = 1 << 20
+    other = cache(k_codes=big, v_codes=2 * big, k_param=3 * big, v_param=4 * big, weight=5 * big, lens=6 * big, device=1)
+    refused(lib.qflash_kv4_evict(c, other, 4, 1, 16, None), b"devices")
+    refused(lib.qflash_kv4_attend(c, 16, 1, ST, 16, ST, 2, 1, None, 1.0, 1, c.weight + 4, 256, 1 << 40, None), b"overlaps")
