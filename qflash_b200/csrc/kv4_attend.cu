@@ -32,7 +32,16 @@
 // CTA holds whole is written by it; pieces go to the workspace with their
 // maximum and sum, and a second kernel joins them in order.  A unit counts for
 // kBegin tiles more than it has, for its queries and its output: without that a CTA
-// that got many units of a tile each was the last by far.
+// that got many units of a tile each was the last by far (16 ragged sequences of up to
+// 4321, weights: 25.6 us; with 1, 2 and 4 tiles 21.0, 20.5 and 22.5).
+//
+// Measured, rows_kernel alone, head dim 128, bf16: 8 heads x 8 rows of 131071 positions
+// (143 MB) 39 us, 3.7 TB/s; 32 ragged sequences of up to 8100 positions, 8 heads x 4 rows
+// (196 MB), 52 us, 3.8 TB/s.  Decoding bounds it: without the masks and subtractions
+// (a copy of the kernel) the latter takes 40 us, without the MMAs 52, and the copies into
+// shared memory alone take 26 for the former.  57 % of issue slots are used, and warps that
+// could issue wait for the arithmetic pipe as often as one issues.  So a pair of codes costs one lop3 (the exponent comes
+// with the mask, from a kernel argument that stays in a register) and one subtraction.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -632,6 +641,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
   }
 }
 
+// Begins while rows_kernel ends, adds about 6 us to a call, and 10 where it adds up weights:
+// bound by the latency of its chain of loads (lengths, the pieces' statistics, pieces).
+// Four rows' scores come in one load, and limits are taken out of the loop over positions: with
+// scalar loads and a division per row, 32 rows over 8 heads of 4000 positions took 62 us in all,
+// now 34.
 // Joins the pieces of units that several CTAs held and writes zeros for units
 // with nothing to see (a block per row of a unit), and adds the attention
 // weights (the blocks behind them: kChunk positions of a head each).

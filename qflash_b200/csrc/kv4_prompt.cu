@@ -26,6 +26,15 @@
 // head) units are numbered, each CTA takes an equal run, pieces of units are
 // joined by a second kernel.
 //
+// Measured, prompt_kernel alone: 2048 tokens over 8000 positions, 8 heads x 4, head dim
+// 128, bf16 (234 GFLOP) 293 us, 800 TFLOP/s, the tensor pipe active 35 % of the time; 4
+// ragged prompts of up to 2049 tokens, 6 heads x 2, head dim 64, fp16 62 us.  A pair of
+// tiles takes some 4900 cycles, of which the products 1560: what bounds it is the softmax
+// warps' chain per 32 columns (TMEM load, exponentials, conversion, TMEM store) with one
+// thread a row.  More instruction parallelism in it cost more than it gave: chunks unrolled or
+// two in turn 322 to 342 us, as the loops' instructions then outgrow their cache;
+// 3 decoding warps 411; separate warps for K's and V's codes 361 to 387.
+//
 // The attention weights need the rows' final maximum and sum, so a third kernel
 // forms S^T = K Q^T again, keys in rows, and adds up exp(S - m) / l along its
 // columns in a fixed order: no atomics.
@@ -803,6 +812,7 @@ out:
   if (warp == 12) tmem_dealloc(tmem, 512);
 }
 
+// Adds about 10 us to a call (reading the pieces back, 32 rows a block for parallel loads).
 // Joins units that several CTAs held: blockIdx.x < 8 grid: 32 rows of the unit that
 // run blockIdx.x / 8's beginning is the first to cut; the others write the
 // zeros of units with nothing to see.
@@ -886,8 +896,9 @@ struct WLayout {
 // Two CTAs (a cluster) per 128 positions of a head, with every other row tile each,
 // as the first positions of a prompt are seen by all its rows, one tile after
 // the other.  Warps 0-7 add up (two threads a position, for 64 columns of a tile
-// each), warps 8-11 bring query tiles, warp 12 issues the products.  What bounds it is exponentials, and with one thread a position the
-// latencies of 4 warps.
+// each), warps 8-11 bring query tiles, warp 12 issues the products.  Bound by the
+// exponentials; the 4 ragged prompts above take 42 us, with one CTA for 128 positions 57,
+// and with two query tiles in flight as well 80.
 template <int D, bool FP16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeigh, 2) prompt_weights_kernel(PromptArgs p) {
   using L = WLayout<D>;
