@@ -462,7 +462,8 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(EvictArgs a) {
       const unsigned bm = __ballot_sync(~0u, heavy), be = __ballot_sync(~0u, even);
       const uint32_t em = pm + __popc(bm & below), es = ps + __popc(be & below);
       // rank among the kept: heavier ones before, and equal ones before as far as they stay
-      if (heavy || (even && es < left)) kept[em + min(es, left)] = at(t, j);
+      // (never past `need`, unless the weights change meanwhile)
+      if ((heavy || (even && es < left)) && em + min(es, left) < (uint32_t)need) kept[em + min(es, left)] = at(t, j);
       pm += __popc(bm), ps += __popc(be);
     }
     __syncthreads();
@@ -491,6 +492,9 @@ __global__ void __launch_bounds__(kThreads) evict_move_kernel(EvictArgs a) {
   float w[kMove];
 #pragma unroll
   for (int k = 0; k < kMove; ++k) src[k] = i0 + k * G < a.budget ? a.kept[(size_t)zh * a.budget + i0 + k * G] : -1;
+#pragma unroll
+  for (int k = 0; k < kMove; ++k)
+    if (src[k] >= f.C) src[k] = -1;  // as kept is where weights changed meanwhile
 #pragma unroll
   for (int k = 0; k < kMove; ++k)
     if (src[k] >= 0) {

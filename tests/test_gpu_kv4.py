@@ -898,3 +898,31 @@ def test_weights_of_any_number_of_rows(rep, N, C, dtype):
     off = (cache.weight.double() - start.double() - cols).abs()
     assert ((off / tol)[live] <= 1).all(), (off / tol)[live].max()
     assert same(cache.weight[~live], before[~live])
+
+
+@pytest.mark.parametrize("Z, N, accumulate", [(3, 1, False), (3, 1, True), (3, 700, False), (40, 60, True), (70, 3, True), (1, 5000, False)])
+@pytest.mark.parametrize("empty", ["cache", "rows"])
+def test_attend_where_nothing_is_seen(Z, N, accumulate, empty):
+    lens = [0] * Z if empty == "cache" else [(31 * z) % 400 for z in range(Z)]
+    cache = make_cache(Z, 2, 400, 64, lens, seed=Z)
+    before = cache.weight.clone()
+    new = torch.zeros(Z, dtype=torch.int32, device="cuda") if empty == "rows" else None
+    q = queries(Z, 4, N, 64, BF16, seed=N)
+    out = torch.full_like(q, float("nan"))
+    cache.attend(q, new_lens=new, accumulate=accumulate, out=out)
+    assert not out.any() and same(cache.weight, before)
+    cache.check()
+
+
+def test_attend_prompts_of_many_sequences():
+    Z, N = 70, 40
+    lens = [(37 * z) % 300 for z in range(Z)]
+    cache = make_cache(Z, 1, 300, 64, lens, seed=2)
+    q, new = queries(Z, 2, N, 64, FP16, seed=5), [min(n, N - z % 20) for z, n in enumerate(lens)]
+    want, spread, cols, size = attend64(cache, q, new, True)
+    cache.weight.zero_()
+    out = cache.attend(q, new_lens=torch.tensor(new, dtype=torch.int32, device="cuda"), accumulate=True)
+    close_out(out, want, spread, size, 64, 300)
+    live = (torch.arange(300, device="cuda") < cache.lens[:, None])[:, None, :].expand(Z, 1, 300)
+    tol = (2 * score_error(size.max(), 64) + (2 * N + 4) * 2.0 ** -24) * cols + 1e-30
+    assert (((cache.weight.double() - cols).abs() / tol)[live] <= 1).all()
