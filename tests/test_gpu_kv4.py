@@ -926,3 +926,39 @@ def test_attend_prompts_of_many_sequences():
     live = (torch.arange(300, device="cuda") < cache.lens[:, None])[:, None, :].expand(Z, 1, 300)
     tol = (2 * score_error(size.max(), 64) + (2 * N + 4) * 2.0 ** -24) * cols + 1e-30
     assert (((cache.weight.double() - cols).abs() / tol)[live] <= 1).all()
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    """Devices, attributes and occupancies are asked for on a first call, which may be a captured one."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import torch
+from qflash_b200 import KV4Cache
+torch.manual_seed(1)
+make = lambda h, n: torch.randn(2, h, n, 64, device="cuda").bfloat16()
+cache, small = KV4Cache.empty(2, 2, 3000, 64), KV4Cache.empty(2, 2, 200, 64)
+k, v, q, piece = make(2, 2500), make(2, 2500), make(4, 1), make(4, 900)
+def step():
+    cache.lens.zero_()
+    cache.append(k, v)
+    outs = [cache.attend(q), cache.attend(q, accumulate=True), cache.attend(piece, accumulate=True)]
+    kept = cache.evict(100, 10, out=small)
+    return [*outs, kept, *small.read(150), small.attend(q)]
+side = torch.cuda.Stream()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=side):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+got = [x.clone() for x in got]
+cache.weight.fill_(7.0)
+assert all(torch.equal(x, y) for x, y in zip(got, step()))
+cache.check()
+small.check()
+print("same")
+"""
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                         cwd=Path(__file__).resolve().parents[1])
+    assert run.returncode == 0 and "same" in run.stdout, run.stderr[-2000:]
