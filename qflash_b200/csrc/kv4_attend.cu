@@ -6,10 +6,11 @@
 //
 // Scales stay outside the products: what the tensor cores multiply is the
 // queries (as given) with whole numbers -15..15, exact in bf16 and fp16, and
-// P vs with whole numbers.  P vs is rounded to bf16 once for bf16 queries
-// (half a step, 2^-8, like the output's own rounding); for fp16 queries it is
-// split into two bf16 terms (2^-16), since one would cost the output's last
-// three bits.
+// P vs with whole numbers.  P vs is split into two bf16 terms (together 16 bits, off
+// by 2^-16): bf16 because values' scales may lie anywhere in its range, two because one
+// (2^-8) would cost fp16 outputs their last three bits, and bf16 outputs as much as their own
+// rounding does (131071 positions: 0.0023 of the outputs' size against 0.0017).  The second
+// term costs 10 % for bf16 queries (131071 positions 39.4 -> 43.3 us).
 //
 // Both products are transposed, so that the cache is the MMA's A operand, decoded
 // straight into A fragments:
@@ -36,10 +37,10 @@
 // 4321, weights: 25.6 us; with 1, 2 and 4 tiles 21.0, 20.5 and 22.5).
 //
 // Measured, rows_kernel alone, head dim 128, bf16: 8 heads x 8 rows of 131071 positions
-// (143 MB) 39 us, 3.7 TB/s; 32 ragged sequences of up to 8100 positions, 8 heads x 4 rows
-// (196 MB), 52 us, 3.8 TB/s.  Decoding bounds it: without the masks and subtractions
-// (a copy of the kernel) the latter takes 40 us, without the MMAs 52, and the copies into
-// shared memory alone take 26 for the former.  57 % of issue slots are used, and warps that
+// (143 MB) 43 us, 3.3 TB/s; 32 ragged sequences of up to 8100 positions, 8 heads x 4 rows
+// (196 MB), 57 us, 3.4 TB/s.  Arithmetic bounds it.  With one term of P vs the latter took 52 us, then
+// 40 without the masks and subtractions (a copy of the kernel), 52 without the MMAs, and the copies into
+// shared memory alone take 26 for the former.  57 % of issue slots were used, and warps that
 // could issue wait for the arithmetic pipe as often as one issues.  So a pair of codes costs one lop3 (the exponent comes
 // with the mask, from a kernel argument that stays in a register) and one subtraction.
 #include <algorithm>
@@ -380,7 +381,7 @@ __device__ __forceinline__ void rows_step(RowsState<D, NT, FP16>& st, uint32_t s
       }
     }
   }
-  // P vs as B fragments [keys of 8][rows]
+  // P vs as B fragments [keys of 8][rows], the first terms and the second ones
   uint32_t ph[NT][4], pl[NT][4];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -399,10 +400,7 @@ __device__ __forceinline__ void rows_step(RowsState<D, NT, FP16>& st, uint32_t s
       }
       const uint32_t hi = pack_bf16(y[0], y[1]);
       ph[n][i] = transpose8(hi);
-      if (FP16) {
-        const uint32_t lo = pack_bf16(y[0] - __uint_as_float(hi << 16), y[1] - __uint_as_float(hi & 0xffff0000u));
-        pl[n][i] = transpose8(lo);
-      }
+      pl[n][i] = transpose8(pack_bf16(y[0] - __uint_as_float(hi << 16), y[1] - __uint_as_float(hi & 0xffff0000u)));
     }
   }
 #pragma unroll
@@ -425,7 +423,7 @@ __device__ __forceinline__ void rows_step(RowsState<D, NT, FP16>& st, uint32_t s
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           mma_bf16(st.o[n][2 * seg + i], af, ph[n][2 * ks], ph[n][2 * ks + 1]);
-          if (FP16) mma_bf16(st.o[n][2 * seg + i], af, pl[n][2 * ks], pl[n][2 * ks + 1]);
+          mma_bf16(st.o[n][2 * seg + i], af, pl[n][2 * ks], pl[n][2 * ks + 1]);
         }
       }
     }

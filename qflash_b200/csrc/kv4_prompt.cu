@@ -12,8 +12,9 @@
 //   2 x 4 warps do the softmax of a row tile each, a thread a row, and write P
 //     over S.  The two tiles take turns: one's products run under the other's
 //     softmax.
-// P vs goes to the tensor cores as bf16 for bf16 queries, as the sum of two bf16
-// terms for fp16 queries (half steps 2^-8 and 2^-16).  A tile's P is formed against
+// P vs goes to the tensor cores as the sum of two bf16 terms (off by 2^-16), for the
+// reasons given in the kernel for few rows; the second one costs bf16 queries 295 -> 355 us
+// for the prompt's piece below.  A tile's P is formed against
 // a reference from the tiles before it (at first the first tile's maximum), in one
 // pass that takes 32 columns at a time and overwrites them: P of any size costs no
 // bits in floating point.  Where a tile's P add up to more than 2^16 the reference is
@@ -27,7 +28,7 @@
 // joined by a second kernel.
 //
 // Measured, prompt_kernel alone: 2048 tokens over 8000 positions, 8 heads x 4, head dim
-// 128, bf16 (234 GFLOP) 293 us, 800 TFLOP/s, the tensor pipe active 35 % of the time; 4
+// 128, bf16 (234 GFLOP) 355 us, 660 TFLOP/s; with one term of P vs 295 us, the tensor pipe active 35 % of the time; 4
 // ragged prompts of up to 2049 tokens, 6 heads x 2, head dim 64, fp16 62 us.  A pair of
 // tiles takes some 4900 cycles, of which the products 1560: what bounds it is the softmax
 // warps' chain per 32 columns (TMEM load, exponentials, conversion, TMEM store) with one
@@ -292,7 +293,7 @@ __device__ __forceinline__ uint64_t k_desc(uint32_t word, int step) { return des
 __device__ __forceinline__ uint64_t mn_desc(uint32_t word, int step) { return desc_of(word + step * (16 * 128 / 16)); }
 
 // P's column for a step of 16 keys: 32 keys' first terms lie in the first 16 of their scores' 32 columns, the
-// second terms (fp16) behind them.
+// second terms behind them.
 __device__ __forceinline__ constexpr uint32_t p_col(int step) { return 32 * (step >> 1) + 8 * (step & 1); }
 
 // ------------------------------------------------------------------ work split
@@ -453,7 +454,7 @@ __device__ __noinline__ float first_reference(uint32_t s_at, const float4* ks, i
 // by a whole number (or from nothing to the first score), and scales O and the P of
 // this tile's chunks before q.  Returns the reference and what the sums are to be
 // multiplied by.  Out of line, as its registers would burden every tile's loop.
-template <int D, bool FP16>
+template <int D>
 __device__ __noinline__ float2 raise_reference(float m, uint32_t s_at, uint32_t o_at, const float4* ks, int q, int lim,
                                                bool high, bool first) {
   float x[32];
@@ -467,9 +468,9 @@ __device__ __noinline__ float2 raise_reference(float m, uint32_t s_at, uint32_t 
   tmem_wait_st();
   const uint32_t ff = pack_bf16(f, f);
 #pragma unroll 1
-  for (int e = 0; e < (FP16 ? 2 : 1) * q; ++e) {
+  for (int e = 0; e < 2 * q; ++e) {
     uint32_t y[16];
-    const uint32_t at = FP16 ? s_at + 16 * e : s_at + 32 * e;
+    const uint32_t at = s_at + 16 * e;
     tmem_ld16(at, y);
 #pragma unroll
     for (int i = 0; i < 16; ++i) asm("mul.bf16x2 %0, %0, %1;" : "+r"(y[i]) : "r"(ff));
@@ -484,7 +485,7 @@ __device__ __noinline__ float2 raise_reference(float m, uint32_t s_at, uint32_t 
 // For the same reason no maximum stands before the exponentials: their sum says
 // afterwards, before P is stored, whether the reference is still good enough, and
 // what it has to become.
-template <int D, bool FP16, bool FULL>
+template <int D, bool FULL>
 __device__ __forceinline__ void softmax_tile(RowState& r, uint32_t s_at, uint32_t o_at, const float4* ks, const float4* vs,
                                              int lim, bool first) {
   if (first) {
@@ -522,18 +523,16 @@ __device__ __forceinline__ void softmax_tile(RowState& r, uint32_t s_at, uint32_
     uint32_t hi[16], lo[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) hi[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
-    if (FP16) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        add2(x[2 * i], x[2 * i + 1], -__uint_as_float(hi[i] << 16), -__uint_as_float(hi[i] & 0xffff0000u));
-        lo[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
-      }
+    for (int i = 0; i < 16; ++i) {
+      add2(x[2 * i], x[2 * i + 1], -__uint_as_float(hi[i] << 16), -__uint_as_float(hi[i] & 0xffff0000u));
+      lo[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
     }
     // Too large to go on with (or, for a row without a score above -inf so far, not to be judged by the sum):
     // the chunk again, against a higher reference.  Asked only here, so that nothing above waits for the answer.
     const bool high = !raised && (sum > 1.8446744e19f || (r.m == -INFINITY && lim > 32 * q));  // 2^64
     if (__any_sync(~0u, high)) {
-      const float2 up = raise_reference<D, FP16>(r.m, s_at, o_at, ks, q, lim, high, first);
+      const float2 up = raise_reference<D>(r.m, s_at, o_at, ks, q, lim, high, first);
       r.m = up.x;
       r.l *= up.y, total *= up.y;
       raised = true;
@@ -543,7 +542,7 @@ __device__ __forceinline__ void softmax_tile(RowState& r, uint32_t s_at, uint32_
     raised = false;
     total += sum;
     tmem_st16(s_at + 32 * q, hi);
-    if (FP16) tmem_st16(s_at + 32 * q + 16, lo);
+    tmem_st16(s_at + 32 * q + 16, lo);
   }
   r.l += total;
   tmem_wait_st();
@@ -648,9 +647,9 @@ __global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
         const float4* vs = reinterpret_cast<const float4*>(vs_ring + (n & (kRing - 1)) * kKeys);
         const int lim = limit - j * kKeys;
         if (__all_sync(~0u, lim >= kKeys))
-          softmax_tile<D, FP16, true>(r, s_at, o_at, ks, vs, lim, j == w.t0);
+          softmax_tile<D, true>(r, s_at, o_at, ks, vs, lim, j == w.t0);
         else
-          softmax_tile<D, FP16, false>(r, s_at, o_at, ks, vs, lim, j == w.t0);
+          softmax_tile<D, false>(r, s_at, o_at, ks, vs, lim, j == w.t0);
         tc_fence_before();
         warp_arrive(p_full(t));
       }
@@ -776,7 +775,7 @@ __global__ void __launch_bounds__(kPrompt, 1) prompt_kernel(PromptArgs p) {
 #pragma unroll
               for (int s = 0; s < 4; ++s) {
                 mma_ts(to, from + 64 * b + p_col(s), mn_desc(vw + 512 * b, s), IO, s > 0 ? 1 : more | b, lane == 0);
-                if (FP16) mma_ts(to, from + 64 * b + 16 + p_col(s), mn_desc(vw + 512 * b, s), IO, 1, lane == 0);
+                mma_ts(to, from + 64 * b + 16 + p_col(s), mn_desc(vw + 512 * b, s), IO, 1, lane == 0);
               }
             if (j + 1 < tiles) {
               scores(t, n + 1);
