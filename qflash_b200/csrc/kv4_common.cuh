@@ -50,22 +50,14 @@ __device__ __forceinline__ __half from_float<__half>(float x) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// 8 fp32 numbers from a 16-byte boundary.  Plain loads, not the read-only path: what a kernel launched by
+// launch_behind reads of the one before it is still being written when it begins.
+__device__ __forceinline__ void read8(const float* p, float (&x)[8]) {  // on a 16-byte boundary
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
 // 8 elements of one thread, as one or two 16-byte transfers where `vec` says
 // that every row starts on a 16-byte boundary, else one by one.
-template <class T>
-__device__ __forceinline__ void load8(const T* p, bool vec, float (&x)[8]) {
-  alignas(16) T r[8];
-  if (vec) {
-    uint4* w = reinterpret_cast<uint4*>(r);
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = p[i];
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = to_float(r[i]);
-}
 template <class T>
 __device__ __forceinline__ void store8(T* p, bool vec, const float (&x)[8]) {
   alignas(16) T r[8];

@@ -859,13 +859,13 @@ __global__ void __launch_bounds__(256) prompt_finish_kernel(PromptArgs p) {
     if (row >= p.rows) break;
     const float* part = p.parts + (size_t)first * kPart;
     float m = part[r], l = part[kRows + r], o[8];
-    load8(part + 2 * kRows + r * D + col, true, o);
+    read8(part + 2 * kRows + r * D + col, o);
     for (int q = k; q < grid && run_begin(total, grid, q) < end; ++q) {
       part = p.parts + (size_t)2 * q * kPart;
       const float pm = part[r], pl = part[kRows + r], mx = fmaxf(m, pm);
       const float f0 = m == -INFINITY ? 1.f : ex2(m - mx), f1 = pm == -INFINITY ? 1.f : ex2(pm - mx);
       float x[8];
-      load8(part + 2 * kRows + r * D + col, true, x);
+      read8(part + 2 * kRows + r * D + col, x);
       l = l * f0 + pl * f1;
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] = o[i] * f0 + x[i] * f1;
