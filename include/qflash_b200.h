@@ -311,7 +311,8 @@ int qflash_kv4_read(const qflash_kv4_cache* cache, void* k, void* v, int dtype, 
  * every stored position j becomes weights_in[j] + the sum over rows and query heads
  * of the probability that position j received.
  * `workspace` holds qflash_kv4_attend_workspace(...) bytes, 16-byte aligned, for this
- * call alone until it has run.
+ * call alone until it has run.  Up to 48 rows per key/value head (N * Hq / H) with weights keep
+ * scores there: 1 GB of them at most, or 4 bytes per row and position of one head where that is more.
  */
 int qflash_kv4_attend(const qflash_kv4_cache* cache, const void* q, int dtype, const int64_t q_strides[4], void* out,
                       const int64_t out_strides[4], int Hq, int N, const int32_t* new_lens, double scale, int causal,

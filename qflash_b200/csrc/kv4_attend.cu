@@ -69,7 +69,7 @@ struct RowsArgs {
   int score_rows; // 2, or rows rounded up to fours: the score buffer's row length
   float* parts;   // [grid][2][8 NT (D + 2)]: m, l, O of a piece
   float2* stats;  // [Z H row_tiles][8 NT]: m, l of units that one CTA held
-  float* scores;  // [Z H][C][score_rows], in units of log2; null without weights
+  float* scores;  // [Z H][C][score_rows] of a launch's sequences and heads, in units of log2; null without weights
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -823,8 +823,15 @@ __global__ void __launch_bounds__(kJoin) rows_finish_kernel(RowsArgs p) {
 // ------------------------------------------------------------------ host
 struct RowsPlan {
   int nt, row_tiles, rows, score_rows;
+  int zs, hs;  // sequences and heads of a launch: all, some sequences with all heads, or some heads of one
   long long parts, stats, scores;  // floats
 };
+// The scores that the weights are formed from take up to 192 bytes per position and head, more than
+// what is stored of them, and go by the capacity (lengths are known on the device only). So a call
+// takes sequences and heads in groups of so many bytes of scores, or one head at a time.  A group costs some
+// 25 us of launches and up to 50 of idle SMs at its end: 48 rows over 256 heads of 131072 positions (6.4 GB in all)
+// 10.5 ms without groups, 12.1 in groups of 256 MB, 10.9 of 1 GB; 0.20, 0.95 and 0.39 where only 300 are stored.
+constexpr long long kScoreBytes = 1LL << 30;
 constexpr int kDevices = 64;  // as many as select_device knows
 
 static RowsPlan plan_rows(const Cache& c, int rep, int N, bool weights) {
@@ -834,8 +841,11 @@ static RowsPlan plan_rows(const Cache& c, int rep, int N, bool weights) {
   p.row_tiles = (p.rows + 8 * p.nt - 1) / (8 * p.nt);
   p.score_rows = p.rows <= 2 ? 2 : (p.rows + 3) / 4 * 4;
   p.parts = 2LL * kGridMax * 8 * p.nt * (c.D + 2);
-  p.stats = weights ? 2LL * c.Z * c.H * p.row_tiles * 8 * p.nt : 0;
-  p.scores = weights ? (long long)c.Z * c.H * c.C * p.score_rows : 0;
+  const long long heads = std::max(1LL, kScoreBytes / (4LL * c.C * p.score_rows));  // of a group
+  p.zs = weights ? (int)std::min<long long>(c.Z, std::max(1LL, heads / c.H)) : c.Z;
+  p.hs = weights ? (int)std::min<long long>(c.H, heads) : c.H;
+  p.stats = weights ? 2LL * p.zs * p.hs * p.row_tiles * 8 * p.nt : 0;
+  p.scores = weights ? (long long)p.zs * p.hs * c.C * p.score_rows : 0;
   return p;
 }
 
@@ -877,11 +887,31 @@ static int launch_rows(RowsArgs r, int dev, cudaStream_t s) {
   return check_launch("kv4 rows finish", grid);
 }
 
+static int launch_rows(const RowsArgs& r, int nt, bool fp16, int dev, cudaStream_t s) {
+  if (r.a.c.D == 64)
+    return nt == 1 ? (fp16 ? launch_rows<64, 1, true>(r, dev, s) : launch_rows<64, 1, false>(r, dev, s))
+                   : (fp16 ? launch_rows<64, 2, true>(r, dev, s) : launch_rows<64, 2, false>(r, dev, s));
+  return nt == 1 ? (fp16 ? launch_rows<128, 1, true>(r, dev, s) : launch_rows<128, 1, false>(r, dev, s))
+                 : (fp16 ? launch_rows<128, 2, true>(r, dev, s) : launch_rows<128, 2, false>(r, dev, s));
+}
+
+// What of a call belongs to nz sequences from z on, and nh heads from h on (all heads, or one sequence).
+static AttendArgs group_of(AttendArgs a, int z, int nz, int h, int nh) {
+  const int64_t head = (int64_t)z * a.c.H + h, at = head * a.c.C;
+  for (int i = 0; i < 2; ++i) a.c.codes[i] += at * (a.c.D / 2), a.c.param[i] += at;
+  a.c.weight += at, a.c.lens += z;
+  a.q = (const uint16_t*)a.q + z * a.qs[0] + (int64_t)h * a.rep * a.qs[1];
+  a.out = (uint16_t*)a.out + z * a.os[0] + (int64_t)h * a.rep * a.os[1];
+  if (a.new_lens) a.new_lens += z;
+  if (a.weights_in) a.weights_in += at;
+  a.c.Z = nz, a.c.H = nh;
+  return a;
+}
+
 int attend_rows(const AttendArgs& a, bool fp16, void* ws, int dev, cudaStream_t s) {
   const bool weights = a.weights_in != nullptr;
   const RowsPlan p = plan_rows(a.c, a.rep, a.N, weights);
   RowsArgs r;
-  r.a = a;
   r.rows = p.rows;
   r.row_tiles = p.row_tiles;
   r.score_rows = p.score_rows;
@@ -891,11 +921,12 @@ int attend_rows(const AttendArgs& a, bool fp16, void* ws, int dev, cudaStream_t 
   r.parts = (float*)ws;
   r.stats = (float2*)(r.parts + p.parts);
   r.scores = weights ? r.parts + p.parts + p.stats : nullptr;
-  if (a.c.D == 64)
-    return p.nt == 1 ? (fp16 ? launch_rows<64, 1, true>(r, dev, s) : launch_rows<64, 1, false>(r, dev, s))
-                     : (fp16 ? launch_rows<64, 2, true>(r, dev, s) : launch_rows<64, 2, false>(r, dev, s));
-  return p.nt == 1 ? (fp16 ? launch_rows<128, 1, true>(r, dev, s) : launch_rows<128, 1, false>(r, dev, s))
-                   : (fp16 ? launch_rows<128, 2, true>(r, dev, s) : launch_rows<128, 2, false>(r, dev, s));
+  for (int z = 0; z < a.c.Z; z += p.zs)
+    for (int h = 0; h < a.c.H; h += p.hs) {
+      r.a = group_of(a, z, std::min(p.zs, a.c.Z - z), h, std::min(p.hs, a.c.H - h));
+      if (int rc = launch_rows(r, p.nt, fp16, dev, s)) return rc;
+    }
+  return QFLASH_OK;
 }
 
 }  // namespace kv4

@@ -29,3 +29,31 @@ def test_outputs_as_exact_as_their_type(rep, N, lens, D, dtype):
     close_to_the_rounding(cache.attend(q), want, spread, size, D, max(lens))
     if rep * N > 48:  # the kernel for many rows
         close_to_the_rounding(both_ways(cache, q)[0], want, spread, size, D, max(lens))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("Z, H, C, L, rep, N", [(5, 1, 1 << 23, 1500, 4, 4), (3, 2, 1 << 22, 1500, 8, 6), (1, 3, 1 << 23, 1500, 24, 2),
+                                           (5000, 2, 2000, 200, 4, 4)])
+def test_weights_of_large_caches(Z, H, C, L, rep, N, dtype):
+    """Caches whose scores are kept for some sequences, or some heads, at a time."""
+    from qflash_b200 import KV4Cache
+    D = 64
+    lens = [(397 * z + 700) % L for z in range(Z)]
+    lens[Z // 2] = 0
+    small = make_cache(Z, H, L, D, lens, seed=N, garbage=False)
+    cache = KV4Cache.empty(Z, H, C, D)
+    for name in ("k_codes", "v_codes", "k_param", "v_param", "weight"):
+        getattr(cache, name)[:, :, :L] = getattr(small, name)
+    cache.lens.copy_(small.lens)
+    new = [min(n, N - z % 2) for z, n in enumerate(lens)]
+    counts = torch.tensor(new, dtype=torch.int32, device="cuda")
+    q = queries(Z, H * rep, N, D, dtype, seed=Z)
+    start = cache.weight.clone()
+    out = cache.attend(q, new_lens=counts, accumulate=True)
+    want, spread, cols, size = attend64(small, q, new, True)
+    close_to_the_rounding(out, want, spread, size, D, L)
+    assert torch.equal(cache.weight[:, :, L:], start[:, :, L:])
+    # p by twice its score error, fp32 sums over the rows by half a step each
+    first = start[:, :, :L].double()
+    tol = (2 * score_error(size.max(), D) + (rep * N + 2) * 2.0 ** -24) * cols + 2.0 ** -23 * (first + cols)
+    assert ((cache.weight[:, :, :L].double() - first - cols).abs() <= tol).all()

@@ -2,6 +2,11 @@
 import re
 from pathlib import Path
 
+import pytest
+
+from qflash_b200 import _lib
+from test_kv4 import cache
+
 CSRC = Path(__file__).resolve().parents[1] / "qflash_b200" / "csrc"
 SOURCES = {p.name: re.sub(r"//[^\n]*", "", p.read_text()) for p in sorted(CSRC.glob("kv4_*"))}
 
@@ -40,3 +45,14 @@ def test_kernels_that_begin_early_read_what_is_being_written_by_plain_loads():
                 what = arguments(body, load.end())
                 assert not re.search(r"\b(?:parts?|stats|scores|kept)\b", what), f"{name}: {load.group()}{what}"
     assert found == 3
+
+
+@pytest.mark.parametrize("Z, H, C, D, rep, N", [
+    (32, 8, 131072, 128, 8, 6), (32, 8, 131072, 128, 8, 1), (1, 8, 1 << 24, 128, 4, 12), (1 << 14, 64, 2048, 64, 1, 16),
+    (1, 1, 1 << 24, 64, 48, 1)])
+def test_scores_kept_for_the_weights_are_bounded(Z, H, C, D, rep, N):
+    """They are kept for some sequences and heads at a time: 1 GB, or one head's where that is more."""
+    need = _lib.load().qflash_kv4_attend_workspace(cache(Z=Z, H=H, capacity=C, D=D), 1, H * rep, N, 1)
+    rows = (rep * N + 3) // 4 * 4
+    pieces, stats = 2 * 148 * 5 * 16 * (D + 2) * 4, 8 * Z * H * (rep * N + 15)
+    assert 0 < need <= max(1 << 30, 4 * C * rows) + pieces + stats
