@@ -1,8 +1,10 @@
 """The 4-bit key/value cache on the GPU where its precision, ranges and sizes end, against plain 64-bit forms."""
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_kv4 import BF16, FP16, HALF_STEP, attend64, both_ways, make_cache, queries, score_error
+from test_gpu_kv4 import (BF16, FP16, FP32, HALF_STEP, attend64, both_ways, gen, make_cache, pack, quantise, queries, same,
+                          score_error)
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +59,74 @@ def test_weights_of_large_caches(Z, H, C, L, rep, N, dtype):
     first = start[:, :, :L].double()
     tol = (2 * score_error(size.max(), D) + (rep * N + 2) * 2.0 ** -24) * cols + 2.0 ** -23 * (first + cols)
     assert ((cache.weight[:, :, :L].double() - first - cols).abs() <= tol).all()
+
+
+def kept64(cache, budget, recent):
+    """Positions that stay, for weights without NaN."""
+    w, kept = cache.weight.cpu().numpy(), np.full((*cache.shape[:2], budget), -1, np.int32)
+    for z, n in enumerate(cache.lens.tolist()):
+        for h in range(cache.shape[1]):
+            keep = np.arange(n)
+            if n > budget:
+                heavy = np.argsort(-w[z, h, :n - recent], kind="stable")[:budget - recent]
+                keep = np.concatenate((np.sort(heavy), np.arange(n - recent, n)))
+            kept[z, h, :len(keep)] = keep
+    return torch.from_numpy(kept).cuda()
+
+
+def check_evict(cache, budget, recent):
+    from qflash_b200 import KV4Cache
+    Z, H, _, D = cache.shape
+    to = KV4Cache.empty(Z, H, budget, D)
+    kept, want = cache.evict(budget, recent, out=to), kept64(cache, budget, recent)
+    assert torch.equal(kept, want) and torch.equal(to.lens, cache.lens.clamp(max=budget))
+    there, at = want >= 0, want.clamp(min=0).long()
+    for name in ("k_codes", "v_codes", "k_param", "v_param"):
+        src = getattr(cache, name)
+        rows = torch.gather(src, 2, at[..., None].expand(*at.shape, src.shape[-1]))
+        assert torch.equal(getattr(to, name)[there], rows[there])
+    assert torch.equal(to.weight[there], torch.gather(cache.weight, 2, at)[there])
+
+
+@pytest.mark.parametrize("Z, H, lens, budget, recent", [
+    (10, 8, None, 5001, 77),  # a CTA per head, two or three tiles of positions each
+    (1, 2, [300001], 7000, 1000),  # eight CTAs per head, three tiles each; two in the next
+    (1, 1, [140000], 69999, 0), (2, 1, [262144, 131073], 4096, 4095)])
+@pytest.mark.parametrize("kind", ["random", "equal", "few", "sparse"])
+def test_evict_over_several_tiles(Z, H, lens, budget, recent, kind):
+    """Counts of heavier and equal positions are carried from tile to tile and from CTA to CTA."""
+    lens = lens or [40000 - 1234 * z for z in range(Z)]
+    cache = make_cache(Z, H, max(lens), 64, lens, seed=budget, garbage=False)
+    g = gen(budget)
+    if kind == "equal":
+        cache.weight.fill_(0.5)
+    elif kind == "few":
+        cache.weight.copy_(torch.randint(0, 3, cache.weight.shape, generator=g, device="cuda"))
+    elif kind == "sparse":  # some hundred heavy positions, and ties among the others
+        cache.weight.mul_((torch.rand(cache.weight.shape, generator=g, device="cuda") < 0.004) * 2.0)
+    check_evict(cache, budget, recent)
+
+
+def test_evict_of_more_heads_than_a_grid_has_rows():
+    """Heads from 65536 on are moved by a launch of their own."""
+    Z, H, C = 1025, 64, 12
+    cache = make_cache(Z, H, C, 64, [(5 * z) % (C + 1) for z in range(Z)], seed=1, garbage=False)
+    check_evict(cache, 7, 2)
+
+
+def test_append_fp32_prompts():
+    """fp32 keys and values at a prompt's length, of which one in some ten thousand lies at a border between codes."""
+    from qflash_b200 import KV4Cache
+    N, D = 3001, 128
+    x = torch.randn(2, 3, N, 2 * D, generator=gen(4), device="cuda") * torch.exp(3 * torch.randn(2, 3, N, 1, generator=gen(5), device="cuda"))
+    x[:, :, ::2] = (x[:, :, ::2] * 8).round() / 8  # many of them do
+    cache = KV4Cache.empty(2, 3, N + 2, D)
+    cache.append(x[..., :D], x[..., D:], new_lens=torch.tensor([N, 1234], dtype=torch.int32, device="cuda"))
+    assert cache.lens.tolist() == [N, 1234]
+    for t, codes, param in ((x[..., :D], cache.k_codes, cache.k_param), (x[..., D:], cache.v_codes, cache.v_param)):
+        code, p = quantise(t)
+        for z, n in enumerate(cache.lens.tolist()):
+            assert torch.equal(codes[z, :, :n], pack(code)[z, :, :n]) and same(param[z, :, :n], p[z, :, :n])
+            assert not codes[z, :, n:].any() and not param[z, :, n:].any()
+    assert cache.read(5, dtype=FP32)[0].any()
+    cache.check()
