@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
   const int unit = blockIdx.x * (kThreads >> lg) + (threadIdx.x >> lg);
   const bool there = unit < a.share.units;
   const int kv = unit & 1, zh = min(unit, a.share.units - 1) >> 1, z = zh / c.H, h = zh - z * c.H;
-  const int base = a.at ? a.at[z] : c.lens[z];
+  const int base = a.at ? a.at[z] : length_of(c, z);
   const int fresh = there ? (a.new_lens ? min(max(a.new_lens[z], 0), a.N) : a.N) : 0;
   const T* x0 = (const T*)(kv ? a.x[1] : a.x[0]) + z * (kv ? a.st[1][0] : a.st[0][0]) + h * (kv ? a.st[1][1] : a.st[0][1]) + lane * 8;
   const int64_t x_step = kv ? a.st[1][2] : a.st[0][2];
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a) {
   __syncthreads();
   if (!last) return;
   for (int i = threadIdx.x; i < c.Z; i += kThreads) {
-    const int first = a.at ? a.at[i] : c.lens[i];
+    const int first = a.at ? a.at[i] : length_of(c, i);
     const long long end = (long long)first + (a.new_lens ? min(max(a.new_lens[i], 0), a.N) : a.N);
     if (first < 0 || end > c.C) atomicOr(&c.ctl[1], 1);
     c.lens[i] = (int)min(max(end, 0LL), (long long)c.C);

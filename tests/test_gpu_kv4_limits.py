@@ -3,8 +3,8 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_kv4 import (BF16, FP16, FP32, HALF_STEP, attend64, both_ways, gen, make_cache, pack, quantise, queries, same,
-                          score_error)
+from test_gpu_kv4 import (BF16, FP16, FP32, HALF_STEP, attend64, both_ways, gen, make_cache, pack, quantise, queries,
+                          same, score_error)
 
 pytestmark = pytest.mark.gpu
 
@@ -130,3 +130,33 @@ def test_append_fp32_prompts():
             assert not codes[z, :, n:].any() and not param[z, :, n:].any()
     assert cache.read(5, dtype=FP32)[0].any()
     cache.check()
+
+
+def test_append_and_evict_read_lengths_outside_the_cache_as_its_ends():
+    from qflash_b200 import KV4Cache
+    C, D, N = 20, 64, 8
+    k = torch.randn(4, 2, N, D, generator=gen(6), device="cuda").to(BF16)
+    cache, want = KV4Cache.empty(4, 2, C, D), KV4Cache.empty(4, 2, C, D)
+    cache.lens.copy_(torch.tensor([-5, 3, -2 ** 31, 0], dtype=torch.int32))
+    want.lens.copy_(torch.tensor([0, 3, 0, 0], dtype=torch.int32))
+    for c in (cache, want):
+        c.append(k, k.flip(2))
+        c.check()  # nothing was dropped
+    assert cache.lens.tolist() == [8, 11, 8, 8]
+    for name in ("k_codes", "v_codes", "k_param", "v_param", "weight", "lens"):
+        assert torch.equal(getattr(cache, name), getattr(want, name)), name
+    full = KV4Cache.empty(2, 2, C, D)
+    full.lens.copy_(torch.tensor([C + 7, 2 ** 31 - 1], dtype=torch.int32))
+    full.append(k[:2], k[:2], new_lens=torch.tensor([0, 0], dtype=torch.int32, device="cuda"))
+    full.check()
+    assert full.lens.tolist() == [C, C]
+    full.lens.fill_(C + 1)
+    full.append(k[:2], k[:2])
+    assert full.lens.tolist() == [C, C] and not full.k_codes.any()
+    with pytest.raises(OverflowError):
+        full.check()
+    cache.lens.copy_(torch.tensor([-5, C + 3, 2 ** 31 - 1, 4], dtype=torch.int32))
+    to = KV4Cache.empty(4, 2, 6, D)
+    kept = cache.evict(6, 2, out=to)
+    assert to.lens.tolist() == [0, 6, 6, 4]
+    assert (kept[0] == -1).all() and kept[1, 0, -2:].tolist() == [C - 2, C - 1] and kept[3, 0].tolist() == [0, 1, 2, 3, -1, -1]
