@@ -512,6 +512,13 @@ __global__ void __launch_bounds__(kThreads) evict_move_kernel(EvictArgs a) {
     }
 }
 
+// What attend leaves of the weights where it has no rows: those that it was given, for stored positions.
+__global__ void __launch_bounds__(kThreads) set_weights_kernel(Cache c, const float* from, int parts) {
+  const int zh = blockIdx.x / parts, len = length_of(c, zh / c.H);
+  const size_t head = (size_t)zh * c.C;
+  for (int j = blockIdx.x % parts * kThreads + threadIdx.x; j < len; j += parts * kThreads) c.weight[head + j] = from[head + j];
+}
+
 // ------------------------------------------------------------------ host
 int check_cache(const qflash_kv4_cache* c, const char* what) {
   if (!c) return set_err(QFLASH_ERR_ARG, "%s: null cache", what);
@@ -750,12 +757,21 @@ extern "C" int qflash_kv4_attend(const qflash_kv4_cache* cache, const void* q, i
                                  size_t workspace_bytes, void* stream) {
   if (int rc = check_attend(cache, dtype, Hq, N)) return rc;
   if (!std::isfinite(scale)) return set_err(QFLASH_ERR_ARG, "kv4 attend: scale is not finite");
-  if (cache->Z == 0 || N == 0) return QFLASH_OK;
-  if (!q || !out || !q_strides || !out_strides) return set_err(QFLASH_ERR_ARG, "kv4 attend: null pointer");
-  if (q_strides[3] != 1 || out_strides[3] != 1) return set_err(QFLASH_ERR_ARG, "kv4 attend: innermost (head-dim) stride must be 1");
+  if (cache->Z == 0) return QFLASH_OK;
   const size_t weight_bytes = (size_t)cache->Z * cache->H * cache->capacity * 4;
   if (weights_in && weights_in != cache->weight && overlap(weights_in, weight_bytes, cache->weight, weight_bytes))
     return set_err(QFLASH_ERR_ARG, "kv4 attend: weights_in overlaps the cache's weights");
+  if (N == 0) {
+    if (!weights_in || weights_in == cache->weight) return QFLASH_OK;
+    OnDevice on(cache);
+    if (on.rc) return on.rc;
+    const int parts = std::min((cache->capacity + kThreads * 16 - 1) / (kThreads * 16), 1024);
+    const unsigned grid = (unsigned)cache->Z * cache->H * parts;
+    set_weights_kernel<<<grid, kThreads, 0, (cudaStream_t)stream>>>(view(cache), weights_in, parts);
+    return check_launch("kv4 attend", grid);
+  }
+  if (!q || !out || !q_strides || !out_strides) return set_err(QFLASH_ERR_ARG, "kv4 attend: null pointer");
+  if (q_strides[3] != 1 || out_strides[3] != 1) return set_err(QFLASH_ERR_ARG, "kv4 attend: innermost (head-dim) stride must be 1");
   const size_t need = attend_workspace(cache, Hq, N, weights_in != nullptr);
   if (!workspace || workspace_bytes < need)
     return set_err(QFLASH_ERR_ARG, "kv4 attend: workspace of %zu bytes, %zu are needed", workspace ? workspace_bytes : 0, need);

@@ -160,3 +160,17 @@ def test_append_and_evict_read_lengths_outside_the_cache_as_its_ends():
     kept = cache.evict(6, 2, out=to)
     assert to.lens.tolist() == [0, 6, 6, 4]
     assert (kept[0] == -1).all() and kept[1, 0, -2:].tolist() == [C - 2, C - 1] and kept[3, 0].tolist() == [0, 1, 2, 3, -1, -1]
+
+
+def test_attend_of_no_rows_still_sets_the_weights():
+    """Weights of stored positions become those given plus nothing, as with rows that all see nothing."""
+    for lens in ([300, 0, 17], [5000, 4999, 1]):
+        cache = make_cache(3, 2, max(lens), 64, lens)
+        before, start = cache.weight.clone(), torch.rand(cache.weight.shape, generator=gen(3), device="cuda")
+        q = torch.empty(3, 4, 0, 64, dtype=BF16, device="cuda")
+        assert cache.attend(q, accumulate=True, weights=start).shape == q.shape
+        live = (torch.arange(max(lens), device="cuda") < cache.lens[:, None])[:, None, :].expand(cache.weight.shape)
+        assert torch.equal(cache.weight, torch.where(live, start, before))
+        cache.attend(q, accumulate=True)
+        cache.attend(q)
+        assert torch.equal(cache.weight, torch.where(live, start, before))
