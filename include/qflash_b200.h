@@ -307,6 +307,9 @@ int qflash_kv4_read(const qflash_kv4_cache* cache, void* k, void* v, int dtype, 
  * i < new_lens[z] (NULL: N) are the sequence's last tokens: with `causal`, row i sees
  * the positions up to lens[z] - new_lens[z] + i, else all lens[z].  Rows that see
  * nothing, and rows i >= new_lens[z], are written as zeros.
+ * Scores and P v are formed in fp32, before they are divided by the sum of P: scores, and every sum that leads
+ * to one, have to lie within fp32's range; vectors of values keep their precision if their largest element
+ * is 0 or between 2^-90 and 2^92.
  * With weights_in ([Z, H, capacity] fp32; cache->weight itself, or apart from it), cache->weight of
  * every stored position j becomes weights_in[j] + the sum over rows and query heads
  * of the probability that position j received.

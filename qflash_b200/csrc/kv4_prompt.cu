@@ -16,10 +16,11 @@
 // reasons given in the kernel for few rows; the second one costs bf16 queries 295 -> 355 us
 // for the prompt's piece below.  A tile's P is formed against
 // a reference from the tiles before it (at first the first tile's maximum), in one
-// pass that takes 32 columns at a time and overwrites them: P of any size costs no
+// pass that takes 32 columns at a time and overwrites them: P above 1 costs no
 // bits in floating point.  Where a tile's P add up to more than 2^16 the reference is
-// raised for the next; only sums above 2^64 stop the pass, and what the tile has so
-// far is scaled.
+// raised for the next; only sums of 32 above 2^32 stop the pass, and what the tile has so
+// far is scaled.  So the terms of an O are below 2^35 in all (2^34 of a tile that comes to that,
+// less than 2^16 from each of the up to 2^17 tiles before it), and values below 2^92 cannot overflow it.
 // The order of d within each 8 is 0 4 1 5 2 6 3 7 everywhere (codes d and d + 4
 // of a word come out of one mask): Q is stored so, and the epilogue undoes it.
 //
@@ -530,7 +531,7 @@ __device__ __forceinline__ void softmax_tile(RowState& r, uint32_t s_at, uint32_
     }
     // Too large to go on with (or, for a row without a score above -inf so far, not to be judged by the sum):
     // the chunk again, against a higher reference.  Asked only here, so that nothing above waits for the answer.
-    const bool high = !raised && (sum > 1.8446744e19f || (r.m == -INFINITY && lim > 32 * q));  // 2^64
+    const bool high = !raised && (sum > 4294967296.f || (r.m == -INFINITY && lim > 32 * q));  // 2^32
     if (__any_sync(~0u, high)) {
       const float2 up = raise_reference<D>(r.m, s_at, o_at, ks, q, lim, high, first);
       r.m = up.x;

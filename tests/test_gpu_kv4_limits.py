@@ -174,3 +174,39 @@ def test_attend_of_no_rows_still_sets_the_weights():
         cache.attend(q, accumulate=True)
         cache.attend(q)
         assert torch.equal(cache.weight, torch.where(live, start, before))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("N", [2, 60])
+@pytest.mark.parametrize("rising", [0, 30, 150, 300, 700])
+@pytest.mark.parametrize("power", [0, 40, 88, -88])
+def test_values_of_any_scale_under_rising_scores(power, rising, N, dtype):
+    """Probabilities are formed against a reference that lags behind where a CTA walks from tile to tile (so there are
+    more heads than CTAs); with the values' scale they must neither overflow nor vanish, in the kernels for few and for
+    many rows alike."""
+    D, H, n = 64, 160, 700
+    cache = make_cache(1, H, n, D, [n], garbage=False)
+    cache.v_param[..., 0] = (cache.v_param[..., 0].double() * 2.0 ** power).to(BF16)  # powers of two: exact
+    q = torch.zeros(1, H, N, D, dtype=dtype, device="cuda")
+    q[..., 0] = 1.0
+    cache.k_codes.fill_(0)
+    cache.k_codes[..., 0] = 1  # element 0 is the key's scale, the others 0
+    ramp = torch.arange(n, device="cuda") / n * rising * np.log(2)  # scores rise by 2^rising in all
+    jump = torch.where(torch.arange(n, device="cuda") % 64 == 37, 5.0 * (rising > 0), 0.0)
+    cache.k_param[..., 0], cache.k_param[..., 1] = (ramp + jump).bfloat16(), 0.0
+    want, spread, cols, size = attend64(cache, q, [N], True, 1.0)
+    # errors of scores stay below 1/8, where exp(x) - 1 < 1.07 x
+    assert 2 * score_error(size.max().item(), D) < 0.125
+    many, weight = both_ways(cache, q, scale=1.0)
+    outs = [cache.attend(q, scale=1.0), many]
+    cache.check()
+    for x in outs:
+        if dtype is FP16 and power > 0:  # beyond the type: infinity wherever the value surely is
+            sure = want.abs() > 2.0 ** 17 + 2.0 ** -8 * spread
+            assert sure.any() and not torch.isnan(x).any()
+            assert torch.equal(x[sure].double(), torch.sign(want[sure]) * torch.inf)
+        else:
+            close_to_the_rounding(x, want, spread * 1.1, size, D, n)
+    # p by twice its score error, fp32 sums over the rows by half a step each; what is below fp32's range counts as 0
+    tol = (1.1 * 2 * score_error(size.max(), D) + (N + 2) * 2.0 ** -24) * cols + N * 2.0 ** -126
+    assert ((weight.double() - cols).abs() <= tol).all()
