@@ -185,14 +185,16 @@ class KV4Cache:
     def check(self) -> None:
         """Raise OverflowError if an append since the last check dropped tokens
         outside [0, capacity), QFlashError if a wait inside a kernel gave up
-        (its output is then not valid).  Synchronises."""
+        (its output is then not valid; where both happened it says so).
+        Synchronises."""
         status = int(self._ctl[1].item())
         if status:
             self._ctl[1] = 0
+        dropped = f"tokens outside the cache's {self.shape[2]} positions were dropped"
         if status & 2:
-            raise _lib.QFlashError("a bounded wait inside an attention kernel gave up")
+            raise _lib.QFlashError("a bounded wait inside an attention kernel gave up" + (f"; {dropped}" if status & 1 else ""))
         if status & 1:
-            raise OverflowError(f"tokens outside the cache's {self.shape[2]} positions were dropped")
+            raise OverflowError(dropped)
 
     def _counts(self, name, t):
         if t is not None and (t.shape != self.shape[:1] or t.dtype != torch.int32 or t.device != self.device

@@ -3,8 +3,9 @@ import re
 from pathlib import Path
 
 import pytest
+import torch
 
-from qflash_b200 import _lib
+from qflash_b200 import KV4Cache, _lib
 from test_kv4 import cache
 
 CSRC = Path(__file__).resolve().parents[1] / "qflash_b200" / "csrc"
@@ -56,3 +57,21 @@ def test_scores_kept_for_the_weights_are_bounded(Z, H, C, D, rep, N):
     rows = (rep * N + 3) // 4 * 4
     pieces, stats = 2 * 148 * 5 * 16 * (D + 2) * 4, 8 * Z * H * (rep * N + 15)
     assert 0 < need <= max(1 << 30, 4 * C * rows) + pieces + stats
+
+
+def handle(**fields):
+    """A KV4Cache with CPU tensors in its fields, past the constructor's refusal of them."""
+    c = object.__new__(KV4Cache)
+    for name, value in fields.items():
+        setattr(c, name, value)
+    return c
+
+
+@pytest.mark.parametrize("status, error, words", [
+    (1, OverflowError, ["dropped"]), (2, _lib.QFlashError, ["gave up"]), (3, _lib.QFlashError, ["gave up", "dropped"])])
+def test_check_reports_all_that_happened(status, error, words):
+    c = handle(shape=(1, 1, 16, 64), _ctl=torch.tensor([0, status], dtype=torch.int32))
+    with pytest.raises(error) as e:
+        c.check()
+    assert all(w in str(e.value) for w in words)
+    c.check()  # reported once
