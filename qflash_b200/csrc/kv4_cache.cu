@@ -756,7 +756,8 @@ extern "C" int qflash_kv4_attend(const qflash_kv4_cache* cache, const void* q, i
                                  double scale, int causal, const float* weights_in, void* workspace,
                                  size_t workspace_bytes, void* stream) {
   if (int rc = check_attend(cache, dtype, Hq, N)) return rc;
-  if (!std::isfinite(scale)) return set_err(QFLASH_ERR_ARG, "kv4 attend: scale is not finite");
+  const float scale_log2e = (float)(scale * 1.4426950408889634);
+  if (!std::isfinite(scale_log2e)) return set_err(QFLASH_ERR_ARG, "kv4 attend: scale is not finite in fp32");
   if (cache->Z == 0) return QFLASH_OK;
   const size_t weight_bytes = (size_t)cache->Z * cache->H * cache->capacity * 4;
   if (weights_in && weights_in != cache->weight && overlap(weights_in, weight_bytes, cache->weight, weight_bytes))
@@ -784,7 +785,7 @@ extern "C" int qflash_kv4_attend(const qflash_kv4_cache* cache, const void* q, i
   a.q = q, a.out = out;
   for (int i = 0; i < 3; ++i) a.qs[i] = q_strides[i], a.os[i] = out_strides[i];
   a.rep = Hq / cache->H, a.N = N, a.new_lens = new_lens, a.causal = causal;
-  a.scale_log2e = (float)(scale * 1.4426950408889634);
+  a.scale_log2e = scale_log2e;
   a.weights_in = weights_in;
   return many_rows(cache, Hq, N, weights_in != nullptr) ? attend_prompt(a, dtype == kF16, workspace, dev, (cudaStream_t)stream)
                                  : attend_rows(a, dtype == kF16, workspace, dev, (cudaStream_t)stream);

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from qflash_b200 import KV4Cache, _lib
-from test_kv4 import cache
+from test_kv4 import BAD_ST, ST, cache, refused
 
 CSRC = Path(__file__).resolve().parents[1] / "qflash_b200" / "csrc"
 SOURCES = {p.name: re.sub(r"//[^\n]*", "", p.read_text()) for p in sorted(CSRC.glob("kv4_*"))}
@@ -75,3 +75,11 @@ def test_check_reports_all_that_happened(status, error, words):
         c.check()
     assert all(w in str(e.value) for w in words)
     c.check()  # reported once
+
+
+def test_attend_refuses_a_scale_beyond_fp32():
+    """It is held in fp32, as a factor of log2(e): one that is finite in fp64 alone would make every output NaN."""
+    lib = _lib.load()
+    for scale in (1e39, -1e39, 3e38, 1.7e308):
+        refused(lib.qflash_kv4_attend(cache(), 16, 1, ST, 16, ST, 2, 1, None, scale, 1, None, 256, 1 << 40, None), b"finite")
+    refused(lib.qflash_kv4_attend(cache(), 16, 1, BAD_ST, 16, ST, 2, 1, None, 2e38, 1, None, 256, 1 << 40, None), b"stride")
