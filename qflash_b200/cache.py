@@ -91,6 +91,8 @@ class KV4Cache:
         Z, H, _, D = self.shape
         if key.dim() != 4 or key.shape != value.shape or key.shape[:2] != (Z, H) or key.shape[3] != D:
             raise ValueError(f"key and value must be [{Z}, {H}, N, {D}], got {tuple(key.shape)}, {tuple(value.shape)}")
+        if key.shape[2] >= 1 << 31:
+            raise ValueError(f"{key.shape[2]} rows, 2^31 or more")
         if key.dtype not in _FLOATS or value.dtype != key.dtype:
             raise ValueError(f"key and value must be float32, float16 or bfloat16 of one dtype, got {key.dtype}, "
                              f"{value.dtype}")

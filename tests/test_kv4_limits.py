@@ -83,3 +83,12 @@ def test_attend_refuses_a_scale_beyond_fp32():
     for scale in (1e39, -1e39, 3e38, 1.7e308):
         refused(lib.qflash_kv4_attend(cache(), 16, 1, ST, 16, ST, 2, 1, None, scale, 1, None, 256, 1 << 40, None), b"finite")
     refused(lib.qflash_kv4_attend(cache(), 16, 1, BAD_ST, 16, ST, 2, 1, None, 2e38, 1, None, 256, 1 << 40, None), b"stride")
+
+
+def test_append_refuses_rows_that_the_library_cannot_count():
+    """2^32 + 1 rows, as an expanded tensor has them without memory, must not be taken for one."""
+    c = handle(shape=(1, 1, 16, 64), device=torch.device("cpu"), _ref=None, _index=0)
+    x = torch.zeros(1, 1, 1, 64)
+    for rows in ((1 << 32) + 1, 1 << 31):
+        with pytest.raises(ValueError, match="rows"):
+            c.append(x.expand(1, 1, rows, 64), x.expand(1, 1, rows, 64))
