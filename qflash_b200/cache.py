@@ -211,7 +211,11 @@ class KV4Cache:
 
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
-_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(device).cuda_stream without the object
+
+
+def _stream(index: int) -> int:
+    # torch.cuda.current_stream(device).cuda_stream without the object; looked up here, as builds of torch without CUDA lack it
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _inner(t: Tensor) -> Tensor:

@@ -1,5 +1,7 @@
 """The 4-bit key/value cache on the CPU: what its sources and host code have to hold to."""
 import re
+import subprocess
+import sys
 from pathlib import Path
 
 import pytest
@@ -92,3 +94,15 @@ def test_append_refuses_rows_that_the_library_cannot_count():
     for rows in ((1 << 32) + 1, 1 << 31):
         with pytest.raises(ValueError, match="rows"):
             c.append(x.expand(1, 1, rows, 64), x.expand(1, 1, rows, 64))
+
+
+def test_package_imports_without_a_cuda_build_of_torch():
+    code = """
+import torch
+for name in [n for n in dir(torch._C) if n.startswith("_cuda")]:
+    delattr(torch._C, name)
+import qflash_b200, qflash
+assert qflash.qflash and qflash.KV4Cache
+"""
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=CSRC.parents[1])
+    assert run.returncode == 0, run.stderr[-2000:]
