@@ -56,8 +56,6 @@ constexpr int kTile = 128;        // keys per CTA tile: 4 warps of 32
 constexpr int kWarps = 4;
 constexpr int kGridMax = 148 * 5;  // CTAs of one resident wave at most
 
-constexpr int kBegin = 2;
-
 struct RowsArgs {
   AttendArgs a;
   int rows;       // N * rep
@@ -72,16 +70,6 @@ struct RowsArgs {
   float* scores;  // [Z H][C][score_rows] of a launch's sequences and heads, in units of log2; null without weights
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float y;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-  return y;
-}
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -97,17 +85,11 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  uint32_t y;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
-  return y;
-}
 // Codes (low 4 bits of both halves) as numbers minus `zero`, exact: the code is
 // set into the mantissa of 128 (bf16) or 1024 (fp16), `zero` is 128 (1024) +
 // zero point.  `magic`, 128 or 1024 twice, comes from the kernel's arguments: as
 // a known constant it and the mask became an instruction each (lop3 takes one
 // immediate), and the integer pipe is what bounds this kernel.
-constexpr uint32_t kMagicBf16 = 0x43004300u, kMagicFp16 = 0x64006400u;
 template <bool FP16>
 __device__ __forceinline__ uint32_t code_pair(uint32_t x, uint32_t magic, uint32_t zero) {
   uint32_t m, y;
@@ -121,7 +103,7 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t x, uint32_t magic, uint32
 
 // A unit of a sequence that shows `most` positions: its tiles, and what it counts for.
 __device__ __forceinline__ int tiles_of(int most) { return (most + kTile - 1) / kTile; }
-__device__ __forceinline__ int cost_of(int most) { return most > 0 ? tiles_of(most) + kBegin : 0; }
+__device__ __forceinline__ int unit_cost(int most) { return cost_of(tiles_of(most)); }
 
 // The cost of all units before sequence z, and of all sequences.  One warp.
 __device__ __forceinline__ void cost_before(const RowsArgs& p, int z, long long* before, long long* total) {
@@ -129,7 +111,7 @@ __device__ __forceinline__ void cost_before(const RowsArgs& p, int z, long long*
   const long long units = (long long)p.a.c.H * p.row_tiles;
   long long blo = 0, ball = 0;
   for (int i = lane; i < p.a.c.Z; i += 32) {
-    const int t = cost_of(span_of(p.a, i).most(p.a));
+    const int t = unit_cost(span_of(p.a, i).most(p.a));
     ball += t;
     if (i < z) blo += t;
   }
@@ -149,7 +131,7 @@ __device__ __forceinline__ int sequence_of(const RowsArgs& p, long long at, long
   long long base = 0;
   for (int z0 = 0; z0 < p.a.c.Z; z0 += 32) {
     const int i = z0 + lane;
-    const long long mine = i < p.a.c.Z ? (long long)cost_of(span_of(p.a, i).most(p.a)) * units : 0;
+    const long long mine = i < p.a.c.Z ? (long long)unit_cost(span_of(p.a, i).most(p.a)) * units : 0;
     long long sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -185,7 +167,7 @@ __device__ __forceinline__ Place begin_of(const RowsArgs& p, int cta) {
     r.z = cta < r.grid ? sequence_of(p, r.at, &r.first) : p.a.c.Z;
     return r;
   }
-  const long long mine = lane < p.a.c.Z ? (long long)cost_of(span_of(p.a, lane).most(p.a)) * p.a.c.H * p.row_tiles : 0;
+  const long long mine = lane < p.a.c.Z ? (long long)unit_cost(span_of(p.a, lane).most(p.a)) * p.a.c.H * p.row_tiles : 0;
   long long sum = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -458,7 +440,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
   int piece = 0;  // the first piece of a CTA goes to slot 0, a later cut one (its last) to slot 1
   const int units = c.H * p.row_tiles;
   if (p.single) {
-    const int cost = cost_of(most);
+    const int cost = unit_cost(most);
     at = (long long)(blockIdx.x % units) * cost, stop = at + cost;
     if (most <= 0) {  // nothing to see
       const int row0 = (int)(blockIdx.x % p.row_tiles) * R, h = (int)(blockIdx.x % units) / p.row_tiles;
@@ -477,14 +459,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) rows_kernel(Rows
   }
   while (at < stop) {
     long long in_z = at - zfirst;
-    while (most <= 0 || in_z >= (long long)units * cost_of(most)) {  // on to the next sequence that shows anything
-      zfirst += (long long)units * cost_of(most);
+    while (most <= 0 || in_z >= (long long)units * unit_cost(most)) {  // on to the next sequence that shows anything
+      zfirst += (long long)units * unit_cost(most);
       in_z = at - zfirst;
       if (++z >= c.Z) return;
       sp = span_of(a, z);
       most = sp.most(a);
     }
-    const int tiles = tiles_of(most), cost = cost_of(most);
+    const int tiles = tiles_of(most), cost = unit_cost(most);
     const int unit = (int)(in_z / cost), u0 = (int)(in_z % cost);  // kBegin places, then the tiles
     const int u1 = (int)min((long long)cost, u0 + (stop - at)), t0 = max(0, u0 - kBegin), t1 = u1 - kBegin;
     at += u1 - u0;
@@ -676,7 +658,7 @@ __global__ void __launch_bounds__(kJoin) rows_finish_kernel(RowsArgs p) {
   const int chunks = (c.C + kChunk - 1) / kChunk;
   const int zh = weigh ? (blockIdx.x - joins) / chunks : blockIdx.x / p.rows, z = zh / c.H, h = zh % c.H;
   const Span sp = span_of(a, z);
-  const int most = sp.most(a), tiles = tiles_of(most), cost = cost_of(most);
+  const int most = sp.most(a), tiles = tiles_of(most), cost = unit_cost(most);
   long long before = 0, total = 0;
   if (tiles) cost_before(p, z, &before, &total);
   const int ctas = (int)min((long long)p.grid, total);
@@ -832,7 +814,6 @@ struct RowsPlan {
 // 25 us of launches and up to 50 of idle SMs at its end: 48 rows over 256 heads of 131072 positions (6.4 GB in all)
 // 10.5 ms without groups, 12.1 in groups of 256 MB, 10.9 of 1 GB; 0.20, 0.95 and 0.39 where only 300 are stored.
 constexpr long long kScoreBytes = 1LL << 30;
-constexpr int kDevices = 64;  // as many as select_device knows
 
 static RowsPlan plan_rows(const Cache& c, int rep, int N, bool weights) {
   RowsPlan p;

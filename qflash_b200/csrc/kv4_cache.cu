@@ -560,7 +560,6 @@ struct OnDevice {
   }
   OnDevice(const OnDevice&) = delete;
   OnDevice& operator=(const OnDevice&) = delete;
-  static constexpr int kDevices = 64;  // as many as select_device knows
   static std::atomic<bool>* seen() {  // devices that select_device has accepted
     static std::atomic<bool> s[kDevices];
     return s;

@@ -126,6 +126,32 @@ struct AttendArgs {
   const float* weights_in;  // null: no weights are accumulated
 };
 
+// Set into the mantissa of 128 (bf16) or 1024 (fp16), a code is a number.
+constexpr uint32_t kMagicBf16 = 0x43004300u, kMagicFp16 = 0x64006400u;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t y;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+  return y;
+}
+
+// What a unit of so many key tiles counts for where the attention kernels split their work: its queries
+// and its output take the time of kBegin tiles.
+constexpr int kBegin = 2;
+__device__ __forceinline__ int cost_of(int tiles) { return tiles ? tiles + kBegin : 0; }
+
+constexpr int kDevices = 64;  // as many as select_device knows
+
 // Rows (tokens x rep) up to which the kernel for few rows also adds up weights.
 constexpr int kWeightRows = 48;
 

@@ -124,16 +124,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]
                "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
                "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]));
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  uint32_t y;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
-  return y;
-}
 // pairs of fp32, one instruction for two
 __device__ __forceinline__ void mul2(float& a, float& b, float x, float y) {
   asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmul.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
@@ -151,11 +141,6 @@ __device__ __forceinline__ void fma2(float& a, float& b, float x, float y, float
       "fma.rn.f32x2 p, p, q, r;\n\tmov.b64 {%0, %1}, p;\n\t}"
       : "+f"(a), "+f"(b)
       : "f"(x), "f"(y), "f"(s), "f"(t));
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float y;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-  return y;
 }
 
 // Waits with a limit; after it (or another warp's) every role leaves its loops.
@@ -183,7 +168,6 @@ struct Waiter {
 // 8 codes as 4 words of two numbers code - zero, in the order 0 4, 1 5, 2 6, 3 7:
 // set into the mantissa of `magic`, 128 (bf16) or 1024 (fp16), which is a kernel
 // argument because lop3 takes one immediate and the mask is it.
-constexpr uint32_t kMagicBf16 = 0x43004300u, kMagicFp16 = 0x64006400u;
 template <bool FP16>
 __device__ __forceinline__ uint4 decode8(uint32_t w, uint32_t magic, uint32_t zero) {
   uint32_t y[4];
@@ -305,9 +289,6 @@ __device__ __forceinline__ int unit_tiles(const PromptArgs& p, int z, int rt) {
   const int first = rt * kRows / a.rep, last = min(min(a.N, sp.fresh), (rt * kRows + kRows - 1) / a.rep + 1);
   return first >= last ? 0 : (sp.limit(a, last - 1) + kKeys - 1) / kKeys;
 }
-// What a unit counts for in the split: its queries and its output take the time of kBegin tiles.
-constexpr int kBegin = 2;
-__device__ __forceinline__ int cost_of(int tiles) { return tiles ? tiles + kBegin : 0; }
 
 // Where a CTA is in its run.  All lanes of a warp hold the same.
 struct Walk {
@@ -1095,7 +1076,7 @@ static PromptArgs plan_prompt(const AttendArgs& a, bool weights, int sms, size_t
   return p;
 }
 
-constexpr int kSms = 148, kDevices = 64;  // as many as select_device knows
+constexpr int kSms = 148;
 
 size_t prompt_workspace(const qflash_kv4_cache* c, int Hq, int N, bool weights) {
   AttendArgs a;

@@ -106,3 +106,30 @@ assert qflash.qflash and qflash.KV4Cache
 """
     run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=CSRC.parents[1])
     assert run.returncode == 0, run.stderr[-2000:]
+
+
+def names_of(source):
+    """Functions, constants and structs that a source defines in its namespaces (indented lines are inside of something)."""
+    for line in source.split("\n"):
+        line = re.sub(r"^template <[^>]*>\s*", "", line)
+        if line.startswith(("static ", "namespace ", "extern ", "using ")):
+            continue
+        if m := re.match(r"struct (\w+) \{", line):
+            yield m.group(1)
+        elif line.startswith("constexpr ") and "(" not in line.split("=")[0]:
+            yield from re.findall(r"(\w+) =", line)
+        elif m := re.match(r"(?:__global__ void (?:__\w+__\([^()]*\) )*|[^\s#}][^;()]*\b)(\w+)\((?!\()", line):
+            yield m.group(1)
+
+
+def test_no_name_is_defined_in_two_sources():
+    """Two bodies of one inline function in a namespace make no valid program, whatever the build makes of them. (A
+    declaration in the header and its one definition are none.)"""
+    where = {}
+    for file, source in SOURCES.items():
+        for name in names_of(source):
+            where.setdefault(name, set()).add(file)
+    assert {"kTile", "kDigits", "Waiter", "to_float", "length_of", "append_kernel"} <= set(where)
+    declared = set(re.findall(r"^(?:int|size_t) (\w+)\([^;{]*;", SOURCES["kv4_common.cuh"], re.M))
+    twice = {n: sorted(files) for n, files in where.items() if len(files) > 1 and n not in declared}
+    assert not twice, twice
