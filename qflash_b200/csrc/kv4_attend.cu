@@ -38,11 +38,14 @@
 //
 // Measured, rows_kernel alone, head dim 128, bf16: 8 heads x 8 rows of 131071 positions
 // (143 MB) 43 us, 3.3 TB/s; 32 ragged sequences of up to 8100 positions, 8 heads x 4 rows
-// (196 MB), 57 us, 3.4 TB/s.  Arithmetic bounds it.  With one term of P vs the latter took 52 us, then
-// 40 without the masks and subtractions (a copy of the kernel), 52 without the MMAs, and the copies into
-// shared memory alone take 26 for the former.  57 % of issue slots were used, and warps that
-// could issue wait for the arithmetic pipe as often as one issues.  So a pair of codes costs one lop3 (the exponent comes
-// with the mask, from a kernel argument that stays in a register) and one subtraction.
+// (196 MB), 57 us, 3.4 TB/s.  Arithmetic bounds it, most of it on codes: when P vs had one term the latter
+// took 52 us, 40 without the masks and subtractions (a copy of the kernel), 52 without the MMAs, and the
+// copies into shared memory alone take 26 of the former's 43.  55 % of issue slots are used, and warps that
+// could issue wait for the arithmetic pipe as often as one issues.  A pair of codes costs one lop3 (the exponent comes
+// with the mask, from a kernel argument that stays in a register), one subtraction, and for three pairs of
+// four a shift.
+// Registers are capped for 4 CTAs an SM (3 where 16 rows are held); ptxas then spills 36 bytes of stores for
+// 8 rows of head dim 128, 16 for 8 rows of 64, and 336 for 16 rows of 128.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -851,9 +854,10 @@ static int launch_rows(RowsArgs r, int dev, cudaStream_t s) {
   }
   const long long units = (long long)c.Z * c.H * r.row_tiles, tiles = (c.C + kTile - 1) / kTile;
   // Short caches: a unit to a CTA, since joining costs a kernel; with longer ones, or few units that have their
-  // weights to add up, SMs would idle for too long.  One kernel and two, us at rep 4: 8 heads of 333 positions
-  // 5.2 and 8.1, of 1024 10.2 and 9.0 (which the launch saved makes up for), with weights 14.8 and 10.6; 128 heads of
-  // 1024 10.9 and 17.8, 512 heads 22.6 and 38.5; 8 heads of 2048 16.9 and 10.3.
+  // weights to add up, SMs would idle for too long.  One kernel and two, us at rep 4, bf16: 8 heads of 333 positions
+  // of 64 5.4 and 8.2; head dim 128, 8 heads of 512 7.6 and 9.1, of 1024 11.2 and 9.1 (which the launch saved makes up
+  // for), with weights 15.9 and 9.2; 128 heads of 1024 11.7 and 18.5, 512 heads 24.7 and 39.5; 8 heads of 2048 some
+  // 17 and 10.3.
   r.single = (tiles <= (r.scores && units < 64 ? 4 : 8) || (units >= 256 && tiles <= 16)) && (!r.scores || r.row_tiles == 1);
   if (r.single) {
     r.grid = (int)units;

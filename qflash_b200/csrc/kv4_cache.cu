@@ -728,14 +728,20 @@ static int check_attend(const qflash_kv4_cache* cache, int dtype, int Hq, int N)
 
 // Whether the kernel for many rows (R per key/value head) is the faster one.  It begins with
 // some 25 us more (128 decoded positions and 256 rows at a time), the other reads the
-// cache once per 16 rows.  us at head dim 128, this one and the other:
-//   8 heads of 4000 positions   64 rows 38 and 23, 256 rows 45 and 48
-//   64 heads of 4000            32 rows 62 and 48,  64 rows 63 and 85
-//   8 heads of 30000            64 rows 70 and 58, 128 rows 73 and 98
-// With weights the other one also stores all scores and reads them back, this one computes them twice:
-//   8 heads of 4000 positions   33 rows 55 and 44,  48 rows 54 and 42,  64 rows 55 and 68
-//   64 heads of 4000            33 rows 165 and 106, 48 rows 166 and 118, 64 rows 168 and 154
-//   256 heads of 1000           33 rows 172 and 137, 48 rows 173 and 176, 64 rows 174 and 229
+// cache once per 16 rows.  us of a call in a graph, bf16, this one and the other, at head dim 128 and at 64:
+//   8 heads of 4000 positions   128 rows 41 and 32, 256 rows 46 and 52  |  128 rows 30 and 23, 256 rows 33 and 37
+//   64 heads of 4000            32 rows 72 and 53, 64 rows 72 and 94, 128 rows 75 and 168  |  64 rows 64 and 66, 128 rows 64 and 116
+//   8 heads of 30000            64 rows 80 and 67, 128 rows 82 and 115  |  64 rows 65 and 40, 128 rows 65 and 68
+//   256 heads of 1000           64 rows 80 and 78, 128 rows 84 and 141  |  64 rows 69 and 40, 128 rows 69 and 73
+// The line drawn goes by positions alone, between the head dims' and the shapes' own; it is farthest off for
+// 64 rows over 64 heads of 4000 at head dim 128.  Positions are the capacity's, since lengths are known on the device
+// only: a large cache that holds little takes the kernel that its capacity would need.
+// With weights the other one also stores all scores and reads them back, this one computes them twice; up to 48
+// rows that other one is the faster or about equal everywhere, with more it depends:
+//   8 heads of 4000 positions   33 rows 55 and 45,  48 rows 56 and 48,  64 rows 56 and 68  |  48 rows 43 and 35, 64 rows 44 and 58
+//   64 heads of 4000            33 rows 175 and 109, 48 rows 175 and 124, 64 rows 176 and 161  |  48 rows 153 and 89, 64 rows 153 and 118
+//   8 heads of 30000            33 rows 174 and 98, 48 rows 174 and 117, 64 rows 175 and 151  |  48 rows 147 and 84, 64 rows 147 and 109
+//   256 heads of 1000           33 rows 182 and 144, 48 rows 183 and 184, 64 rows 183 and 238  |  48 rows 160 and 141, 64 rows 159 and 184
 static bool many_rows(const qflash_kv4_cache* c, int Hq, int N, bool weights) {
   const long long rows = (long long)Hq / c->H * N, passes = (rows + 15) / 16, positions = (long long)c->Z * c->H * c->capacity;
   return weights ? rows > kWeightRows : 2 * passes * positions > 800000 + 5 * positions;

@@ -29,13 +29,16 @@
 // joined by a second kernel.
 //
 // Measured, prompt_kernel alone: 2048 tokens over 8000 positions, 8 heads x 4, head dim
-// 128, bf16 (234 GFLOP) 355 us, 660 TFLOP/s; with one term of P vs 295 us, the tensor pipe active 35 % of the time; 4
-// ragged prompts of up to 2049 tokens, 6 heads x 2, head dim 64, fp16 62 us.  A pair of
-// tiles takes some 4900 cycles, of which the products 1560: what bounds it is the softmax
+// 128, bf16 (234 GFLOP) 355 us, 660 TFLOP/s, the tensor pipe active 46 % of the time; 4
+// ragged prompts of up to 2049 tokens, 6 heads x 2, head dim 64, fp16 63 us.  A pair of
+// tiles takes some 6700 cycles, of which its six products of 128 x 128 x 128 take 3072 (8192
+// operations a cycle) and its 32768 exponentials 2048 (16 a cycle): what bounds it is the softmax
 // warps' chain per 32 columns (TMEM load, exponentials, conversion, TMEM store) with one
-// thread a row.  More instruction parallelism in it cost more than it gave: chunks unrolled or
+// thread a row, and that products with V wait for the whole tile's P.  More instruction parallelism in
+// the chain cost more than it gave.  With one term of P vs, 291 us then: chunks unrolled or
 // two in turn 322 to 342 us, as the loops' instructions then outgrow their cache;
 // 3 decoding warps 411; separate warps for K's and V's codes 361 to 387.
+// ptxas spills 16 bytes of stores for head dim 128, and in prompt_weights_kernel 24 for 128 and 8 for 64.
 //
 // The attention weights need the rows' final maximum and sum, so a third kernel
 // forms S^T = K Q^T again, keys in rows, and adds up exp(S - m) / l along its
@@ -878,7 +881,7 @@ struct WLayout {
 // as the first positions of a prompt are seen by all its rows, one tile after
 // the other.  Warps 0-7 add up (two threads a position, for 64 columns of a tile
 // each), warps 8-11 bring query tiles, warp 12 issues the products.  Bound by the
-// exponentials; the 4 ragged prompts above take 42 us, with one CTA for 128 positions 57,
+// chain from TMEM load to exponentials and sums; the 4 ragged prompts above take 42 us, with one CTA for 128 positions 57,
 // and with two query tiles in flight as well 80.
 template <int D, bool FP16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWeigh, 2) prompt_weights_kernel(PromptArgs p) {
