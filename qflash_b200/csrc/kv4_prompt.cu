@@ -31,7 +31,7 @@
 // Measured, prompt_kernel alone: 2048 tokens over 8000 positions, 8 heads x 4, head dim
 // 128, bf16 (234 GFLOP) 355 us, 660 TFLOP/s, the tensor pipe active 46 % of the time; 4
 // ragged prompts of up to 2049 tokens, 6 heads x 2, head dim 64, fp16 63 us.  A pair of
-// tiles takes some 6700 cycles, of which its six products of 128 x 128 x 128 take 3072 (8192
+// tiles takes some 6700 cycles, of which its six products of 128 x 128 x 128 take 512 each (8192
 // operations a cycle) and its 32768 exponentials 2048 (16 a cycle): what bounds it is the softmax
 // warps' chain per 32 columns (TMEM load, exponentials, conversion, TMEM store) with one
 // thread a row, and that products with V wait for the whole tile's P.  More instruction parallelism in
